@@ -29,7 +29,8 @@ extern "C" {
 
 typedef void* papr_stream_t;
 
-enum { PAPR_ACT_NONE = 0, PAPR_ACT_RELU = 1, PAPR_ACT_LEAKY_RELU = 2 /* slope 0.2 */ };
+enum { PAPR_ACT_NONE = 0, PAPR_ACT_RELU = 1, PAPR_ACT_LEAKY_RELU = 2 /* slope 0.2 */,
+       PAPR_ACT_GELU = 3 /* erf form */, PAPR_ACT_SILU = 4 /* these two: papr_linear_* only */ };
 
 int papr_abi_version(void);
 const char* papr_last_error(void);
@@ -560,6 +561,62 @@ int32_t papr_get_switch(int32_t which);
 /* Waits for the recorded events, writes up to `cap` records (oldest first), clears the log and
  * returns the number of records that were pending. */
 int papr_profile_collect(papr_profile_record* out, int cap);
+
+/* ------------------------------------------------------------------------------------
+ * Row blocks (ABI 28): the parts of a residual feed-forward block -- FeedForward.forward of the reference, models/attn.py:111-117, with its
+ * `residual_ff` branch, and Linear layers of 16-bit rows -- as calls of their own.  Rows are float32, float16 or bfloat16 (PAPR_TYPE_*), arithmetic and
+ * sums float32, every output rounded once.  Row strides are in elements; rows need not be 16-byte aligned (odd widths and strides run on kernels with
+ * narrower loads).  Sums run in a fixed order: the same bits on every run.  Workspaces are the caller's, their contents irrelevant on entry; two calls
+ * that may run at the same time (other streams, captured graphs) need workspaces of their own. */
+enum { PAPR_TYPE_F32 = 0, PAPR_TYPE_F16 = 1, PAPR_TYPE_BF16 = 2 };
+
+/* Linear layer with its epilogue: y = act(x W^T + bias) + res, x (M, K), W (N, K), bias (N) or NULL, res (M, N) or NULL, y (M, N) contiguous.
+ * z (M, N) or NULL: receives x W^T + bias in the rows' type, what the backward pass of an activation reads (not needed for PAPR_ACT_NONE).
+ * Backward: with d_z = d_y act'(z):  d_x = d_z W (M, K),  d_w = d_z^T x (N, K),  d_b = column sums of d_z (N); each optional (NULL).  d_z is rounded to the
+ * rows' type in front of the two products.  keep != 0: x is rows kept in 8 bits (papr_rows8_pack; ldx in codes, exps its exponents) and d_w = d_z^T of the
+ * values they stand for.  M = 0: the forward call does nothing, the backward call is an error (the gradients are zero: the caller's).
+ * float32 rows: infinities give NaN.  workspace: papr_linear_bwd_workspace_bytes(desc) bytes. */
+enum { PAPR_KEEP_ROWS = 0, PAPR_KEEP_E4M3 = 1, PAPR_KEEP_INT8 = 2 };
+typedef struct { int32_t type, act, keep, reserved; int64_t M, N, K; } papr_linear_desc;
+int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ld_res,
+                    void* y, void* z, papr_stream_t stream);
+size_t papr_linear_bwd_workspace_bytes(const papr_linear_desc* d);
+int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64_t ld_dy, const void* z, const void* x, int64_t ldx, const void* exps, const void* w, int64_t ldw,
+                    void* d_x, void* d_w, void* d_b, void* workspace, papr_stream_t stream);
+
+/* Rows kept in 8 bits: 32 columns of a row share a scale 2^e, the smallest (e >= -120) with max|x| <= top 2^e, and hold x / 2^e rounded to nearest even as
+ * e4m3 (top 448) or int8 (top 127).  codes (rows, 32 ceil(width / 32)) bytes, padding zero; exps (rows, ceil(width / 32)) bytes = e + 127.  Magnitudes above
+ * 1.875 (e4m3) / 1.984375 (int8) times 2^15 (float16) / 2^127 (float32, bfloat16) are kept as that; NaN and infinities come back as NaN. */
+int papr_rows8_pack(int32_t type, int32_t fmt, const void* x, int64_t ldx, int64_t rows, int32_t width, void* codes, void* exps, papr_stream_t stream);
+int papr_rows8_unpack(int32_t type, int32_t fmt, const void* codes, const void* exps, int64_t rows, int32_t width, void* x, papr_stream_t stream);
+
+/* The joint of a residual block:  y = x + s a(g) N_post(f),  h = N_pre(y).  f NULL: y is x (not written), h = N_pre(x) -- the norm alone.
+ * N: PAPR_NORM_NONE v gain + shift, PAPR_NORM_LAYER (v - mean) / (std_unbiased + eps) gain + shift (models/attn.py:39-42; width >= 2),
+ * PAPR_NORM_RMS v / sqrt(mean v^2 + eps) gain + shift; gain and shift (width) or NULL, of one type.  s: scale_cols (width) or the number `scale`.
+ * gate: (rows, width), one per row (rows, 1), or absent; a = identity, sigmoid, silu.  y, h (rows, width) contiguous, either may be NULL.
+ * stats (rows, 6) floats or NULL: what papr_join_bwd reads.  Backward: d_y, d_h (rows, width) contiguous, one may be NULL; d_x, d_f (rows, width), d_g (like the
+ * gate, contiguous) and the parameters' gradients (in the parameters' types; g and each of its members optional).
+ * workspace: papr_join_bwd_workspace_bytes(rows, width) bytes where a parameter's gradient is asked for.  width <= PAPR_JOIN_MAX_WIDTH. */
+enum { PAPR_NORM_NONE = 0, PAPR_NORM_LAYER = 1, PAPR_NORM_RMS = 2 };
+enum { PAPR_GATE_NONE = 0, PAPR_GATE_SIGMOID = 1, PAPR_GATE_SILU = 2 };                       /* gate_act */
+enum { PAPR_GATE_ABSENT = 0, PAPR_GATE_ROW = 1, PAPR_GATE_FULL = 2 };                         /* gate_form */
+#define PAPR_JOIN_MAX_WIDTH 8192
+typedef struct { int32_t kind, type; float eps; int32_t reserved; const void* gain; const void* shift; } papr_block_norm;
+typedef struct {
+    int64_t rows;
+    int32_t width, type;
+    const void* x; int64_t ldx;
+    const void* f; int64_t ldf;
+    const void* gate; int64_t ldg;
+    int32_t gate_form, gate_act;
+    const void* scale_cols; int32_t scale_type; float scale;
+    papr_block_norm post, pre;
+} papr_join_desc;
+typedef struct { void* pre_gain; void* pre_shift; void* post_gain; void* post_shift; void* scale_cols; } papr_join_grads;
+int papr_join_fwd(const papr_join_desc* d, void* y, void* h, float* stats, papr_stream_t stream);
+size_t papr_join_bwd_workspace_bytes(int64_t rows, int32_t width);
+int papr_join_bwd(const papr_join_desc* d, const float* stats, const void* d_y, const void* d_h, void* d_x, void* d_f, void* d_g, const papr_join_grads* g,
+                  void* workspace, papr_stream_t stream);
 
 #ifdef __cplusplus
 }

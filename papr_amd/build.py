@@ -11,7 +11,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libpapr_hip.so")
-SOURCES = ["error.hip", "knn.hip", "cloud.hip", "features.hip", "pairs.hip", "rowops.hip", "gemm.hip", "chain4.hip", "conv.hip", "unet.hip", "small_unet.hip", "adam.hip"]
+SOURCES = ["error.hip", "knn.hip", "cloud.hip", "features.hip", "pairs.hip", "rowops.hip", "gemm.hip", "chain4.hip", "conv.hip", "unet.hip", "small_unet.hip", "adam.hip", "linear.hip", "join.hip", "rows8.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics",
          "-Wall", "-Wno-unused-function", "-Wno-inline-asm"]
 # chain4.hip: no packed-fp32 VALU (v_pk_mul_f32 / v_pk_add_f32 come from the SLP vectoriser).  Measured on MI355X (round 2,
@@ -19,7 +19,9 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
 # products for a few rows per launch, non-deterministically (packed fp32 runs on the matrix pipe); the same source built with
 # -fno-slp-vectorize is bit-identical to the reference kernel on every run.  Packed fp32 beside MFMAs is also slower
 # (MI355X_MICROARCH.md, "price of one filler beside MFMAs").
-EXTRA_FLAGS = {"chain4.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"]}
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]      # (the same caution by target feature: the host pass warns that it does not know it)
+EXTRA_FLAGS = {"chain4.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"],
+               "linear.hip": NO_PACKED_FP32, "join.hip": NO_PACKED_FP32, "rows8.hip": NO_PACKED_FP32}
 # chain4.hip keeps its weight fragments in a[0:127] by name, from inline asm; the compiler does not know they are taken in between
 # and moves values of its own into AGPRs when it runs out of VGPRs.  A build whose device code holds any v_accvgpr_* is wrong.
 NO_ACCVGPR = ["chain4.hip"]
@@ -95,7 +97,7 @@ def _stale(target, deps):
 
 def build_library(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    headers = [os.path.join(CSRC, h) for h in ("papr_common.h", "h3_common.h", "unet_parts.h", "chain.h", "chain4_kloop.inc", "chain4_fused.inc", "chain4_krun.inc")] + [os.path.join(os.path.dirname(PKG), "include", "papr_hip.h")]
+    headers = [os.path.join(CSRC, h) for h in ("papr_common.h", "block_types.h", "h3_common.h", "unet_parts.h", "chain.h", "chain4_kloop.inc", "chain4_fused.inc", "chain4_krun.inc")] + [os.path.join(os.path.dirname(PKG), "include", "papr_hip.h")]
     objdir = os.path.join(PKG, "build")
     os.makedirs(objdir, exist_ok=True)
     objs, procs = [], []

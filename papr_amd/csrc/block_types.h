@@ -1,0 +1,67 @@
+// Element types of the row-block operators (linear.hip, join.hip, rows8.hip): rows in float32, float16 or bfloat16, arithmetic in float32.
+#pragma once
+#include "papr_common.h"
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) papr_pack { T v[N]; };
+
+// the row types behind the PAPR_TYPE_* codes: the statement sees the type as T
+#define PAPR_TYPE_SWITCH(code, ...)                                                   \
+    do {                                                                              \
+        if ((code) == PAPR_TYPE_F32) { typedef float T; __VA_ARGS__; }                \
+        else if ((code) == PAPR_TYPE_F16) { typedef f16 T; __VA_ARGS__; }             \
+        else { typedef bf16 T; __VA_ARGS__; }                                         \
+    } while (0)
+
+static inline bool papr_type_ok(int t) { return t == PAPR_TYPE_F32 || t == PAPR_TYPE_F16 || t == PAPR_TYPE_BF16; }
+static inline int papr_type_bytes(int t) { return t == PAPR_TYPE_F32 ? 4 : 2; }
+// whole 16-byte vectors: base, row stride (elements) and width
+static inline bool papr_rows_aligned(const void* p, int64_t ld, int64_t width, int bytes) {
+    return ((uintptr_t)p & 15) == 0 && (ld * bytes) % 16 == 0 && (width * bytes) % 16 == 0;
+}
+
+// Parameters (norm gains and shifts, column scales) may be held in another type than the rows: N values from element `at` on, the type uniform.
+template <int N>
+__device__ __forceinline__ void load_param(float (&v)[N], const void* p, int type, int64_t at) {
+    if (type == PAPR_TYPE_F32) {
+        const auto t = *reinterpret_cast<const papr_pack<float, N>*>(reinterpret_cast<const float*>(p) + at);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = t.v[i];
+    } else if (type == PAPR_TYPE_F16) {
+        const auto t = *reinterpret_cast<const papr_pack<f16, N>*>(reinterpret_cast<const f16*>(p) + at);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (float)t.v[i];
+    } else {
+        const auto t = *reinterpret_cast<const papr_pack<bf16, N>*>(reinterpret_cast<const bf16*>(p) + at);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (float)t.v[i];
+    }
+}
+__device__ __forceinline__ void store_param(void* p, int type, int64_t at, float v) {
+    if (type == PAPR_TYPE_F32) reinterpret_cast<float*>(p)[at] = v;
+    else if (type == PAPR_TYPE_F16) reinterpret_cast<f16*>(p)[at] = (f16)v;
+    else reinterpret_cast<bf16*>(p)[at] = (bf16)v;
+}
+
+// Column sums left as one partial row per workgroup, part (blocks, n), added up in block order (the same bits on every run).  One workgroup takes 64
+// columns; its 16 waves take strips of the blocks.
+struct papr_colsum_out { void* p[5]; int32_t type[5]; };
+int papr_colsum_reduce(const float* part, int64_t n_blocks, int32_t width, int32_t n_arrays, const papr_colsum_out& out, hipStream_t s);      // join.hip
+
+// Four 8-bit codes (rows8.hip) times their block's power-of-two scale.
+template <int FMT>
+__device__ __forceinline__ void papr_codes_to_float(unsigned w, float scale, float* v) {
+    if (FMT == PAPR_KEEP_E4M3) {
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+        v[0] = a[0] * scale; v[1] = a[1] * scale; v[2] = b[0] * scale; v[3] = b[1] * scale;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = (int)(w << (24 - 8 * i)) >> 24;
+            v[i] = c == -128 ? __uint_as_float(0x7FC00000u) : (float)c * scale;
+        }
+    }
+}

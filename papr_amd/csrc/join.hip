@@ -1,0 +1,459 @@
+// The joint of a residual block, one pass over the rows:
+//     y = x + s * a(g) * N_post(f)        (the block's output f normed, gated, scaled and added to the stream x)
+//     h = N_pre(y)                        (the next block's input)
+// with N = layernorm (v - mean) / (std_unbiased + eps) * gain + shift -- the framework's own form (models/attn.py:39-42) -- or rmsnorm
+// v / sqrt(mean(v^2) + eps) * gain (+ shift), a = identity, sigmoid or silu, g one gate per element or per row, s a number or one per column.
+// Bound by HBM: forward reads x, f, g and writes y, h; backward reads x, f, g, d_y, d_h and writes d_x, d_f, d_g.  The backward pass reads x and
+// recomputes y in float32 (reading the rounded y instead would move the same bytes).
+//
+// A row lies in the registers of G lanes, eight elements each (G = the power of two that covers the width): sums over a row are DPP steps inside a
+// wave, one LDS exchange where a row takes several waves.  Norms in two passes over the registers (mean, then squares): no cancellation.
+#include "block_types.h"
+
+namespace {
+
+constexpr int E = 8;                              // elements of a row per lane
+
+template <int G, int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float (*lds)[N][16], int& turn) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        v[n] += PAPR_DPP_F(v[n], 0xB1);
+        v[n] += PAPR_DPP_F(v[n], 0x4E);
+        if (G >= 8) v[n] += PAPR_DPP_F(v[n], 0x141);
+        if (G >= 16) v[n] += PAPR_DPP_F(v[n], 0x140);
+        if (G >= 32) v[n] += __shfl_xor(v[n], 16);
+        if (G >= 64) v[n] += __shfl_xor(v[n], 32);
+    }
+    if (G > 64) {                                 // (two turns of the table: a wave writes one while slower waves still read the other)
+        const int wave = threadIdx.x >> 6;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) lds[turn][n][wave] = v[n];
+        __syncthreads();
+        const int first = wave / (G / 64) * (G / 64);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < G / 64; ++w) s += lds[turn][n][first + w];
+            v[n] = s;
+        }
+    }
+}
+
+template <typename T, int V, int G>
+struct Row {
+    static constexpr int CH = E / V;
+    // column of element i of lane j
+    static __device__ __forceinline__ int col(int j, int i) { return (i / V * G + j) * V + i % V; }
+    static __device__ __forceinline__ void load(float (&v)[E], const T* row, int width, int j) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * G + j) * V;
+            papr_pack<T, V> t;
+            if (at < width) t = *reinterpret_cast<const papr_pack<T, V>*>(row + at);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[c * V + i] = at < width ? (float)t.v[i] : 0.f;
+        }
+    }
+    static __device__ __forceinline__ void store(const float (&v)[E], T* row, int width, int j) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * G + j) * V;
+            if (at >= width) continue;
+            papr_pack<T, V> t;
+#pragma unroll
+            for (int i = 0; i < V; ++i) t.v[i] = (T)v[c * V + i];
+            *reinterpret_cast<papr_pack<T, V>*>(row + at) = t;
+        }
+    }
+    static __device__ __forceinline__ void param(float (&v)[E], const void* p, int type, int width, int j, float absent) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int at = (c * G + j) * V;
+            float t[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[i] = absent;
+            if (p && at < width) load_param<V>(t, p, type, at);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[c * V + i] = at < width ? t[i] : 0.f;
+        }
+    }
+};
+
+__device__ __forceinline__ float gate_value(float g, int act) {
+    if (act == PAPR_GATE_NONE) return g;
+    const float p = 1.f / (1.f + expf(-g));
+    return act == PAPR_GATE_SIGMOID ? p : g * p;
+}
+__device__ __forceinline__ float gate_slope(float g, int act) {
+    if (act == PAPR_GATE_NONE) return 1.f;
+    const float p = 1.f / (1.f + expf(-g));
+    return act == PAPR_GATE_SIGMOID ? p * (1.f - p) : p * (1.f + g * (1.f - p));
+}
+
+// v <- standardised rows; stats = {mean, 1 / divisor, factor of the correlation term in the backward pass}
+template <int G, int V>
+__device__ __forceinline__ void standardise(float (&v)[E], int kind, float eps, int width, int j, float (&stats)[3], float (*lds)[1][16], int& turn) {
+    if (kind == PAPR_NORM_NONE) return;
+    const float rw = 1.f / (float)width;
+    float s[1] = {0.f};
+    stats[0] = 0.f;
+    if (kind == PAPR_NORM_LAYER) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s[0] += v[i];
+        group_sum<G, 1>(s, lds, turn);
+        stats[0] = s[0] * rw;
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = (i / V * G + j) * V < width ? v[i] - stats[0] : 0.f;
+    }
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) s[0] = __builtin_fmaf(v[i], v[i], s[0]);
+    group_sum<G, 1>(s, lds, turn);
+    if (kind == PAPR_NORM_LAYER) {
+        const float std = sqrtf(s[0] / (float)(width - 1)), div = std + eps;
+        stats[1] = 1.f / div;
+        stats[2] = std > 0.f ? div / ((float)(width - 1) * std) : 0.f;      // (a constant row: the deviation's slope is taken as zero, like torch's)
+    } else {
+        stats[1] = 1.f / sqrtf(s[0] * rw + eps);
+        stats[2] = rw;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] *= stats[1];
+}
+
+template <typename T, int V, int G>
+__global__ __launch_bounds__(G > 256 ? G : 256) void join_fwd_kernel(papr_join_desc d, T* __restrict__ y_out, T* __restrict__ h_out, float* __restrict__ stats_out) {
+    typedef Row<T, V, G> R;
+    constexpr int THREADS = G > 256 ? G : 256, RPB = THREADS / G;
+    __shared__ float lds[2][1][16];
+    int turn = 0;
+    const int j = threadIdx.x % G, width = d.width;
+    float pa[E], pb[E], qa[E], qb[E], sc[E];
+    R::param(pa, d.post.gain, d.post.type, width, j, 1.f);
+    R::param(pb, d.post.shift, d.post.type, width, j, 0.f);
+    R::param(qa, d.pre.gain, d.pre.type, width, j, 1.f);
+    R::param(qb, d.pre.shift, d.pre.type, width, j, 0.f);
+    R::param(sc, d.scale_cols, d.scale_type, width, j, d.scale);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < d.rows; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t at = r0 + threadIdx.x / G, row = at < d.rows ? at : d.rows - 1;
+        const bool live = at < d.rows;
+        float y[E], f[E], g[E], st[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        R::load(y, reinterpret_cast<const T*>(d.x) + row * d.ldx, width, j);
+        if (d.f) {
+            R::load(f, reinterpret_cast<const T*>(d.f) + row * d.ldf, width, j);
+            if (d.gate_form == PAPR_GATE_FULL) R::load(g, reinterpret_cast<const T*>(d.gate) + row * d.ldg, width, j);
+            float g1 = 0.f;
+            if (d.gate_form == PAPR_GATE_ROW) g1 = gate_value((float)reinterpret_cast<const T*>(d.gate)[row * d.ldg], d.gate_act);
+            float s3[3] = {0.f, 0.f, 0.f};
+            standardise<G, V>(f, d.post.kind, d.post.eps, width, j, s3, lds, turn);
+            st[0] = s3[0]; st[1] = s3[1]; st[2] = s3[2];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float ga = d.gate_form == PAPR_GATE_FULL ? gate_value(g[i], d.gate_act) : d.gate_form == PAPR_GATE_ROW ? g1 : 1.f;
+                y[i] += sc[i] * ga * __builtin_fmaf(f[i], pa[i], pb[i]);
+            }
+            if (live && y_out) R::store(y, y_out + row * width, width, j);
+        }
+        if (h_out) {
+            float s3[3] = {0.f, 0.f, 0.f};
+            standardise<G, V>(y, d.pre.kind, d.pre.eps, width, j, s3, lds, turn);
+            st[3] = s3[0]; st[4] = s3[1]; st[5] = s3[2];
+#pragma unroll
+            for (int i = 0; i < E; ++i) y[i] = __builtin_fmaf(y[i], qa[i], qb[i]);
+            if (live) R::store(y, h_out + row * width, width, j);
+        }
+        if (stats_out && live && j == 0) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) stats_out[row * 6 + i] = st[i];
+        }
+    }
+}
+
+template <typename T, int V, int G>
+__global__ __launch_bounds__(G > 256 ? G : 256) void join_bwd_kernel(papr_join_desc d, const float* __restrict__ stats, const T* __restrict__ d_y, const T* __restrict__ d_h,
+                                                                     T* __restrict__ d_x, T* __restrict__ d_f, T* __restrict__ d_g, float* __restrict__ part) {
+    typedef Row<T, V, G> R;
+    constexpr int THREADS = G > 256 ? G : 256, RPB = THREADS / G;
+    __shared__ float lds[2][3][16];
+    __shared__ float fold[RPB > 1 ? RPB * G * E : 1];
+    int turn = 0;
+    const int j = threadIdx.x % G, width = d.width;
+    const float rw = 1.f / (float)width;
+    float pa[E], pb[E], qa[E], sc[E];
+    R::param(pa, d.post.gain, d.post.type, width, j, 1.f);
+    R::param(pb, d.post.shift, d.post.type, width, j, 0.f);
+    R::param(qa, d.pre.gain, d.pre.type, width, j, 1.f);
+    R::param(sc, d.scale_cols, d.scale_type, width, j, d.scale);
+    float acc[5][E];                              // column sums: d(pre gain), d(pre shift), d(post gain), d(post shift), d(scale)
+#pragma unroll
+    for (int a = 0; a < 5; ++a)
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[a][i] = 0.f;
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < d.rows; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t at = r0 + threadIdx.x / G, row = at < d.rows ? at : d.rows - 1;
+        const bool live = at < d.rows;
+        float x[E], f[E], g[E], dy[E], dh[E];
+        const int seen = live ? width : 0;        // (a row past the end: zero gradients, nothing reaches the sums)
+        R::load(x, reinterpret_cast<const T*>(d.x) + row * d.ldx, width, j);
+        if (d.f) R::load(f, reinterpret_cast<const T*>(d.f) + row * d.ldf, width, j);
+        if (d.gate_form == PAPR_GATE_FULL) R::load(g, reinterpret_cast<const T*>(d.gate) + row * d.ldg, width, j);
+        if (d_y) R::load(dy, d_y + row * width, seen, j);
+        if (d_h) R::load(dh, d_h + row * width, seen, j);
+        float g1 = 0.f;
+        if (d.gate_form == PAPR_GATE_ROW) g1 = (float)reinterpret_cast<const T*>(d.gate)[row * d.ldg];
+        const float* st = stats + row * 6;
+        const float m1 = st[0], r1 = st[1], c1 = st[2], m2 = st[3], r2 = st[4], c2 = st[5];
+        float ga[E], p[E];
+        if (d.f) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const bool in = (i / V * G + j) * V < width;
+                if (d.post.kind != PAPR_NORM_NONE) f[i] = in ? (f[i] - m1) * r1 : 0.f;
+                p[i] = __builtin_fmaf(f[i], pa[i], pb[i]);
+                ga[i] = d.gate_form == PAPR_GATE_FULL ? gate_value(g[i], d.gate_act) : d.gate_form == PAPR_GATE_ROW ? gate_value(g1, d.gate_act) : 1.f;
+                x[i] += sc[i] * ga[i] * p[i];
+            }
+        }
+        if (!d_y)
+#pragma unroll
+            for (int i = 0; i < E; ++i) dy[i] = 0.f;
+        if (d_h) {
+            if (d.pre.kind == PAPR_NORM_NONE) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    acc[0][i] = __builtin_fmaf(dh[i], x[i], acc[0][i]);
+                    acc[1][i] += dh[i];
+                    dy[i] = __builtin_fmaf(dh[i], qa[i], dy[i]);
+                }
+            } else {
+                float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const bool in = (i / V * G + j) * V < width;
+                    x[i] = in ? (x[i] - m2) * r2 : 0.f;
+                    acc[0][i] = __builtin_fmaf(dh[i], x[i], acc[0][i]);
+                    acc[1][i] += dh[i];
+                    dh[i] *= qa[i];
+                    s[0] = __builtin_fmaf(dh[i], x[i], s[0]);
+                    s[1] += dh[i];
+                }
+                group_sum<G, 3>(s, lds, turn);
+                const float t = s[0] * c2, m = d.pre.kind == PAPR_NORM_LAYER ? s[1] * rw : 0.f;
+#pragma unroll
+                for (int i = 0; i < E; ++i) dy[i] += (dh[i] - x[i] * t - m) * r2;
+            }
+        }
+        if (live && d_x) R::store(dy, d_x + row * width, width, j);
+        if (!d.f) continue;
+        float s[3] = {0.f, 0.f, 0.f}, dp[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const bool in = (i / V * G + j) * V < width;
+            const float dyi = in ? dy[i] : 0.f;
+            const float slope = d.gate_form == PAPR_GATE_FULL ? gate_slope(g[i], d.gate_act) : d.gate_form == PAPR_GATE_ROW ? gate_slope(g1, d.gate_act) : 0.f;
+            acc[4][i] = __builtin_fmaf(dyi * ga[i], p[i], acc[4][i]);
+            g[i] = dyi * sc[i] * p[i] * slope;
+            s[2] += g[i];
+            dp[i] = dyi * sc[i] * ga[i];
+            acc[2][i] = __builtin_fmaf(dp[i], f[i], acc[2][i]);
+            acc[3][i] += dp[i];
+            dp[i] *= pa[i];
+            s[0] = __builtin_fmaf(dp[i], f[i], s[0]);
+            s[1] += dp[i];
+        }
+        group_sum<G, 3>(s, lds, turn);
+        if (d_g) {
+            if (d.gate_form == PAPR_GATE_FULL) { if (live) R::store(g, d_g + row * width, width, j); }
+            else if (live && j == 0) d_g[row] = (T)s[2];
+        }
+        if (d.post.kind != PAPR_NORM_NONE) {
+            const float t = s[0] * c1, m = d.post.kind == PAPR_NORM_LAYER ? s[1] * rw : 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) dp[i] = (dp[i] - f[i] * t - m) * r1;
+        }
+        if (live && d_f) R::store(dp, d_f + row * width, width, j);
+    }
+    if (!part) return;
+    // the workgroup's row groups meet in LDS, in group order; one partial row per workgroup and array
+    float* out = part + (int64_t)blockIdx.x * 5 * width;
+#pragma unroll
+    for (int a = 0; a < 5; ++a) {
+        if (RPB > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; ++i) fold[(threadIdx.x / G * E + i) * G + j] = acc[a][i];
+            __syncthreads();
+            for (int q = threadIdx.x; q < E * G; q += THREADS) {
+                float s = 0.f;
+                for (int k = 0; k < RPB; ++k) s += fold[k * E * G + q];
+                const int c = R::col(q % G, q / G);
+                if (c < width) out[(int64_t)a * width + c] = s;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int c = R::col(j, i);
+                if (c < width) out[(int64_t)a * width + c] = acc[a][i];
+            }
+        }
+    }
+}
+
+int lanes_for(int width, bool vec) {
+    const int need = (width + E - 1) / E;
+    for (int g = vec ? 8 : 16; g <= 1024; g *= vec ? 2 : 4)
+        if (g >= need) return g;
+    return 0;
+}
+
+template <typename T, int V, int G>
+int launch_join(const papr_join_desc& d, bool bwd, void* y, void* h, float* stats, const void* d_y, const void* d_h, void* d_x, void* d_f, void* d_g, float* part,
+                int64_t blocks, hipStream_t s) {
+    constexpr int THREADS = G > 256 ? G : 256;
+    if (bwd)
+        join_bwd_kernel<T, V, G><<<dim3((unsigned)blocks), dim3(THREADS), 0, s>>>(d, stats, (const T*)d_y, (const T*)d_h, (T*)d_x, (T*)d_f, (T*)d_g, part);
+    else
+        join_fwd_kernel<T, V, G><<<dim3((unsigned)blocks), dim3(THREADS), 0, s>>>(d, (T*)y, (T*)h, stats);
+    PAPR_CHECK_LAUNCH(bwd ? "papr_join_bwd" : "papr_join_fwd");
+    return 0;
+}
+
+template <typename T, int V>
+int pick_join(int G, const papr_join_desc& d, bool bwd, void* y, void* h, float* stats, const void* d_y, const void* d_h, void* d_x, void* d_f, void* d_g, float* part,
+              int64_t blocks, hipStream_t s) {
+#define PAPR_JOIN_CASE(g) case g: return launch_join<T, V, g>(d, bwd, y, h, stats, d_y, d_h, d_x, d_f, d_g, part, blocks, s);
+    if constexpr (V > 1) {
+        switch (G) { PAPR_JOIN_CASE(8) PAPR_JOIN_CASE(16) PAPR_JOIN_CASE(32) PAPR_JOIN_CASE(64) PAPR_JOIN_CASE(128) PAPR_JOIN_CASE(256) PAPR_JOIN_CASE(512) PAPR_JOIN_CASE(1024) }
+    } else {
+        switch (G) { PAPR_JOIN_CASE(16) PAPR_JOIN_CASE(64) PAPR_JOIN_CASE(256) PAPR_JOIN_CASE(1024) }
+    }
+#undef PAPR_JOIN_CASE
+    papr_set_error("papr_join: no kernel for %d lanes a row", G);
+    return 1;
+}
+
+bool join_vec(const papr_join_desc& d) {
+    const int b = papr_type_bytes(d.type);
+    bool ok = papr_rows_aligned(d.x, d.ldx, d.width, b) && (!d.f || papr_rows_aligned(d.f, d.ldf, d.width, b)) &&
+              (d.gate_form != PAPR_GATE_FULL || papr_rows_aligned(d.gate, d.ldg, d.width, b));
+    const void* params[5] = {d.post.gain, d.post.shift, d.pre.gain, d.pre.shift, d.scale_cols};
+    for (const void* p : params) ok = ok && ((uintptr_t)p & 31) == 0;
+    return ok;
+}
+
+int64_t join_blocks(const papr_join_desc& d, int G, bool bwd) {
+    const int64_t rpb = G > 256 ? 1 : 256 / G, need = (d.rows + rpb - 1) / rpb;
+    const int64_t cap = (int64_t)papr_cu_count() * (G >= 512 ? 2 : bwd ? 4 : 8);
+    return need < cap ? need : cap;
+}
+
+int join_check(const papr_join_desc* d, const char* who) {
+    PAPR_REQUIRE(d, "%s: no descriptor", who);
+    PAPR_REQUIRE(papr_type_ok(d->type), "%s: unknown row type %d", who, d->type);
+    PAPR_REQUIRE(d->rows >= 0 && d->width >= 1 && d->width <= PAPR_JOIN_MAX_WIDTH, "%s: rows %lld, width %d (1 .. %d)", who, (long long)d->rows, d->width, PAPR_JOIN_MAX_WIDTH);
+    PAPR_REQUIRE(d->gate_form >= PAPR_GATE_ABSENT && d->gate_form <= PAPR_GATE_FULL, "%s: unknown gate form %d", who, d->gate_form);
+    PAPR_REQUIRE(d->gate_act >= PAPR_GATE_NONE && d->gate_act <= PAPR_GATE_SILU, "%s: unknown gate activation %d", who, d->gate_act);
+    PAPR_REQUIRE(d->rows == 0 || d->x, "%s: x is missing", who);
+    PAPR_REQUIRE(d->rows == 0 || (d->gate_form != PAPR_GATE_ABSENT) == (d->gate != nullptr), "%s: gate and gate_form disagree", who);
+    PAPR_REQUIRE(d->gate_form == PAPR_GATE_ABSENT || d->f || d->rows == 0, "%s: a gate without the block's output f", who);
+    const papr_block_norm* norms[2] = {&d->post, &d->pre};
+    for (const papr_block_norm* n : norms) {
+        PAPR_REQUIRE(n->kind >= PAPR_NORM_NONE && n->kind <= PAPR_NORM_RMS, "%s: unknown norm %d", who, n->kind);
+        PAPR_REQUIRE(n->kind != PAPR_NORM_LAYER || d->width >= 2, "%s: layernorm's unbiased deviation needs two columns", who);
+        PAPR_REQUIRE(papr_type_ok(n->type), "%s: unknown parameter type %d", who, n->type);
+    }
+    PAPR_REQUIRE(papr_type_ok(d->scale_type), "%s: unknown scale type %d", who, d->scale_type);
+    return 0;
+}
+
+__global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ part, int64_t n_blocks, int32_t width, int32_t n_arrays, papr_colsum_out out) {
+    __shared__ float lds[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = blockIdx.y;
+    if (!out.p[a]) return;                        // (uniform over the workgroup)
+    const int c = blockIdx.x * 64 + lane;
+    const int64_t step = (int64_t)n_arrays * width, per = (n_blocks + 15) / 16;
+    int64_t b = wave * per, end = b + per < n_blocks ? b + per : n_blocks;
+    const float* p = part + (int64_t)a * width + (c < width ? c : 0);
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    for (; b + 4 <= end; b += 4) {
+        s0 += p[b * step]; s1 += p[(b + 1) * step]; s2 += p[(b + 2) * step]; s3 += p[(b + 3) * step];
+    }
+    for (; b < end; ++b) s0 += p[b * step];
+    lds[wave][lane] = (s0 + s1) + (s2 + s3);
+    __syncthreads();
+    if (wave == 0 && c < width) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) s += lds[w][lane];
+        store_param(out.p[a], out.type[a], c, s);
+    }
+}
+
+}  // namespace
+
+int papr_colsum_reduce(const float* part, int64_t n_blocks, int32_t width, int32_t n_arrays, const papr_colsum_out& out, hipStream_t s) {
+    colsum_kernel<<<dim3((width + 63) / 64, n_arrays), dim3(1024), 0, s>>>(part, n_blocks, width, n_arrays, out);
+    PAPR_CHECK_LAUNCH("papr column sums");
+    return 0;
+}
+
+extern "C" int papr_join_fwd(const papr_join_desc* d, void* y, void* h, float* stats, papr_stream_t stream) {
+    if (int rc = join_check(d, "papr_join_fwd")) return rc;
+    if (d->rows == 0) return 0;
+    PAPR_REQUIRE(y || h, "papr_join_fwd: neither y nor h is asked for");
+    PAPR_REQUIRE(!y || d->f, "papr_join_fwd: y without the block's output f (it would be x)");
+    const bool vec = join_vec(*d) && ((uintptr_t)y & 15) == 0 && ((uintptr_t)h & 15) == 0;
+    const int G = lanes_for(d->width, vec);
+    const int64_t blocks = join_blocks(*d, G, false);
+    PAPR_TYPE_SWITCH(d->type, {
+        if (vec) return pick_join<T, 16 / sizeof(T)>(G, *d, false, y, h, stats, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, blocks, as_stream(stream));
+        return pick_join<T, 1>(G, *d, false, y, h, stats, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, blocks, as_stream(stream));
+    });
+}
+
+extern "C" size_t papr_join_bwd_workspace_bytes(int64_t rows, int32_t width) {
+    if (rows <= 0 || width <= 0) return 0;
+    papr_join_desc d = {};
+    d.rows = rows; d.width = width;
+    int64_t most = 0;
+    for (int v = 0; v < 2; ++v) {
+        const int G = lanes_for(width, v != 0);
+        const int64_t b = G ? join_blocks(d, G, true) : 0;
+        most = b > most ? b : most;
+    }
+    return (size_t)most * 5 * (size_t)width * sizeof(float);
+}
+
+extern "C" int papr_join_bwd(const papr_join_desc* d, const float* stats, const void* d_y, const void* d_h, void* d_x, void* d_f, void* d_g,
+                             const papr_join_grads* g, void* workspace, papr_stream_t stream) {
+    if (int rc = join_check(d, "papr_join_bwd")) return rc;
+    papr_colsum_out out = {};
+    bool sums = false;
+    if (g) {
+        void* p[5] = {g->pre_gain, g->pre_shift, g->post_gain, g->post_shift, g->scale_cols};
+        const int32_t t[5] = {d->pre.type, d->pre.type, d->post.type, d->post.type, d->scale_type};
+        for (int i = 0; i < 5; ++i) { out.p[i] = p[i]; out.type[i] = t[i]; sums = sums || p[i]; }
+    }
+    PAPR_REQUIRE(!sums || d->rows == 0 || workspace, "papr_join_bwd: parameter gradients need the workspace");
+    if (d->rows == 0) return sums ? papr_colsum_reduce(nullptr, 0, d->width, 5, out, as_stream(stream)) : 0;
+    PAPR_REQUIRE(stats, "papr_join_bwd: the forward call's stats are missing");
+    PAPR_REQUIRE(d_y || d_h, "papr_join_bwd: neither d_y nor d_h is given");
+    PAPR_REQUIRE(d->f || (!d_f && !d_g), "papr_join_bwd: gradients of f or its gate without f");
+    const void* rows_out[5] = {d_y, d_h, d_x, d_f, d->gate_form == PAPR_GATE_FULL ? d_g : nullptr};
+    bool vec = join_vec(*d);
+    for (const void* p : rows_out) vec = vec && ((uintptr_t)p & 15) == 0;
+    const int G = lanes_for(d->width, vec);
+    const int64_t blocks = join_blocks(*d, G, true);
+    float* part = sums ? (float*)workspace : nullptr;
+    int rc = 0;
+    PAPR_TYPE_SWITCH(d->type, {
+        rc = vec ? pick_join<T, 16 / sizeof(T)>(G, *d, true, nullptr, nullptr, const_cast<float*>(stats), d_y, d_h, d_x, d_f, d_g, part, blocks, as_stream(stream))
+                 : pick_join<T, 1>(G, *d, true, nullptr, nullptr, const_cast<float*>(stats), d_y, d_h, d_x, d_f, d_g, part, blocks, as_stream(stream));
+    });
+    if (rc || !sums) return rc;
+    return papr_colsum_reduce(part, blocks, d->width, 5, out, as_stream(stream));
+}

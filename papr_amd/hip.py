@@ -13,7 +13,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PAPR_HIP_LIB", os.path.join(_PKG, "libpapr_hip.so"))   # override: instrumented builds (scripts/probes)
 
 ACT = {"none": 0, "relu": 1, "leakyrelu": 2}
-EXPECTED_ABI = 27
+EXPECTED_ABI = 28
 # `mode` argument of papr_mlp_fwd / papr_mlp_bwd (include/papr_hip.h: PAPR_MLP_*)
 MLP_MODES = {"h3": 0, "h1": 1, "f32": 2, "fwd": 3, "dgrad": 4, "layers": 5, "h1_f32rows": 6, "h3_f16rows": 7}
 # process-wide A/B switches of the library (papr_set_switch; PAPR_SW_* in include/papr_hip.h).  The library itself reads no environment:
@@ -27,6 +27,8 @@ EXPORTS = [
     "papr_rownorm_fwd", "papr_rownorm_bwd", "papr_row_dots", "papr_qk_bias_bwd_workspace_bytes", "papr_qk_bias_bwd", "papr_mse_workspace_bytes", "papr_mse_fwd", "papr_ln_fold_fwd", "papr_ln_fold_bwd", "papr_ln_fold_fwd_batch", "papr_ln_fold_bwd_batch", "papr_mlp_fwd_workspace_bytes", "papr_mlp_bwd_workspace_bytes", "papr_mlp_saved_floats", "papr_mlp_bwd_needs_weight_t", "papr_mlp_fwd",
     "papr_mlp_bwd", "papr_mlp_bwd_takes_f16_rows",
     "papr_attn_tail_fwd", "papr_attn_tail_bwd", "papr_conv3x3_weight_halfs", "papr_conv3x3_workspace_bytes", "papr_conv3x3_fwd", "papr_conv3x3_wgrad_workspace_bytes", "papr_conv3x3_wgrad", "papr_maxpool2_fwd", "papr_maxpool2_bwd", "papr_upconv2x2_fwd", "papr_upconv2x2_dgrad", "papr_upconv2x2_wgrad_workspace_bytes", "papr_upconv2x2_wgrad", "papr_conv1x1_fwd", "papr_conv1x1_bwd_workspace_bytes", "papr_conv1x1_bwd", "papr_small_unet_state_bytes", "papr_small_unet_bwd_workspace_bytes", "papr_small_unet_fwd", "papr_small_unet_bwd", "papr_adam_step", "papr_adam_step_scaled", "papr_composite_fwd", "papr_composite_bwd_workspace_bytes", "papr_composite_bwd", "papr_profile_enable", "papr_profile_collect", "papr_set_switch", "papr_get_switch",
+    "papr_linear_fwd", "papr_linear_bwd_workspace_bytes", "papr_linear_bwd", "papr_rows8_pack", "papr_rows8_unpack",
+    "papr_join_fwd", "papr_join_bwd_workspace_bytes", "papr_join_bwd",
 ]
 
 
@@ -85,6 +87,25 @@ class UnetGrads(C.Structure):            # papr_unet_grads
                 ("out_w", C.c_void_p), ("out_b", C.c_void_p)]
 
 
+class LinearDesc(C.Structure):           # papr_linear_desc
+    _fields_ = [("type", C.c_int32), ("act", C.c_int32), ("keep", C.c_int32), ("reserved", C.c_int32), ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64)]
+
+
+class BlockNorm(C.Structure):            # papr_block_norm
+    _fields_ = [("kind", C.c_int32), ("type", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32), ("gain", C.c_void_p), ("shift", C.c_void_p)]
+
+
+class JoinDesc(C.Structure):             # papr_join_desc
+    _fields_ = [("rows", C.c_int64), ("width", C.c_int32), ("type", C.c_int32), ("x", C.c_void_p), ("ldx", C.c_int64), ("f", C.c_void_p), ("ldf", C.c_int64),
+                ("gate", C.c_void_p), ("ldg", C.c_int64), ("gate_form", C.c_int32), ("gate_act", C.c_int32), ("scale_cols", C.c_void_p), ("scale_type", C.c_int32),
+                ("scale", C.c_float), ("post", BlockNorm), ("pre", BlockNorm)]
+
+
+class JoinGrads(C.Structure):            # papr_join_grads
+    _fields_ = [("pre_gain", C.c_void_p), ("pre_shift", C.c_void_p), ("post_gain", C.c_void_p), ("post_shift", C.c_void_p), ("scale_cols", C.c_void_p)]
+
+
+JOIN_MAX_WIDTH = 8192
 _lib = None
 
 
@@ -179,6 +200,16 @@ def lib():
     L.papr_attn_tail_fwd.argtypes = [C.POINTER(TailDesc), vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp]
     L.papr_attn_tail_bwd.argtypes = [C.POINTER(TailDesc), vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                      C.POINTER(F16Rows), C.POINTER(F16Rows), vp]
+    L.papr_linear_fwd.argtypes = [C.POINTER(LinearDesc), vp, i64, vp, i64, vp, vp, i64, vp, vp, vp]
+    L.papr_linear_bwd_workspace_bytes.restype = C.c_size_t
+    L.papr_linear_bwd_workspace_bytes.argtypes = [C.POINTER(LinearDesc)]
+    L.papr_linear_bwd.argtypes = [C.POINTER(LinearDesc), vp, i64, vp, vp, i64, vp, vp, i64, vp, vp, vp, vp, vp]
+    L.papr_rows8_pack.argtypes = [i32, i32, vp, i64, i64, i32, vp, vp, vp]
+    L.papr_rows8_unpack.argtypes = [i32, i32, vp, vp, i64, i32, vp, vp]
+    L.papr_join_fwd.argtypes = [C.POINTER(JoinDesc), vp, vp, vp, vp]
+    L.papr_join_bwd_workspace_bytes.restype = C.c_size_t
+    L.papr_join_bwd_workspace_bytes.argtypes = [i64, i32]
+    L.papr_join_bwd.argtypes = [C.POINTER(JoinDesc), vp, vp, vp, vp, vp, vp, C.POINTER(JoinGrads), vp, vp]
     L.papr_profile_enable.argtypes = [i32]
     L.papr_profile_collect.argtypes = [C.POINTER(ProfileRecord), i32]
     L.papr_set_switch.argtypes = [i32, i32]
