@@ -19,22 +19,71 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 namespace {
 
-__device__ __forceinline__ float act_value(float z, int act) {
-    switch (act) {
-        case PAPR_ACT_RELU: return z > 0.f ? z : 0.f;
-        case PAPR_ACT_LEAKY_RELU: return z > 0.f ? z : 0.2f * z;
-        case PAPR_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
-        case PAPR_ACT_SILU: return z / (1.f + expf(-z));
-        default: return z;
+// 1 / (1 + exp(-z)): the exponent's product with log2(e) in two parts (relative error of a few ulp for every z), hardware exp2 and reciprocal.
+__device__ __forceinline__ float sigmoid(float z) {
+    const float a = fminf(z * -1.44269504f, 126.f), rest = a < 126.f ? __builtin_fmaf(z, -1.44269504f, -a) + z * -1.92596299e-8f : 0.f;
+    const float e = __builtin_amdgcn_exp2f(a);
+    return __builtin_amdgcn_rcpf(1.f + __builtin_fmaf(e, rest * 0.693147181f, e));
+}
+// Phi(z) and phi(z) of the erf form of gelu.  float32 rows: the library's erf and exp.  16-bit rows: erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2), t = 1 / (1 + p x)
+// (Abramowitz and Stegun 7.1.26, 1.5e-7 absolute), a sixteenth of the rows' own rounding and a third of erf's instructions: erf in the epilogue of an
+// 8192 x 1024 -> 4096 layer took longer than its matrix instructions.
+template <bool EXACT>
+__device__ __forceinline__ void gauss(float z, float& cdf, float& pdf) {
+    if (EXACT) {
+        cdf = 0.5f * erfcf(z * -0.70710678f);
+        pdf = 0.39894228f * expf(-0.5f * z * z);
+    } else {
+        const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+        const float e = __builtin_amdgcn_exp2f(x * x * -1.44269504f);
+        const float q = 0.5f * t * e * __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        cdf = z < 0.f ? q : 1.f - q;
+        pdf = 0.39894228f * e;
     }
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case PAPR_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case PAPR_ACT_LEAKY_RELU: return z > 0.f ? 1.f : 0.2f;
-        case PAPR_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
-        case PAPR_ACT_SILU: { const float p = 1.f / (1.f + expf(-z)); return p * (1.f + z * (1.f - p)); }
-        default: return 1.f;
+// v <- act(v)
+template <bool EXACT, int N>
+__device__ __forceinline__ void act_values(float (&v)[N], int act) {
+    if (act == PAPR_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] > 0.f ? v[i] : (v[i] == v[i] ? 0.f : v[i]);
+    } else if (act == PAPR_ACT_LEAKY_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] > 0.f ? v[i] : 0.2f * v[i];
+    } else if (act == PAPR_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float cdf, pdf;
+            gauss<EXACT>(v[i], cdf, pdf);
+            v[i] *= cdf;
+        }
+    } else if (act == PAPR_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
+    }
+}
+// g <- g act'(z)
+template <bool EXACT, int N>
+__device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], int act) {
+    if (act == PAPR_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = z[i] > 0.f ? g[i] : 0.f;
+    } else if (act == PAPR_ACT_LEAKY_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = z[i] > 0.f ? g[i] : 0.2f * g[i];
+    } else if (act == PAPR_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float cdf, pdf;
+            gauss<EXACT>(z[i], cdf, pdf);
+            g[i] *= __builtin_fmaf(z[i], pdf, cdf);
+        }
+    } else if (act == PAPR_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float p = sigmoid(z[i]);
+            g[i] *= p * __builtin_fmaf(z[i], 1.f - p, 1.f);
+        }
     }
 }
 
@@ -42,10 +91,11 @@ enum { K_RUNS = 0, ROWS_RUN = 1 };                // which index of an operand i
 enum { OUT_FORWARD = 0, OUT_ROWS = 1, OUT_SLAB = 2 };
 
 struct Operand { const void* p; int64_t ld; int64_t rows; const uint8_t* exps; };       // exps: 8-bit rows only (ld in codes)
-struct Epilogue {
-    void* out; int64_t ld_out;
+struct Epilogue {                                  // out and z (M, N) contiguous
+    void* out;
     const void* bias; const void* res; int64_t ld_res; void* z;
     int act;
+    int wide;                                      // whole 16-byte vectors in every row of out, z and res
 };
 
 template <typename T> struct Matrix { typedef bf16x8 frag; };
@@ -62,12 +112,13 @@ __device__ __forceinline__ s16x4 read_tr4(unsigned a) { return __builtin_amdgcn_
 //   K_RUNS:   image [R][BK] halfs, 16-byte pieces exchanged by the row number so that 8 rows' reads of one piece cover all banks.
 //   ROWS_RUN: image [BK][R + pad] halfs as it lies in memory; the transposing LDS read hands a lane 8 consecutive k of its row.  The row stride is
 //             64 bytes modulo 256: the four k a 16-lane group reads lie on different quarters of the banks.
-// FMT: 0 rows of type T, else 8-bit rows (ROWS_RUN only).
+// FMT: 0 rows of type T, else 8-bit rows (ROWS_RUN only).  A thread's pieces sit at fixed 32-bit offsets from a uniform tile address that advances with k.
 template <typename T, int LAYOUT, int FMT, bool VEC, int R, int BK, int THREADS>
 struct Tile {
     static constexpr bool SPLIT = sizeof(T) == 4 && FMT == 0;
     static constexpr int PLANES = SPLIT ? 3 : 1;
     static constexpr int PIECE = SPLIT ? 4 : 8;                                   // elements of one load
+    static constexpr int BYTES = FMT ? 1 : sizeof(T);
     static constexpr int N = R * BK / PIECE / THREADS;
     static constexpr int STRIDE = LAYOUT == K_RUNS ? BK : (R * 2 % 256 == 64 ? R : R + 32);
     static constexpr int PLANE = (LAYOUT == K_RUNS ? R : BK) * STRIDE;            // halfs
@@ -76,7 +127,12 @@ struct Tile {
     typedef typename Matrix<T>::frag frag;
 
     uint4 reg[N];
+    unsigned off[N];                                                              // bytes from the tile's address
     uint8_t ex[FMT ? N : 1];
+    unsigned exo[FMT ? N : 1];
+    const char* base;                                                             // (uniform) rows r0, the next k
+    const uint8_t* exb;
+    int64_t ld;
 
     // piece q of this thread: (row, k) of its first element inside the tile
     static __device__ __forceinline__ void where(int q, int& r, int& k) {
@@ -84,49 +140,70 @@ struct Tile {
         if (LAYOUT == K_RUNS) { r = id / (BK / PIECE); k = id % (BK / PIECE) * PIECE; }
         else { k = id / (R / PIECE); r = id % (R / PIECE) * PIECE; }
     }
+    // swizzled place of 16-byte piece c of row r (halfs)
+    static __device__ __forceinline__ int place(int r, int c) {
+        const int sw = BK == 64 ? r & 7 : BK == 32 ? (r >> 1) & 3 : (r >> 2) & 1;
+        return r * STRIDE + ((c ^ sw) << 3);
+    }
 
-    // the tile at rows r0 .., k0 .. of an operand with K terms; `inside`: every piece that starts inside the operand may be read whole and no k is past K
-    __device__ __forceinline__ void load(const Operand& o, int64_t r0, int64_t k0, int64_t K) {
-        bool inside = k0 + BK <= K;
-        // (a piece that crosses the end of a contiguous row of rows reads the start of the next one; those rows of the product are never stored, but
-        // behind the last k there is no next one)
-        if (LAYOUT == ROWS_RUN && !VEC && FMT == 0) inside = k0 + BK < K && o.rows >= PIECE;
+    __device__ __forceinline__ void start(const Operand& o, int64_t r0, int64_t k0) {
+        ld = o.ld;
+        base = reinterpret_cast<const char*>(o.p) + (LAYOUT == K_RUNS ? r0 * ld + k0 : k0 * ld + r0) * BYTES;
+        if (FMT) exb = o.exps + k0 * (ld >> 5) + (r0 >> 5);
+        const int64_t left = (FMT ? ld : o.rows) - r0;
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             int r, k;
             where(q, r, k);
-            const int64_t kk = k0 + k;
-            int64_t rr = r0 + r;
-            if (FMT) {                                                            // 8-bit rows: padded to whole blocks of 32 codes, aligned
-                rr = rr < o.ld ? rr : 0;
-                const bool in = kk < K;
-                const int64_t ks = in ? kk : 0;
-                const uint2 c = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(o.p) + ks * o.ld + rr);
-                ex[q] = o.exps[ks * (o.ld >> 5) + (rr >> 5)];
-                reg[q].x = in ? c.x : 0u;
-                reg[q].y = in ? c.y : 0u;
-                continue;
-            }
-            rr = rr < o.rows ? rr : (LAYOUT == K_RUNS ? o.rows - 1 : 0);
-            const T* src = reinterpret_cast<const T*>(o.p) + (LAYOUT == K_RUNS ? rr * o.ld + kk : kk * o.ld + rr);
-            if (inside) {
-                if (VEC) reg[q] = *reinterpret_cast<const uint4*>(src);
-                else __builtin_memcpy(&reg[q], src, 16);
-            } else if (VEC) {
-                const bool in = kk < K;
-                if (!in) src = reinterpret_cast<const T*>(o.p);
-                const uint4 t = *reinterpret_cast<const uint4*>(src);
-                reg[q].x = in ? t.x : 0u; reg[q].y = in ? t.y : 0u; reg[q].z = in ? t.z : 0u; reg[q].w = in ? t.w : 0u;
-            } else {
-                papr_pack<T, PIECE> t;
+            if (r >= left) r = LAYOUT == K_RUNS ? (int)left - 1 : 0;              // (rows past the end: some row of the operand, its results are never stored)
+            off[q] = (unsigned)((LAYOUT == K_RUNS ? (int64_t)r * ld + k : (int64_t)k * ld + r) * BYTES);
+            if (FMT) exo[q] = (unsigned)(k * (ld >> 5) + (r >> 5));
+        }
+    }
+    // the next tile: k0 .. k0 + BK of K terms.  `inside`: every piece may be read whole.  A piece that crosses the end of a contiguous row of rows reads the start
+    // of the next one (those rows of the product are never stored), but behind the last k there is no next one.
+    __device__ __forceinline__ void load(const Operand& o, int64_t r0, int64_t k0, int64_t K) {
+        bool inside = k0 + BK <= K;
+        if (LAYOUT == ROWS_RUN && !VEC && FMT == 0) inside = k0 + BK < K && o.rows >= PIECE;
+        if (inside) {
 #pragma unroll
-                for (int i = 0; i < PIECE; ++i) {
-                    const bool in = LAYOUT == K_RUNS ? kk + i < K : kk < K && rr + i < o.rows;
-                    t.v[i] = in ? src[i] : (T)0.f;
+            for (int q = 0; q < N; ++q) {
+                const char* src = base + off[q];
+                if (FMT) {
+                    const uint2 c = *reinterpret_cast<const uint2*>(src);
+                    reg[q].x = c.x; reg[q].y = c.y;
+                    ex[q] = exb[exo[q]];
+                } else if (VEC) reg[q] = *reinterpret_cast<const uint4*>(src);
+                else __builtin_memcpy(&reg[q], __builtin_assume_aligned(src, sizeof(T)), 16);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                int r, k;
+                where(q, r, k);
+                const bool in = k0 + k < K;
+                const char* src = in ? base + off[q] : base;                      // (base: rows r0, the tile's first k < K)
+                if (FMT) {
+                    const uint2 c = *reinterpret_cast<const uint2*>(src);
+                    reg[q].x = in ? c.x : 0u; reg[q].y = in ? c.y : 0u;
+                    ex[q] = exb[in ? exo[q] : 0u];
+                } else if (VEC) {
+                    const uint4 t = *reinterpret_cast<const uint4*>(src);
+                    reg[q].x = in ? t.x : 0u; reg[q].y = in ? t.y : 0u; reg[q].z = in ? t.z : 0u; reg[q].w = in ? t.w : 0u;
+                } else {
+                    papr_pack<T, PIECE> t;
+                    if (LAYOUT == ROWS_RUN && r0 + r >= o.rows) r = 0;
+#pragma unroll
+                    for (int i = 0; i < PIECE; ++i) {
+                        const bool ok = LAYOUT == K_RUNS ? k0 + k + i < K : in && r0 + r + i < o.rows;
+                        t.v[i] = ok ? reinterpret_cast<const T*>(src)[i] : (T)0.f;
+                    }
+                    __builtin_memcpy(&reg[q], &t, 16);
                 }
-                __builtin_memcpy(&reg[q], &t, 16);
             }
         }
+        base += (LAYOUT == K_RUNS ? (int64_t)BK : BK * ld) * BYTES;
+        if (FMT) exb += BK * (ld >> 5);
     }
 
     __device__ __forceinline__ void store(short* lds) const {
@@ -134,19 +211,15 @@ struct Tile {
         for (int q = 0; q < N; ++q) {
             int r, k;
             where(q, r, k);
-            int at;
-            if (LAYOUT == K_RUNS) {
-                const int sw = BK == 64 ? r & 7 : (r >> 1) & 3;
-                at = r * STRIDE + (((k >> 3) ^ sw) << 3) + (k & 7);
-            } else at = k * STRIDE + r;
+            const int at = LAYOUT == K_RUNS ? place(r, k >> 3) + (k & 7) : k * STRIDE + r;
             if (FMT) {
-                float v[8];
+                float v[4], w[4];
                 const float scale = __uint_as_float((unsigned)ex[q] << 23);
                 papr_codes_to_float<FMT>(reg[q].x, scale, v);
-                papr_codes_to_float<FMT>(reg[q].y, scale, v + 4);
+                papr_codes_to_float<FMT>(reg[q].y, scale, w);
                 frag h;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) h[i] = v[i];                          // (exact: at most 8 significant bits)
+                for (int i = 0; i < 4; ++i) { h[i] = v[i]; h[4 + i] = w[i]; }     // (exact: at most 8 significant bits)
                 *reinterpret_cast<frag*>(lds + at) = h;
             } else if (SPLIT) {
                 const float f[4] = {__uint_as_float(reg[q].x), __uint_as_float(reg[q].y), __uint_as_float(reg[q].z), __uint_as_float(reg[q].w)};
@@ -165,15 +238,14 @@ struct Tile {
     }
 
     // this lane's operand of the 16-term step ks: row base + (lane & 31), k = 8 (lane >> 5) + 0 .. 7
-    static __device__ __forceinline__ frag read(const short* lds, int plane, int base, int ks) {
+    static __device__ __forceinline__ frag read(const short* lds, int plane, int row, int ks) {
         const int lane = threadIdx.x & 63;
         s16x8 v;
         if (LAYOUT == K_RUNS) {
-            const int r = base + (lane & 31), sw = BK == 64 ? r & 7 : (r >> 1) & 3;
-            v = *reinterpret_cast<const s16x8*>(lds + plane * PLANE + r * STRIDE + (((ks * 2 + (lane >> 5)) ^ sw) << 3));
+            v = *reinterpret_cast<const s16x8*>(lds + plane * PLANE + place(row + (lane & 31), ks * 2 + (lane >> 5)));
         } else {
             const unsigned a = (unsigned)(size_t)(lds + plane * PLANE) +
-                               2u * (unsigned)((ks * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * STRIDE + base + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+                               2u * (unsigned)((ks * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * STRIDE + row + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
             const s16x4 lo = read_tr4(a), hi = read_tr4(a + 8 * STRIDE);
             v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
@@ -181,16 +253,72 @@ struct Tile {
     }
 };
 
-template <typename T, int LA, int LB, int FMT, bool VEC, int OUT, int WM, int WN, int IM, int IN>
-__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operand A, Operand B, int64_t K, int64_t k_per_split, Epilogue ep) {
-    constexpr int THREADS = 64 * WM * WN, TM = WM * IM * 32, TN = WN * IN * 32, BK = sizeof(T) == 4 ? 32 : 64;
-    typedef Tile<T, LA, 0, VEC, TM, BK, THREADS> TA;
-    typedef Tile<T, LB, FMT, VEC, TN, BK, THREADS> TB;
-    constexpr int BUF = TA::HALFS + TB::HALFS;
+// Workgroup -> (row tile, column tile, part of the sum).  Workgroups go to the eight XCDs in turn: each takes a contiguous run of tiles, and the run walks
+// GROUP row tiles down before it steps to the next column tile, so that an XCD's workgroups of one moment share operand tiles in its L2.
+struct Place { int m, n, part; };
+__device__ __forceinline__ Place place_of(unsigned id, unsigned total, unsigned tm, unsigned tn) {
+    constexpr unsigned XCDS = 8, GROUP = 8;
+    const unsigned x = id % XCDS, q = id / XCDS, per = total / XCDS, rem = total % XCDS;
+    const unsigned t = x * per + (x < rem ? x : rem) + q;
+    Place p;
+    p.part = (int)(t / (tm * tn));
+    const unsigned r = t % (tm * tn), g = r / (GROUP * tn), in = r % (GROUP * tn), high = tm - g * GROUP < GROUP ? tm - g * GROUP : GROUP;
+    p.m = (int)(g * GROUP + in % high);
+    p.n = (int)(in / high);
+    return p;
+}
+
+// Tile shapes: waves WM x WN, each IM x IN blocks of 32 x 32.
+template <int WM_, int WN_, int IM_, int IN_>
+struct Shape {
+    static constexpr int WM = WM_, WN = WN_, IM = IM_, IN = IN_, THREADS = 64 * WM * WN, TM = WM * IM * 32, TN = WN * IN * 32;
+};
+
+template <typename T, int LA, int LB, int FMT, bool VEC, typename S>
+struct Plan {
+    static constexpr int BK = sizeof(T) == 2 ? 64 : S::TM > 64 ? 16 : 32;       // (divides step_of)
+    typedef Tile<T, LA, 0, VEC, S::TM, BK, S::THREADS> TA;
+    typedef Tile<T, LB, FMT, VEC, S::TN, BK, S::THREADS> TB;
+    static constexpr int BUF = TA::HALFS + TB::HALFS;
+    static constexpr int EPI_STRIDE = S::IN * 32 + 8;                             // floats: rows four apart lie on the other half of the banks
+    static constexpr size_t EPI = (size_t)S::WM * S::WN * 32 * EPI_STRIDE * 4, LOOP = (size_t)2 * BUF * 2;
+    static constexpr size_t LDS = EPI > LOOP ? EPI : LOOP;
+};
+
+// E consecutive results of row m from column n on
+template <typename T, int OUT, int E>
+__device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int64_t N, const float (&bias)[E], const papr_pack<T, E>& res, const Epilogue& ep) {
+    if (OUT == OUT_FORWARD) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] += bias[i];
+        if (ep.z) {
+            papr_pack<T, E> t;
+#pragma unroll
+            for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
+            *reinterpret_cast<papr_pack<T, E>*>(reinterpret_cast<T*>(ep.z) + m * N + n) = t;
+        }
+        act_values<sizeof(T) == 4>(v, ep.act);
+        if (ep.res)
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] += (float)res.v[i];
+    }
+    papr_pack<T, E> t;
+#pragma unroll
+    for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
+    *reinterpret_cast<papr_pack<T, E>*>(reinterpret_cast<T*>(ep.out) + m * N + n) = t;
+}
+
+template <typename T, int LA, int LB, int FMT, bool VEC, int OUT, typename S>
+__global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Operand B, int64_t K, int64_t k_per_part, unsigned tiles_m, unsigned tiles_n, Epilogue ep) {
+    typedef Plan<T, LA, LB, FMT, VEC, S> P;
+    typedef typename P::TA TA;
+    typedef typename P::TB TB;
+    constexpr int IM = S::IM, IN = S::IN, BK = P::BK;
     extern __shared__ __attribute__((aligned(16))) short smem[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-    const int64_t m0 = (int64_t)blockIdx.x * TM, n0 = (int64_t)blockIdx.y * TN;
-    const int64_t kb = (int64_t)blockIdx.z * k_per_split, ke = kb + k_per_split < K ? kb + k_per_split : K;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+    const Place at = place_of(blockIdx.x, gridDim.x, tiles_m, tiles_n);
+    const int64_t m0 = (int64_t)at.m * S::TM, n0 = (int64_t)at.n * S::TN;
+    const int64_t kb = at.part * k_per_part, ke = kb + k_per_part < K ? kb + k_per_part : K;
     f32x16 acc[IM][IN];
 #pragma unroll
     for (int i = 0; i < IM; ++i)
@@ -200,6 +328,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operand A, Operan
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     TA a;
     TB b;
+    a.start(A, m0, kb);
+    b.start(B, n0, kb);
     a.load(A, m0, kb, K);
     b.load(B, n0, kb, K);
     a.store(smem);
@@ -212,7 +342,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operand A, Operan
             a.load(A, m0, k0 + BK, K);
             b.load(B, n0, k0 + BK, K);
         }
-        const short *la = smem + buf * BUF, *lb = la + TA::HALFS;
+        const short *la = smem + buf * P::BUF, *lb = la + TA::HALFS;
 #pragma unroll
         for (int ks = 0; ks < BK / 16; ++ks) {
             typename TA::frag fa[TA::PLANES][IM];
@@ -236,46 +366,102 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operand A, Operan
                             for (int j = 0; j < IN; ++j) acc[i][j] = mfma(fa[p][i], fb[q][j], acc[i][j]);
         }
         if (more) {
-            a.store(smem + (buf ^ 1) * BUF);
-            b.store(smem + (buf ^ 1) * BUF + TA::HALFS);
+            a.store(smem + (buf ^ 1) * P::BUF);
+            b.store(smem + (buf ^ 1) * P::BUF + TA::HALFS);
         }
         __syncthreads();
     }
-    // a lane holds column lane & 31 of a 32 x 32 block, rows (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
+    const int64_t M = A.rows, N = B.rows;
+    if (OUT == OUT_SLAB) {
+        // float32, as it lies: a lane holds column lane & 31 of a 32 x 32 block, rows (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
+        float* out = reinterpret_cast<float*>(ep.out) + (int64_t)at.part * M * N;
 #pragma unroll
-    for (int j = 0; j < IN; ++j) {
-        const int64_t n = n0 + (wn * IN + j) * 32 + (lane & 31);
-        if (n >= B.rows) continue;
-        const float bias = OUT == OUT_FORWARD && ep.bias ? (float)reinterpret_cast<const T*>(ep.bias)[n] : 0.f;
+        for (int j = 0; j < IN; ++j) {
+            const int64_t n = n0 + (wn * IN + j) * 32 + (lane & 31);
 #pragma unroll
-        for (int i = 0; i < IM; ++i)
+            for (int i = 0; i < IM; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int64_t m = m0 + (wm * IM + i) * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
-                if (m >= A.rows) continue;
-                float v = acc[i][j][e];
-                if (OUT == OUT_SLAB) {
-                    reinterpret_cast<float*>(ep.out)[((int64_t)blockIdx.z * A.rows + m) * B.rows + n] = v;
-                    continue;
+                for (int e = 0; e < 16; ++e) {
+                    const int64_t m = m0 + (wm * IM + i) * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+                    if (n < N && m < M) out[m * N + n] = acc[i][j][e];
                 }
-                if (OUT == OUT_FORWARD) {
-                    v += bias;
-                    if (ep.z) reinterpret_cast<T*>(ep.z)[m * B.rows + n] = (T)v;
-                    v = act_value(v, ep.act);
-                    if (ep.res) v += (float)reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
-                }
-                reinterpret_cast<T*>(ep.out)[m * ep.ld_out + n] = (T)v;
+        }
+        return;
+    }
+    // Through LDS, 32 rows of the wave's own at a time (no barrier), so that a lane takes 16 bytes of a row: 16-byte loads and stores of whole lines.  Rows that do not
+    // start on 16 bytes: a lane takes single columns, 64 (32) lanes a row.
+    float* epi = reinterpret_cast<float*>(smem) + wave * 32 * P::EPI_STRIDE;
+    constexpr int COLS = IN * 32, E = 16 / sizeof(T), LPR = COLS / E, RPP = 64 / LPR;
+    const int64_t nw = n0 + wn * COLS;
+    const bool wide = ep.wide;
+    const int64_t n = nw + (wide ? lane % LPR * E : lane % COLS);
+    float bias[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) bias[i] = 0.f;
+    if (OUT == OUT_FORWARD && ep.bias && n < N) {
+        const T* src = reinterpret_cast<const T*>(ep.bias) + n;
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) bias[i] = (float)src[i];
+        } else bias[0] = (float)src[0];
+    }
+#pragma unroll
+    for (int i = 0; i < IM; ++i) {
+        const int64_t mw = m0 + (wm * IM + i) * 32;
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) epi[((e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * P::EPI_STRIDE + j * 32 + (lane & 31)] = acc[i][j][e];
+        if (wide) {
+            papr_pack<T, E> res[32 / RPP];
+#pragma unroll
+            for (int r = 0; r < 32 / RPP; ++r) {
+                const int64_t m = mw + r * RPP + lane / LPR;
+                if (OUT == OUT_FORWARD && ep.res && m < M && n < N) res[r] = *reinterpret_cast<const papr_pack<T, E>*>(reinterpret_cast<const T*>(ep.res) + m * ep.ld_res + n);
             }
+#pragma unroll
+            for (int r = 0; r < 32 / RPP; ++r) {
+                const int64_t m = mw + r * RPP + lane / LPR;
+                float v[E];
+#pragma unroll
+                for (int c = 0; c < E; c += 4) {
+                    const float4 t = *reinterpret_cast<const float4*>(epi + (r * RPP + lane / LPR) * P::EPI_STRIDE + lane % LPR * E + c);
+                    v[c] = t.x; v[c + 1] = t.y; v[c + 2] = t.z; v[c + 3] = t.w;
+                }
+                if (m < M && n < N) finish<T, OUT, E>(v, m, n, N, bias, res[r], ep);
+            }
+        } else {
+            constexpr int ROWS = 64 / COLS;
+#pragma unroll 4
+            for (int r = 0; r < 32; r += ROWS) {
+                const int64_t m = mw + r + lane / COLS;
+                float v[1] = {epi[(r + lane / COLS) * P::EPI_STRIDE + lane % COLS]};
+                const float b1[1] = {bias[0]};
+                if (m < M && n < N) {
+                    papr_pack<T, 1> res;
+                    if (OUT == OUT_FORWARD && ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
+                    finish<T, OUT, 1>(v, m, n, N, b1, res, ep);
+                }
+            }
+        }
     }
 }
 
-// the slabs of a split sum, added in split order
+// The slabs of a sum in parts: a workgroup takes 64 results, its four waves a quarter of the parts each, quarters added in order.
 template <typename T>
-__global__ __launch_bounds__(256) void join_slabs_kernel(const float* __restrict__ slab, int64_t n, int splits, T* __restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void join_slabs_kernel(const float* __restrict__ slab, int64_t n, int parts, T* __restrict__ out) {
+    __shared__ float lds[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (parts + 3) / 4;
+    for (int64_t i0 = (int64_t)blockIdx.x * 64; i0 < n; i0 += (int64_t)gridDim.x * 64) {
+        const int64_t i = i0 + lane < n ? i0 + lane : n - 1;
+        const int end = (wave + 1) * per < parts ? (wave + 1) * per : parts;
         float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += slab[k * n + i];
-        out[i] = (T)s;
+#pragma unroll 8
+        for (int k = wave * per; k < end; ++k) s += slab[k * n + i];
+        lds[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0 && i0 + lane < n) out[i] = (T)((lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]));
+        __syncthreads();
     }
 }
 
@@ -298,11 +484,14 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
             auto g = *reinterpret_cast<const papr_pack<T, V>*>(d_y + m * ld + c);
             if (d_z) {
                 const auto t = *reinterpret_cast<const papr_pack<T, V>*>(z + m * N + c);
+                float v[V], zv[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) { v[i] = (float)g.v[i]; zv[i] = (float)t.v[i]; }
+                act_slopes<sizeof(T) == 4>(v, zv, act);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float v = (float)g.v[i] * act_slope((float)t.v[i], act);
-                    sum[i] += v;
-                    g.v[i] = (T)v;
+                    sum[i] += v[i];
+                    g.v[i] = (T)v[i];
                 }
                 *reinterpret_cast<papr_pack<T, V>*>(d_z + m * N + c) = g;
             } else {
@@ -322,70 +511,90 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
     }
 }
 
-constexpr int TILE = 128;
+typedef Shape<2, 4, 4, 2> Large;                   // 256 x 256, eight waves
+typedef Shape<2, 2, 2, 2> Middle;                  // 128 x 128, four waves
+typedef Shape<2, 2, 1, 1> Small;                   // 64 x 64, four waves
 
-int64_t splits_for(int64_t M, int64_t N, int64_t K, int bk) {
-    // enough workgroups for two on every compute unit, at least eight steps of the sum in each
-    const int64_t tiles = ((M + TILE - 1) / TILE) * ((N + TILE - 1) / TILE), steps = (K + bk - 1) / bk;
-    int64_t s = 2 * (int64_t)papr_cu_count() / tiles;
-    if (s > steps / 8) s = steps / 8;
-    if (s > 1024) s = 1024;
-    return s < 1 ? 1 : s;
+// Which tile, and into how many parts the sum is cut: the least estimated time.  A tile's time is its area times the steps of its part over the rate its shape
+// reaches, the launch as many of them in turn as a compute unit gets; parts cost their slabs' way to memory and back.
+struct Choice { int shape; int64_t parts, per; };      // per: terms of a part
+int step_of(int type) { return type == PAPR_TYPE_F32 ? 32 : 64; }
+Choice choose(int64_t M, int64_t N, int64_t K, int type, bool may_split) {
+    const int bk = step_of(type);
+    const int64_t cus = papr_cu_count(), steps = (K + bk - 1) / bk;
+    static const int side[3] = {256, 128, 64}, resident[3] = {1, 2, 4};
+    static const double rate[3] = {1.0, 0.8, 0.45};
+    Choice best = {0, 1, 0};
+    double least = 0;
+    for (int s = 0; s < 3; ++s) {
+        const int64_t tiles = ((M + side[s] - 1) / side[s]) * ((N + side[s] - 1) / side[s]), slots = cus * resident[s];
+        int64_t tried[3] = {1, slots / tiles, 2 * slots / tiles};
+        for (int64_t parts : tried) {
+            if (parts > steps / 4) parts = steps / 4;
+            if (parts > 1024) parts = 1024;
+            if (parts < 1 || !may_split) parts = 1;
+            const int64_t per = (steps + parts - 1) / parts;
+            parts = (steps + per - 1) / per;
+            const int64_t turns = (tiles * parts + slots - 1) / slots;
+            // (in matrix instruction time of one compute unit: 4096 products of a 16-bit type a cycle; slabs at 2 KB a cycle over the chip; 3 us a launch)
+            double t = (double)turns * resident[s] * ((double)side[s] * side[s] * (per + 3) * bk / (4096 * rate[s]));
+            if (parts > 1) t += 2.0 * parts * M * N * 4 / 2048 + 7000;
+            if (least == 0 || t < least) { least = t; best = {s, parts, per * bk}; }
+        }
+    }
+    return best;
 }
 
-template <typename T, int LA, int LB, int FMT, bool VEC, int OUT>
-int launch_product(const Operand& A, const Operand& B, int64_t K, int64_t splits, const Epilogue& ep, hipStream_t s) {
-    constexpr int WM = 2, WN = 2, IM = 2, IN = 2, BK = sizeof(T) == 4 ? 32 : 64;
-    typedef Tile<T, LA, 0, VEC, TILE, BK, 256> TA;
-    typedef Tile<T, LB, FMT, VEC, TILE, BK, 256> TB;
-    constexpr size_t lds = 2 * (TA::HALFS + TB::HALFS) * 2;
-    auto kernel = product_kernel<T, LA, LB, FMT, VEC, OUT, WM, WN, IM, IN>;
-    const int64_t steps = (K + BK - 1) / BK, per = (steps + splits - 1) / splits * BK;
-    const dim3 grid((unsigned)((A.rows + TILE - 1) / TILE), (unsigned)((B.rows + TILE - 1) / TILE), (unsigned)((K + per - 1) / per));
+template <typename T, int LA, int LB, int FMT, bool VEC, int OUT, typename S>
+int launch_shape(const Operand& A, const Operand& B, int64_t K, const Choice& c, const Epilogue& ep, hipStream_t s) {
+    typedef Plan<T, LA, LB, FMT, VEC, S> P;
+    static_assert(P::LDS <= 160 * 1024, "a compute unit's LDS");
+    auto kernel = product_kernel<T, LA, LB, FMT, VEC, OUT, S>;
+    static_assert(32 % P::BK == 0 || 64 % P::BK == 0, "parts are whole steps");
+    const int64_t tm = (A.rows + S::TM - 1) / S::TM, tn = (B.rows + S::TN - 1) / S::TN, grid = tm * tn * c.parts;
+    PAPR_REQUIRE(grid < (int64_t)1 << 31, "papr_linear: %lld tiles", (long long)grid);
     static std::atomic<uint64_t> ready{0};            // (devices on which this kernel may already use more than 64 KB of LDS)
     int dev = 0;
     (void)hipGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
-    if (lds > 65536 && !(ready.load(std::memory_order_relaxed) & bit)) {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (P::LDS > 65536 && !(ready.load(std::memory_order_relaxed) & bit)) {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)P::LDS);
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
-    kernel<<<grid, dim3(256), lds, s>>>(A, B, K, per, ep);
+    kernel<<<dim3((unsigned)grid), dim3(S::THREADS), P::LDS, s>>>(A, B, K, c.per, (unsigned)tm, (unsigned)tn, ep);
     PAPR_CHECK_LAUNCH("papr_linear product");
     return 0;
 }
 
 template <typename T, int LA, int LB, int FMT, int OUT>
-int launch_aligned(bool vec, const Operand& A, const Operand& B, int64_t K, int64_t splits, const Epilogue& ep, hipStream_t s) {
-    return vec ? launch_product<T, LA, LB, FMT, true, OUT>(A, B, K, splits, ep, s) : launch_product<T, LA, LB, FMT, false, OUT>(A, B, K, splits, ep, s);
+int launch_product(const Choice& c, bool vec, const Operand& A, const Operand& B, int64_t K, const Epilogue& ep, hipStream_t s) {
+    if (c.shape == 0) return vec ? launch_shape<T, LA, LB, FMT, true, OUT, Large>(A, B, K, c, ep, s) : launch_shape<T, LA, LB, FMT, false, OUT, Large>(A, B, K, c, ep, s);
+    if (c.shape == 1) return vec ? launch_shape<T, LA, LB, FMT, true, OUT, Middle>(A, B, K, c, ep, s) : launch_shape<T, LA, LB, FMT, false, OUT, Middle>(A, B, K, c, ep, s);
+    return vec ? launch_shape<T, LA, LB, FMT, true, OUT, Small>(A, B, K, c, ep, s) : launch_shape<T, LA, LB, FMT, false, OUT, Small>(A, B, K, c, ep, s);
 }
 
-// C = A B^T into rows of type T, the sum split where the tiles alone do not fill the chip
+// C = A B^T into contiguous rows of type T, the sum in parts where the tiles alone do not fill the chip
 template <typename T, int LA, int LB, int FMT>
 int rows_product(bool vec, const Operand& A, const Operand& B, int64_t K, void* out, float* slab, hipStream_t s) {
-    constexpr int BK = sizeof(T) == 4 ? 32 : 64;
-    const int64_t steps = (K + BK - 1) / BK;
-    int64_t splits = slab ? splits_for(A.rows, B.rows, K, BK) : 1;
-    const int64_t per = (steps + splits - 1) / splits;
-    splits = (steps + per - 1) / per;
+    const Choice c = choose(A.rows, B.rows, K, sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, true);
     Epilogue ep = {};
-    if (splits == 1) {
+    if (c.parts == 1) {
         ep.out = out;
-        ep.ld_out = B.rows;
-        return launch_aligned<T, LA, LB, FMT, OUT_ROWS>(vec, A, B, K, 1, ep, s);
+        ep.wide = ((uintptr_t)out & 15) == 0 && (B.rows * sizeof(T)) % 16 == 0;
+        return launch_product<T, LA, LB, FMT, OUT_ROWS>(c, vec, A, B, K, ep, s);
     }
     ep.out = slab;
-    if (int rc = launch_aligned<T, LA, LB, FMT, OUT_SLAB>(vec, A, B, K, splits, ep, s)) return rc;
-    const int64_t n = A.rows * B.rows, need = (n + 255) / 256, cap = (int64_t)papr_cu_count() * 16;
-    join_slabs_kernel<T><<<dim3((unsigned)(need < cap ? need : cap)), dim3(256), 0, s>>>(slab, n, (int)splits, (T*)out);
+    if (int rc = launch_product<T, LA, LB, FMT, OUT_SLAB>(c, vec, A, B, K, ep, s)) return rc;
+    const int64_t n = A.rows * B.rows, need = (n + 63) / 64, cap = (int64_t)papr_cu_count() * 16;
+    join_slabs_kernel<T><<<dim3((unsigned)(need < cap ? need : cap)), dim3(256), 0, s>>>(slab, n, (int)c.parts, (T*)out);
     PAPR_CHECK_LAUNCH("papr_linear slabs");
     return 0;
 }
 
-// float32 slabs of a weight gradient (N, K) summed over M rows
+// float32 slabs of one product
 size_t slab_floats(int type, int64_t M, int64_t N, int64_t K) {
-    const int64_t s = splits_for(N, K, M, type == PAPR_TYPE_F32 ? 32 : 64);
-    return s > 1 ? (size_t)(s * N * K) : 0;
+    const int64_t parts = choose(M, N, K, type, true).parts;
+    return parts > 1 ? (size_t)(parts * M * N) : 0;
 }
 
 struct SlopeGrid { int lanes; int64_t blocks, rows_per_block; unsigned cols; };
@@ -425,8 +634,10 @@ extern "C" int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t
     const int b = papr_type_bytes(d->type);
     const bool vec = papr_rows_aligned(x, ldx, d->K, b) && papr_rows_aligned(w, ldw, d->K, b);
     const Operand A = {x, ldx, d->M, nullptr}, B = {w, ldw, d->N, nullptr};
-    const Epilogue ep = {y, d->N, bias, res, ld_res, z, d->act};
-    PAPR_TYPE_SWITCH(d->type, return launch_aligned<T, K_RUNS, K_RUNS, 0, OUT_FORWARD>(vec, A, B, d->K, 1, ep, as_stream(stream)));
+    const Epilogue ep = {y, bias, res, ld_res, z, d->act,
+                         papr_rows_aligned(y, d->N, d->N, b) && (!z || ((uintptr_t)z & 15) == 0) && (!res || papr_rows_aligned(res, ld_res, d->N, b))};
+    const Choice c = choose(d->M, d->N, d->K, d->type, false);
+    PAPR_TYPE_SWITCH(d->type, return (launch_product<T, K_RUNS, K_RUNS, 0, OUT_FORWARD>(c, vec, A, B, d->K, ep, as_stream(stream))));
 }
 
 extern "C" size_t papr_linear_bwd_workspace_bytes(const papr_linear_desc* d) {
@@ -437,7 +648,8 @@ extern "C" size_t papr_linear_bwd_workspace_bytes(const papr_linear_desc* d) {
         const size_t p = (size_t)slope_grid(d->M, (int)d->N, piece).blocks * d->N * sizeof(float);
         part = p > part ? p : part;
     }
-    return dz + up16(part) + slab_floats(d->type, d->M, d->N, d->K) * sizeof(float);
+    const size_t sx = slab_floats(d->type, d->M, d->K, d->N), sw = slab_floats(d->type, d->N, d->K, d->M);
+    return dz + up16(part) + (sx > sw ? sx : sw) * sizeof(float);
 }
 
 extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64_t ld_dy, const void* z, const void* x, int64_t ldx, const void* exps, const void* w, int64_t ldw,
@@ -486,7 +698,7 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
         const Operand A = {g, ldg, M, nullptr}, B = {w, ldw, K, nullptr};
         const bool vec = vg && papr_rows_aligned(w, ldw, K, b);
         int rc = 0;
-        PAPR_TYPE_SWITCH(d->type, rc = (rows_product<T, K_RUNS, ROWS_RUN, 0>(vec, A, B, N, d_x, nullptr, s)));
+        PAPR_TYPE_SWITCH(d->type, rc = (rows_product<T, K_RUNS, ROWS_RUN, 0>(vec, A, B, N, d_x, slab, s)));
         if (rc) return rc;
     }
     if (d_w) {
