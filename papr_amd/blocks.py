@@ -53,10 +53,12 @@ def _check_device(who, x, *others):
 
 def _rows(t, width):
     """t as (rows, width) with unit column stride and rows that do not overlap; a copy only where its strides ask for one."""
-    t = t.detach()
+    if t.requires_grad:
+        t = t.detach()
     if t.dim() != 2:
         t = t.reshape(-1, width)
-    if t.numel() and ((width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width)):
+    down, across = t.stride()
+    if (across != 1 and width > 1) or (down < width and t.shape[0] > 1):
         t = t.contiguous()
     return t
 
@@ -69,25 +71,27 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """The rows' device as the current one, and its stream (the library launches on the current device)."""
+_stream = torch._C._cuda_getCurrentRawStream
 
-    def __init__(self, dev):
-        self.guard = torch.cuda.device(dev) if torch.cuda.current_device() != dev.index else None
-        self.index = dev.index
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(what, dev, fn, *args):
+    """fn(*args, stream) on the rows' device (the library launches on the current one) and its current stream."""
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:
+        code = fn(*args, _stream(i))
+    else:
+        with torch.cuda.device(i):
+            code = fn(*args, _stream(i))
+    if code or hip.DEBUG_SYNC:
+        hip.check(code, what)
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---------------------------------------------------------------------------------------------- rows in 8 bits
@@ -104,9 +108,8 @@ class PackedRows:
     def rows(self):
         """The values they stand for, in the type and shape that was packed."""
         out = torch.empty(self.shape, device=self.codes.device, dtype=self.dtype)
-        with _on(out.device) as s:
-            hip.check(hip.lib().papr_rows8_unpack(TYPES[self.dtype], KEEPS[self.fmt], _p(self.codes), _p(self.exps), self.codes.shape[0], self.shape[-1], _p(out), s),
-                      "papr_rows8_unpack")
+        _launch("papr_rows8_unpack", out.device, hip.lib().papr_rows8_unpack, TYPES[self.dtype], KEEPS[self.fmt], self.codes.data_ptr(), self.exps.data_ptr(),
+                self.codes.shape[0], self.shape[-1], out.data_ptr())
         return out
 
 
@@ -118,28 +121,30 @@ def pack_rows(x, fmt="e4m3"):
     if fmt not in KEEPS:
         _fail("pack_rows", "unknown format %r (%s)" % (fmt, ", ".join(KEEPS)))
     _check_device("pack_rows", x)
-    width = x.shape[-1]
-    rows = _rows(x, width)
-    n, blocks = rows.shape[0], (width + BLOCK - 1) // BLOCK
-    codes = torch.empty((n, blocks * BLOCK), device=x.device, dtype=torch.uint8)
-    exps = torch.empty((n, blocks), device=x.device, dtype=torch.uint8)
-    with _on(x.device) as s:
-        hip.check(hip.lib().papr_rows8_pack(TYPES[x.dtype], KEEPS[fmt], _p(rows), _ld(rows), n, width, _p(codes), _p(exps), s), "papr_rows8_pack")
-    return PackedRows(codes, exps, fmt, tuple(x.shape), x.dtype)
+    return _pack(_rows(x, x.shape[-1]), fmt, x.shape)
+
+
+def _pack(rows, fmt, shape):
+    n, width = rows.shape
+    blocks = (width + BLOCK - 1) // BLOCK
+    codes = torch.empty((n, blocks * BLOCK), device=rows.device, dtype=torch.uint8)
+    exps = torch.empty((n, blocks), device=rows.device, dtype=torch.uint8)
+    _launch("papr_rows8_pack", rows.device, hip.lib().papr_rows8_pack, TYPES[rows.dtype], KEEPS[fmt], rows.data_ptr(), _ld(rows), n, width, codes.data_ptr(), exps.data_ptr())
+    return PackedRows(codes, exps, fmt, shape, rows.dtype)
 
 
 # ---------------------------------------------------------------------------------------------- linear layers
 def _linear_call(x, weight, bias, residual, act, want_z):
-    """(y, z or None) of 2-D rows"""
+    """(y, z or None, descriptor) of 2-D rows"""
     M, K = x.shape
     N = weight.shape[0]
-    y = torch.empty((M, N), device=x.device, dtype=x.dtype)
-    z = torch.empty_like(y) if want_z else None
-    d = hip.LinearDesc(TYPES[x.dtype], act, 0, 0, M, N, K)
-    with _on(x.device) as s:
-        hip.check(hip.lib().papr_linear_fwd(d, _p(x), _ld(x), _p(weight), _ld(weight), _p(bias), _p(residual), 0 if residual is None else _ld(residual), _p(y), _p(z), s),
-                  "papr_linear_fwd")
-    return y, z
+    dt, dev = x.dtype, x.device
+    y = torch.empty((M, N), device=dev, dtype=dt)
+    z = torch.empty((M, N), device=dev, dtype=dt) if want_z else None
+    d = hip.LinearDesc(TYPES[dt], act, 0, 0, M, N, K)
+    _launch("papr_linear_fwd", dev, hip.lib().papr_linear_fwd, d, x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight), _p(bias), _p(residual),
+            0 if residual is None else _ld(residual), y.data_ptr(), _p(z))
+    return y, z, d
 
 
 class _LinearFn(torch.autograd.Function):
@@ -148,37 +153,39 @@ class _LinearFn(torch.autograd.Function):
         K, N = weight.shape[1], weight.shape[0]
         need = ctx.needs_input_grad
         rows, w2 = _rows(x, K), _rows(weight, K)
-        y, z = _linear_call(rows, w2, None if bias is None else bias.detach().contiguous(), None if residual is None else _rows(residual, N), act,
-                            act != 0 and any(need[:3]))
-        packed = pack_rows(rows, keep) if keep is not None and need[1] else None
+        y, z, d = _linear_call(rows, w2, None if bias is None else bias.detach().contiguous(), None if residual is None else _rows(residual, N), act,
+                               act != 0 and (need[0] or need[1] or need[2]))
+        packed = _pack(rows, keep, rows.shape) if keep is not None and need[1] else None
         held = None if not need[1] else rows if packed is None else packed.codes
         ctx.save_for_backward(held, None if packed is None else packed.exps, w2 if need[0] else None, z)
-        ctx.act, ctx.keep, ctx.dims, ctx.shapes = act, keep if packed is not None else None, (rows.shape[0], N, K), (x.shape, weight.shape)
-        return y.reshape(x.shape[:-1] + (N,))
+        if packed is not None:
+            d.keep = KEEPS[keep]
+        ctx.desc, ctx.shapes = d, (x.shape, weight.shape)
+        return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (N,))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_y):
         held, exps, w2, z = ctx.saved_tensors
-        M, N, K = ctx.dims
-        need = ctx.needs_input_grad
-        d_res = d_y if need[3] else None
-        if not any(need[:3]):
+        d = ctx.desc
+        M, N, K = d.M, d.N, d.K
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        d_res = d_y if need_r else None
+        if not (need_x or need_w or need_b):
             return None, None, None, d_res, None, None
         dev, dt = d_y.device, d_y.dtype
+        x_shape, w_shape = ctx.shapes
         if M == 0:
-            return (d_y.new_zeros(ctx.shapes[0]) if need[0] else None, d_y.new_zeros(ctx.shapes[1]) if need[1] else None, d_y.new_zeros(N) if need[2] else None,
-                    d_res, None, None)
+            return (d_y.new_zeros(x_shape) if need_x else None, d_y.new_zeros(w_shape) if need_w else None, d_y.new_zeros(N) if need_b else None, d_res, None, None)
         g = _rows(d_y, N)
-        new = lambda *shape: torch.empty(shape, device=dev, dtype=dt)
-        d_x, d_w, d_b = new(M, K) if need[0] else None, new(N, K) if need[1] else None, new(N) if need[2] else None
-        d = hip.LinearDesc(TYPES[dt], ctx.act, KEEPS.get(ctx.keep, 0), 0, M, N, K)
+        d_x = torch.empty((M, K), device=dev, dtype=dt) if need_x else None
+        d_w = torch.empty((N, K), device=dev, dtype=dt) if need_w else None
+        d_b = torch.empty((N,), device=dev, dtype=dt) if need_b else None
         lib = hip.lib()
-        with _on(dev) as s:
-            ws = torch.empty(max(int(lib.papr_linear_bwd_workspace_bytes(d)), 16), device=dev, dtype=torch.uint8)
-            hip.check(lib.papr_linear_bwd(d, _p(g), _ld(g), _p(z), _p(held), 0 if held is None else _ld(held), _p(exps), _p(w2), 0 if w2 is None else _ld(w2),
-                                          _p(d_x), _p(d_w), _p(d_b), _p(ws), s), "papr_linear_bwd")
-        return None if d_x is None else d_x.reshape(ctx.shapes[0]), d_w, d_b, d_res, None, None
+        ws = torch.empty(lib.papr_linear_bwd_workspace_bytes(d) + 16, device=dev, dtype=torch.uint8)
+        _launch("papr_linear_bwd", dev, lib.papr_linear_bwd, d, g.data_ptr(), _ld(g), _p(z), _p(held), 0 if held is None else _ld(held), _p(exps), _p(w2),
+                0 if w2 is None else _ld(w2), _p(d_x), _p(d_w), _p(d_b), ws.data_ptr())
+        return d_x if d_x is None or len(x_shape) == 2 else d_x.reshape(x_shape), d_w, d_b, d_res, None, None
 
 
 def linear_rows(x, weight, bias=None, residual=None, act="none", keep=None):
@@ -188,6 +195,29 @@ def linear_rows(x, weight, bias=None, residual=None, act="none", keep=None):
     keep = "e4m3" / "int8": in training the rows x are held for the weight's gradient as pack_rows keeps them -- a quarter (float32) or half of the memory -- and that
     gradient is d_z^T times the values they stand for; y and every other gradient are those of keep=None.  An activation's argument is held in the rows' type.  float32
     rows with infinities give NaN."""
+    if not _linear_fits(x, weight, bias, residual, act, keep):
+        _explain_linear(x, weight, bias, residual, act, keep)
+    if _wants_grad(x, weight, bias, residual):
+        return _LinearFn.apply(x, weight, bias, residual, ACTS[act], keep)
+    K = x.shape[-1]
+    y = _linear_call(_rows(x, K), _rows(weight, K), None if bias is None else bias.contiguous(), None if residual is None else _rows(residual, weight.shape[0]),
+                     ACTS[act], False)[0]
+    return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (weight.shape[0],))
+
+
+def _linear_fits(x, weight, bias, residual, act, keep):
+    """Everything in order?  (One pass of cheap comparisons: a serving call is over in microseconds; what is wrong is _explain_linear's to say.)"""
+    if not (isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and x.is_cuda and x.dim() and weight.dim() == 2):
+        return False
+    dt, dev, (N, K) = x.dtype, x.device, weight.shape
+    if dt not in TYPES or weight.dtype != dt or weight.device != dev or x.shape[-1] != K or K < 1 or N < 1 or act not in ACTS or not (keep is None or keep in KEEPS):
+        return False
+    if bias is not None and not (isinstance(bias, torch.Tensor) and bias.dtype == dt and bias.shape == (N,) and bias.device == dev):
+        return False
+    return residual is None or (isinstance(residual, torch.Tensor) and residual.dtype == dt and residual.device == dev and residual.shape == x.shape[:-1] + (N,))
+
+
+def _explain_linear(x, weight, bias, residual, act, keep):
     who = "linear_rows"
     _check_rows(who, "x", x)
     if act not in ACTS:
@@ -208,32 +238,46 @@ def linear_rows(x, weight, bias=None, residual=None, act="none", keep=None):
         if t is not None and t.dtype != x.dtype:
             _fail(who, "%s is %s, x %s" % (name, t.dtype, x.dtype))
     _check_device(who, x, weight, bias, residual)
-    if _wants_grad(x, weight, bias, residual):
-        return _LinearFn.apply(x, weight, bias, residual, ACTS[act], keep)
-    K = x.shape[-1]
-    y, _ = _linear_call(_rows(x, K), _rows(weight, K), None if bias is None else bias.detach().contiguous(), None if residual is None else _rows(residual, N), ACTS[act], False)
-    return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (N,))
+    _fail(who, "arguments that do not fit")
 
 
 # ---------------------------------------------------------------------------------------------- the joint of a block
-def _join_desc(x, f, gate, scale, scale_cols, norms, gate_act):
-    """The descriptor of a call over 2-D rows; norms = ((kind, gain, shift, eps) of the block's output, of the next block)."""
-    rows, width = x.shape
-    form = 0 if gate is None else 2 if gate.shape[1] == width else 1
-    ns = [hip.BlockNorm(kind, TYPES[gain.dtype] if gain is not None else TYPES[shift.dtype] if shift is not None else 0, eps, 0, _p(gain), _p(shift))
-          for kind, gain, shift, eps in norms]
-    return hip.JoinDesc(rows, width, TYPES[x.dtype], _p(x), _ld(x), _p(f), 0 if f is None else _ld(f), _p(gate), 0 if gate is None else _ld(gate), form, gate_act,
-                        _p(scale_cols), 0 if scale_cols is None else TYPES[scale_cols.dtype], scale, ns[0], ns[1])
+def _flat(t):
+    if t is None:
+        return None
+    return (t.detach() if t.requires_grad else t).contiguous()
 
 
-def _join_call(d, like, want_y, want_h, want_stats):
-    rows, width = like.shape
-    y = torch.empty((rows, width), device=like.device, dtype=like.dtype) if want_y else None
-    h = torch.empty((rows, width), device=like.device, dtype=like.dtype) if want_h else None
-    stats = torch.empty((rows, 6), device=like.device, dtype=torch.float32) if want_stats else None
-    with _on(like.device) as s:
-        hip.check(hip.lib().papr_join_fwd(d, _p(y), _p(h), _p(stats), s), "papr_join_fwd")
-    return y, h, stats
+class _Joint:
+    """One call's operands as the library takes them: 2-D rows, contiguous parameters, the descriptor over them."""
+    __slots__ = ("x", "f", "gate", "params", "desc", "has_h")
+
+    def __init__(self, x, f, gate, scale_cols, post_gain, post_shift, pre_gain, pre_shift, meta):
+        scale, post_kind, post_eps, pre_kind, pre_eps, gate_act = meta
+        width = x.shape[-1]
+        self.x = x = _rows(x, width)
+        self.f = f = None if f is None else _rows(f, width)
+        form = 0
+        if gate is not None:
+            form = 2 if gate.shape[-1] == width else 1
+            gate = _rows(gate, gate.shape[-1])
+        self.gate = gate
+        self.params = p = (_flat(scale_cols), _flat(post_gain), _flat(post_shift), _flat(pre_gain), _flat(pre_shift))
+        self.has_h = pre_kind is not None
+        norm = lambda kind, eps, gain, shift: hip.BlockNorm(kind, 0 if gain is None and shift is None else TYPES[(shift if gain is None else gain).dtype], eps, 0,
+                                                            _p(gain), _p(shift))
+        self.desc = hip.JoinDesc(x.shape[0], width, TYPES[x.dtype], x.data_ptr(), _ld(x), _p(f), 0 if f is None else _ld(f), _p(gate), 0 if gate is None else _ld(gate),
+                                 form, gate_act, _p(p[0]), 0 if p[0] is None else TYPES[p[0].dtype], scale, norm(post_kind, post_eps, p[1], p[2]),
+                                 norm(pre_kind or 0, pre_eps, p[3], p[4]))
+
+    def run(self, want_stats):
+        x = self.x
+        shape, dt, dev = x.shape, x.dtype, x.device
+        y = None if self.f is None else torch.empty(shape, device=dev, dtype=dt)
+        h = torch.empty(shape, device=dev, dtype=dt) if self.has_h else None
+        stats = torch.empty((shape[0], 6), device=dev, dtype=torch.float32) if want_stats else None
+        _launch("papr_join_fwd", dev, hip.lib().papr_join_fwd, self.desc, _p(y), _p(h), _p(stats))
+        return y, h, stats
 
 
 class _JoinFn(torch.autograd.Function):
@@ -241,53 +285,46 @@ class _JoinFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, f, gate, scale_cols, post_gain, post_shift, pre_gain, pre_shift, meta):
-        scale, post, pre, gate_act = meta
-        width = x.shape[-1]
-        two = lambda t, w=width: None if t is None else _rows(t, w)
-        flat = lambda t: None if t is None else t.detach().contiguous()
-        xr, fr, gr = two(x), two(f), two(gate, None if gate is None else gate.shape[-1])
-        params = [flat(t) for t in (scale_cols, post_gain, post_shift, pre_gain, pre_shift)]
-        d = _join_desc(xr, fr, gr, scale, params[0], ((post[0], params[1], params[2], post[1]), (pre[0], params[3], params[4], pre[1]) if pre else (0, None, None, 0.0)), gate_act)
-        y, h, stats = _join_call(d, xr, f is not None, pre is not None, True)
-        ctx.save_for_backward(xr, fr, gr, stats, *params)
-        ctx.meta, ctx.shapes = meta, (x.shape, None if gate is None else gate.shape)
+        j = _Joint(x, f, gate, scale_cols, post_gain, post_shift, pre_gain, pre_shift, meta)
+        y, h, stats = j.run(True)
+        ctx.save_for_backward(j.x, j.f, j.gate, stats, *j.params)
+        ctx.desc, ctx.has_h, ctx.shapes = j.desc, j.has_h, (x.shape, None if gate is None else gate.shape)      # (the descriptor points at the saved tensors)
         ctx.set_materialize_grads(False)
-        out = [t.reshape(x.shape) for t in (y, h) if t is not None]
-        return tuple(out) if len(out) > 1 else out[0]
+        if x.dim() != 2:
+            y, h = (None if t is None else t.reshape(x.shape) for t in (y, h))
+        return h if y is None else y if h is None else (y, h)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *d_out):
-        xr, fr, gr, stats = ctx.saved_tensors[:4]
-        params = ctx.saved_tensors[4:]
-        scale, post, pre, gate_act = ctx.meta
+        saved = ctx.saved_tensors                      # (refuses operands that were written to in between)
+        xr, fr, gr, stats = saved[:4]
+        params = saved[4:]
         need = ctx.needs_input_grad
         rows, width = xr.shape
         dev, dt = xr.device, xr.dtype
-        d_out = list(d_out)
-        d_y = d_out.pop(0) if fr is not None else None
-        d_h = d_out.pop(0) if pre else None
-        none = (None,) * 9
+        d_y = d_out[0] if fr is not None else None
+        d_h = d_out[-1] if ctx.has_h else None
         if d_y is None and d_h is None:
-            return none
-        full = lambda t: None if t is None else t.reshape(rows, width).contiguous()
-        d_y, d_h = full(d_y), full(d_h)
-        new = lambda *shape: torch.empty(shape, device=dev, dtype=dt)
-        d_x = new(rows, width) if need[0] else None
-        d_f = new(rows, width) if need[1] else None
-        d_g = new(rows, gr.shape[1]) if need[2] else None
-        # scale, post gain, post shift, pre gain, pre shift (the last two have none without d_h)
-        d_p = [torch.empty_like(p) if need[3 + i] and p is not None else None for i, p in enumerate(params)]
-        d = _join_desc(xr, fr, gr, scale, params[0], ((post[0], params[1], params[2], post[1]), (pre[0], params[3], params[4], pre[1]) if pre else (0, None, None, 0.0)), gate_act)
-        grads = hip.JoinGrads(_p(d_p[3]), _p(d_p[4]), _p(d_p[1]), _p(d_p[2]), _p(d_p[0]))
+            return (None,) * 9
+        if d_y is not None:
+            d_y = d_y.reshape(rows, width).contiguous()
+        if d_h is not None:
+            d_h = d_h.reshape(rows, width).contiguous()
+        d_x = torch.empty((rows, width), device=dev, dtype=dt) if need[0] else None
+        d_f = torch.empty((rows, width), device=dev, dtype=dt) if need[1] else None
+        d_g = torch.empty((rows, gr.shape[1]), device=dev, dtype=dt) if need[2] else None
+        # scale, post gain, post shift, pre gain, pre shift (without d_h the last two are zero)
+        d_p = [torch.empty((width,), device=dev, dtype=p.dtype) if need[3 + i] and p is not None else None for i, p in enumerate(params)]
+        s, pg, ps, qg, qs = [_p(t) for t in d_p]
         lib = hip.lib()
-        with _on(dev) as s:
-            ws = None
-            if any(t is not None for t in d_p):
-                ws = torch.empty(max(int(lib.papr_join_bwd_workspace_bytes(rows, width)), 16), device=dev, dtype=torch.uint8)
-            hip.check(lib.papr_join_bwd(d, _p(stats), _p(d_y), _p(d_h), _p(d_x), _p(d_f), _p(d_g), grads, _p(ws), s), "papr_join_bwd")
-        back = lambda t, shape: None if t is None else t.reshape(shape)
-        return (back(d_x, ctx.shapes[0]), back(d_f, ctx.shapes[0]), back(d_g, ctx.shapes[1])) + tuple(d_p) + (None,)
+        ws = torch.empty(lib.papr_join_bwd_workspace_bytes(rows, width) + 16, device=dev, dtype=torch.uint8) if any(need[3:8]) else None
+        _launch("papr_join_bwd", dev, lib.papr_join_bwd, ctx.desc, stats.data_ptr(), _p(d_y), _p(d_h), _p(d_x), _p(d_f), _p(d_g), hip.JoinGrads(qg, qs, pg, ps, s), _p(ws))
+        shape, g_shape = ctx.shapes
+        if len(shape) != 2:
+            d_x, d_f = (None if t is None else t.reshape(shape) for t in (d_x, d_f))
+            d_g = None if d_g is None else d_g.reshape(g_shape)
+        return (d_x, d_f, d_g, *d_p, None)
 
 
 def _check_norm(who, name, norm, x):
@@ -315,17 +352,13 @@ def _check_width(who, x):
 
 def _join(x, f, gate, scale, scale_cols, post, pre, gate_act):
     tensors = (x, f, gate, scale_cols, post.gain, post.shift) + ((pre.gain, pre.shift) if pre else (None, None))
-    meta = (scale, (NORMS[post.kind], float(post.eps)), (NORMS[pre.kind], float(pre.eps)) if pre else None, gate_act)
+    meta = (scale, NORMS[post.kind], float(post.eps), NORMS[pre.kind] if pre else None, float(pre.eps) if pre else 0.0, gate_act)
     if _wants_grad(*tensors):
         return _JoinFn.apply(*tensors, meta)
-    width = x.shape[-1]
-    two = lambda t, w=width: None if t is None else _rows(t, w)
-    flat = lambda t: None if t is None else t.detach().contiguous()
-    xr, fr, gr, sc = two(x), two(f), two(gate, None if gate is None else gate.shape[-1]), flat(scale_cols)
-    held = [flat(t) for t in tensors[4:]]
-    d = _join_desc(xr, fr, gr, scale, sc, ((meta[1][0], held[0], held[1], meta[1][1]), (meta[2][0], held[2], held[3], meta[2][1]) if pre else (0, None, None, 0.0)), gate_act)
-    out = [t if x.dim() == 2 else t.reshape(x.shape) for t in _join_call(d, xr, f is not None, pre is not None, False)[:2] if t is not None]
-    return tuple(out) if len(out) > 1 else out[0]
+    y, h, _ = _Joint(*tensors, meta).run(False)
+    if x.dim() != 2:
+        y, h = (None if t is None else t.reshape(x.shape) for t in (y, h))
+    return h if y is None else y if h is None else (y, h)
 
 
 def norm_rows(x, norm):

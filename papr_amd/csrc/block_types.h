@@ -23,6 +23,12 @@ static inline bool papr_rows_aligned(const void* p, int64_t ld, int64_t width, i
     return ((uintptr_t)p & 15) == 0 && (ld * bytes) % 16 == 0 && (width * bytes) % 16 == 0;
 }
 
+// 1 / (1 + exp(-z)): the exponent's product with log2(e) in two parts (a relative error of a few ulp for every z), hardware exp2 and reciprocal.
+__device__ __forceinline__ float papr_sigmoid(float z) {
+    const float a = z * -1.44269504f, rest = fabsf(a) < 126.f ? __builtin_fmaf(z, -1.44269504f, -a) + z * -1.92596299e-8f : 0.f;
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a) * __builtin_fmaf(rest, 0.693147181f, 1.f));
+}
+
 // Parameters (norm gains and shifts, column scales) may be held in another type than the rows: N values from element `at` on, the type uniform.
 template <int N>
 __device__ __forceinline__ void load_param(float (&v)[N], const void* p, int type, int64_t at) {

@@ -48,14 +48,20 @@ struct Row {
     static constexpr int CH = E / V;
     // column of element i of lane j
     static __device__ __forceinline__ int col(int j, int i) { return (i / V * G + j) * V + i % V; }
-    static __device__ __forceinline__ void load(float (&v)[E], const T* row, int width, int j) {
+    struct Raw { papr_pack<T, V> t[CH]; };         // a row on its way: in the rows' type, a third of the registers
+    static __device__ __forceinline__ void fetch(Raw& r, const T* row, int width, int j) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int at = (c * G + j) * V;
-            papr_pack<T, V> t;
-            if (at < width) t = *reinterpret_cast<const papr_pack<T, V>*>(row + at);
+            if (at < width) r.t[c] = *reinterpret_cast<const papr_pack<T, V>*>(row + at);
+        }
+    }
+    static __device__ __forceinline__ void values(float (&v)[E], const Raw& r, int width, int j) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[c * V + i] = at < width ? (float)t.v[i] : 0.f;
+        for (int c = 0; c < CH; ++c) {
+            const bool in = (c * G + j) * V < width;
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[c * V + i] = in ? (float)r.t[c].v[i] : 0.f;
         }
     }
     static __device__ __forceinline__ void store(const float (&v)[E], T* row, int width, int j) {
@@ -83,15 +89,12 @@ struct Row {
     }
 };
 
-__device__ __forceinline__ float gate_value(float g, int act) {
-    if (act == PAPR_GATE_NONE) return g;
-    const float p = 1.f / (1.f + expf(-g));
-    return act == PAPR_GATE_SIGMOID ? p : g * p;
-}
-__device__ __forceinline__ float gate_slope(float g, int act) {
-    if (act == PAPR_GATE_NONE) return 1.f;
-    const float p = 1.f / (1.f + expf(-g));
-    return act == PAPR_GATE_SIGMOID ? p * (1.f - p) : p * (1.f + g * (1.f - p));
+// a(g) and a'(g)
+__device__ __forceinline__ void gate_of(float g, int act, float& value, float& slope) {
+    if (act == PAPR_GATE_NONE) { value = g; slope = 1.f; return; }
+    const float p = papr_sigmoid(g);
+    value = act == PAPR_GATE_SIGMOID ? p : g * p;
+    slope = act == PAPR_GATE_SIGMOID ? p * (1.f - p) : p * __builtin_fmaf(g, 1.f - p, 1.f);
 }
 
 // v <- standardised rows; stats = {mean, 1 / divisor, factor of the correlation term in the backward pass}
@@ -138,24 +141,44 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_fwd_kernel(papr_join_d
     R::param(qa, d.pre.gain, d.pre.type, width, j, 1.f);
     R::param(qb, d.pre.shift, d.pre.type, width, j, 0.f);
     R::param(sc, d.scale_cols, d.scale_type, width, j, d.scale);
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < d.rows; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t at = r0 + threadIdx.x / G, row = at < d.rows ? at : d.rows - 1;
+    // the next row's loads are on their way while this one is computed: a wave has 2 to 3 KB in flight all the time
+    typename R::Raw rx, rf, rg;
+    float g1 = 0.f;
+    const int64_t step = (int64_t)gridDim.x * RPB, first = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
+    auto fetch = [&](int64_t at) {
+        const int64_t row = at < d.rows ? at : d.rows - 1;
+        R::fetch(rx, reinterpret_cast<const T*>(d.x) + row * d.ldx, width, j);
+        if (d.f) R::fetch(rf, reinterpret_cast<const T*>(d.f) + row * d.ldf, width, j);
+        if (d.gate_form == PAPR_GATE_FULL) R::fetch(rg, reinterpret_cast<const T*>(d.gate) + row * d.ldg, width, j);
+        if (d.gate_form == PAPR_GATE_ROW) g1 = (float)reinterpret_cast<const T*>(d.gate)[row * d.ldg];
+    };
+    fetch(first);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB, at = first; r0 < d.rows; r0 += step, at += step) {
         const bool live = at < d.rows;
-        float y[E], f[E], g[E], st[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        R::load(y, reinterpret_cast<const T*>(d.x) + row * d.ldx, width, j);
+        const int64_t row = live ? at : d.rows - 1;
+        float y[E], f[E], ga[E], st[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, slope;
+        R::values(y, rx, width, j);
         if (d.f) {
-            R::load(f, reinterpret_cast<const T*>(d.f) + row * d.ldf, width, j);
-            if (d.gate_form == PAPR_GATE_FULL) R::load(g, reinterpret_cast<const T*>(d.gate) + row * d.ldg, width, j);
-            float g1 = 0.f;
-            if (d.gate_form == PAPR_GATE_ROW) g1 = gate_value((float)reinterpret_cast<const T*>(d.gate)[row * d.ldg], d.gate_act);
+            R::values(f, rf, width, j);
+            if (d.gate_form == PAPR_GATE_FULL) {
+                R::values(ga, rg, width, j);
+#pragma unroll
+                for (int i = 0; i < E; ++i) gate_of(ga[i], d.gate_act, ga[i], slope);
+            } else {
+                float g = 1.f;
+                if (d.gate_form == PAPR_GATE_ROW) gate_of(g1, d.gate_act, g, slope);
+#pragma unroll
+                for (int i = 0; i < E; ++i) ga[i] = g;
+            }
+        }
+        if (r0 + step < d.rows) fetch(at + step);
+        __builtin_amdgcn_sched_barrier(0);
+        if (d.f) {
             float s3[3] = {0.f, 0.f, 0.f};
             standardise<G, V>(f, d.post.kind, d.post.eps, width, j, s3, lds, turn);
             st[0] = s3[0]; st[1] = s3[1]; st[2] = s3[2];
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float ga = d.gate_form == PAPR_GATE_FULL ? gate_value(g[i], d.gate_act) : d.gate_form == PAPR_GATE_ROW ? g1 : 1.f;
-                y[i] += sc[i] * ga * __builtin_fmaf(f[i], pa[i], pb[i]);
-            }
+            for (int i = 0; i < E; ++i) y[i] += sc[i] * ga[i] * __builtin_fmaf(f[i], pa[i], pb[i]);
             if (live && y_out) R::store(y, y_out + row * width, width, j);
         }
         if (h_out) {
@@ -193,28 +216,50 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_bwd_kernel(papr_join_d
     for (int a = 0; a < 5; ++a)
 #pragma unroll
         for (int i = 0; i < E; ++i) acc[a][i] = 0.f;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < d.rows; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t at = r0 + threadIdx.x / G, row = at < d.rows ? at : d.rows - 1;
+    typename R::Raw rx, rf, rg, ry, rh;
+    float raw_gate = 0.f, rst[6];
+    const int64_t step = (int64_t)gridDim.x * RPB, first = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
+    auto fetch = [&](int64_t at) {
+        const int64_t row = at < d.rows ? at : d.rows - 1;
+        R::fetch(rx, reinterpret_cast<const T*>(d.x) + row * d.ldx, width, j);
+        if (d.f) R::fetch(rf, reinterpret_cast<const T*>(d.f) + row * d.ldf, width, j);
+        if (d.gate_form == PAPR_GATE_FULL) R::fetch(rg, reinterpret_cast<const T*>(d.gate) + row * d.ldg, width, j);
+        if (d.gate_form == PAPR_GATE_ROW) raw_gate = (float)reinterpret_cast<const T*>(d.gate)[row * d.ldg];
+        if (d_y) R::fetch(ry, d_y + row * width, width, j);
+        if (d_h) R::fetch(rh, d_h + row * width, width, j);
+#pragma unroll
+        for (int i = 0; i < 6; ++i) rst[i] = stats[row * 6 + i];
+    };
+    fetch(first);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB, at = first; r0 < d.rows; r0 += step, at += step) {
         const bool live = at < d.rows;
+        const int64_t row = live ? at : d.rows - 1;
         float x[E], f[E], g[E], dy[E], dh[E];
         const int seen = live ? width : 0;        // (a row past the end: zero gradients, nothing reaches the sums)
-        R::load(x, reinterpret_cast<const T*>(d.x) + row * d.ldx, width, j);
-        if (d.f) R::load(f, reinterpret_cast<const T*>(d.f) + row * d.ldf, width, j);
-        if (d.gate_form == PAPR_GATE_FULL) R::load(g, reinterpret_cast<const T*>(d.gate) + row * d.ldg, width, j);
-        if (d_y) R::load(dy, d_y + row * width, seen, j);
-        if (d_h) R::load(dh, d_h + row * width, seen, j);
-        float g1 = 0.f;
-        if (d.gate_form == PAPR_GATE_ROW) g1 = (float)reinterpret_cast<const T*>(d.gate)[row * d.ldg];
-        const float* st = stats + row * 6;
-        const float m1 = st[0], r1 = st[1], c1 = st[2], m2 = st[3], r2 = st[4], c2 = st[5];
-        float ga[E], p[E];
+        R::values(x, rx, width, j);
+        if (d.f) R::values(f, rf, width, j);
+        if (d.gate_form == PAPR_GATE_FULL) R::values(g, rg, width, j);
+        if (d_y) R::values(dy, ry, seen, j);
+        if (d_h) R::values(dh, rh, seen, j);
+        const float g1 = raw_gate, m1 = rst[0], r1 = rst[1], c1 = rst[2], m2 = rst[3], r2 = rst[4], c2 = rst[5];
+        if (r0 + step < d.rows) fetch(at + step);
+        __builtin_amdgcn_sched_barrier(0);
+        float ga[E], gs[E], p[E];
         if (d.f) {
+            if (d.gate_form == PAPR_GATE_FULL) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) gate_of(g[i], d.gate_act, ga[i], gs[i]);
+            } else {
+                float gv = 1.f, sv = 0.f;
+                if (d.gate_form == PAPR_GATE_ROW) gate_of(g1, d.gate_act, gv, sv);
+#pragma unroll
+                for (int i = 0; i < E; ++i) { ga[i] = gv; gs[i] = sv; }
+            }
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const bool in = (i / V * G + j) * V < width;
                 if (d.post.kind != PAPR_NORM_NONE) f[i] = in ? (f[i] - m1) * r1 : 0.f;
                 p[i] = __builtin_fmaf(f[i], pa[i], pb[i]);
-                ga[i] = d.gate_form == PAPR_GATE_FULL ? gate_value(g[i], d.gate_act) : d.gate_form == PAPR_GATE_ROW ? gate_value(g1, d.gate_act) : 1.f;
                 x[i] += sc[i] * ga[i] * p[i];
             }
         }
@@ -254,9 +299,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_bwd_kernel(papr_join_d
         for (int i = 0; i < E; ++i) {
             const bool in = (i / V * G + j) * V < width;
             const float dyi = in ? dy[i] : 0.f;
-            const float slope = d.gate_form == PAPR_GATE_FULL ? gate_slope(g[i], d.gate_act) : d.gate_form == PAPR_GATE_ROW ? gate_slope(g1, d.gate_act) : 0.f;
             acc[4][i] = __builtin_fmaf(dyi * ga[i], p[i], acc[4][i]);
-            g[i] = dyi * sc[i] * p[i] * slope;
+            g[i] = dyi * sc[i] * p[i] * gs[i];
             s[2] += g[i];
             dp[i] = dyi * sc[i] * ga[i];
             acc[2][i] = __builtin_fmaf(dp[i], f[i], acc[2][i]);
@@ -347,7 +391,8 @@ bool join_vec(const papr_join_desc& d) {
 
 int64_t join_blocks(const papr_join_desc& d, int G, bool bwd) {
     const int64_t rpb = G > 256 ? 1 : 256 / G, need = (d.rows + rpb - 1) / rpb;
-    const int64_t cap = (int64_t)papr_cu_count() * (G >= 512 ? 2 : bwd ? 4 : 8);
+    // (the waves that are resident at once: the backward kernel's registers allow eight a compute unit, the forward kernel's sixteen)
+    const int64_t cap = (int64_t)papr_cu_count() * (G >= 512 ? (bwd ? 1 : 2) : bwd ? 2 : 4);
     return need < cap ? need : cap;
 }
 

@@ -19,12 +19,6 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 namespace {
 
-// 1 / (1 + exp(-z)): the exponent's product with log2(e) in two parts (relative error of a few ulp for every z), hardware exp2 and reciprocal.
-__device__ __forceinline__ float sigmoid(float z) {
-    const float a = fminf(z * -1.44269504f, 126.f), rest = a < 126.f ? __builtin_fmaf(z, -1.44269504f, -a) + z * -1.92596299e-8f : 0.f;
-    const float e = __builtin_amdgcn_exp2f(a);
-    return __builtin_amdgcn_rcpf(1.f + __builtin_fmaf(e, rest * 0.693147181f, e));
-}
 // Phi(z) and phi(z) of the erf form of gelu.  float32 rows: the library's erf and exp.  16-bit rows: erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2), t = 1 / (1 + p x)
 // (Abramowitz and Stegun 7.1.26, 1.5e-7 absolute), a sixteenth of the rows' own rounding and a third of erf's instructions: erf in the epilogue of an
 // 8192 x 1024 -> 4096 layer took longer than its matrix instructions.
@@ -59,7 +53,7 @@ __device__ __forceinline__ void act_values(float (&v)[N], int act) {
         }
     } else if (act == PAPR_ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
+        for (int i = 0; i < N; ++i) v[i] *= papr_sigmoid(v[i]);
     }
 }
 // g <- g act'(z)
@@ -81,7 +75,7 @@ __device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], i
     } else if (act == PAPR_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float p = sigmoid(z[i]);
+            const float p = papr_sigmoid(z[i]);
             g[i] *= p * __builtin_fmaf(z[i], 1.f - p, 1.f);
         }
     }
@@ -109,7 +103,7 @@ __device__ __forceinline__ s16x4 read_tr4(unsigned a) { return __builtin_amdgcn_
 #pragma clang diagnostic pop
 
 // One operand's tile of R rows x BK in LDS, `PLANES` of them, and the registers its next tile waits in.
-//   K_RUNS:   image [R][BK] halfs, 16-byte pieces exchanged by the row number so that 8 rows' reads of one piece cover all banks.
+//   K_RUNS:   image [R][BK] halfs, 16-byte pieces exchanged by the row number so that 16 rows' reads of one piece cover all 64 banks.
 //   ROWS_RUN: image [BK][R + pad] halfs as it lies in memory; the transposing LDS read hands a lane 8 consecutive k of its row.  The row stride is
 //             64 bytes modulo 256: the four k a 16-lane group reads lie on different quarters of the banks.
 // FMT: 0 rows of type T, else 8-bit rows (ROWS_RUN only).  A thread's pieces sit at fixed 32-bit offsets from a uniform tile address that advances with k.
@@ -142,7 +136,7 @@ struct Tile {
     }
     // swizzled place of 16-byte piece c of row r (halfs)
     static __device__ __forceinline__ int place(int r, int c) {
-        const int sw = BK == 64 ? r & 7 : BK == 32 ? (r >> 1) & 3 : (r >> 2) & 1;
+        const int sw = BK == 64 ? (r >> 1) & 7 : BK == 32 ? (r >> 2) & 3 : (r >> 3) & 1;
         return r * STRIDE + ((c ^ sw) << 3);
     }
 
