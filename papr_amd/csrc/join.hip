@@ -14,14 +14,16 @@ namespace {
 
 constexpr int E = 8;                              // elements of a row per lane
 
+// (a DPP operand that the compiler may fold into the addition)
+#define LANES(v, ctrl) __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true))
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float (*lds)[N][16], int& turn) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        v[n] += PAPR_DPP_F(v[n], 0xB1);
-        v[n] += PAPR_DPP_F(v[n], 0x4E);
-        if (G >= 8) v[n] += PAPR_DPP_F(v[n], 0x141);
-        if (G >= 16) v[n] += PAPR_DPP_F(v[n], 0x140);
+        v[n] += LANES(v[n], 0xB1);
+        v[n] += LANES(v[n], 0x4E);
+        if (G >= 8) v[n] += LANES(v[n], 0x141);
+        if (G >= 16) v[n] += LANES(v[n], 0x140);
         if (G >= 32) v[n] += __shfl_xor(v[n], 16);
         if (G >= 64) v[n] += __shfl_xor(v[n], 32);
     }
@@ -56,7 +58,13 @@ struct Row {
             if (at < width) r.t[c] = *reinterpret_cast<const papr_pack<T, V>*>(row + at);
         }
     }
-    static __device__ __forceinline__ void values(float (&v)[E], const Raw& r, int width, int j) {
+    // whole: (uniform) every lane's chunks lie inside the row
+    static __device__ __forceinline__ void values(float (&v)[E], const Raw& r, int width, int j, bool whole) {
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = (float)r.t[i / V].v[i % V];
+            return;
+        }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const bool in = (c * G + j) * V < width;
@@ -117,11 +125,12 @@ __device__ __forceinline__ void standardise(float (&v)[E], int kind, float eps, 
     for (int i = 0; i < E; ++i) s[0] = __builtin_fmaf(v[i], v[i], s[0]);
     group_sum<G, 1>(s, lds, turn);
     if (kind == PAPR_NORM_LAYER) {
-        const float std = sqrtf(s[0] / (float)(width - 1)), div = std + eps;
-        stats[1] = 1.f / div;
-        stats[2] = std > 0.f ? div / ((float)(width - 1) * std) : 0.f;      // (a constant row: the deviation's slope is taken as zero, like torch's)
+        // (hardware square root and reciprocals, an ulp each: the precise forms were a fifth of the forward kernel's instructions at 256 columns)
+        const float rest = __builtin_amdgcn_rcpf((float)(width - 1)), std = __builtin_amdgcn_sqrtf(s[0] * rest), div = std + eps;
+        stats[1] = __builtin_amdgcn_rcpf(div);
+        stats[2] = std > 0.f ? div * rest * __builtin_amdgcn_rcpf(std) : 0.f;      // (a constant row: the deviation's slope is taken as zero, like torch's)
     } else {
-        stats[1] = 1.f / sqrtf(s[0] * rw + eps);
+        stats[1] = __builtin_amdgcn_rsqf(__builtin_fmaf(s[0], rw, eps));
         stats[2] = rw;
     }
 #pragma unroll
@@ -142,6 +151,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_fwd_kernel(papr_join_d
     R::param(qb, d.pre.shift, d.pre.type, width, j, 0.f);
     R::param(sc, d.scale_cols, d.scale_type, width, j, d.scale);
     // the next row's loads are on their way while this one is computed: a wave has 2 to 3 KB in flight all the time
+    const bool whole = width == G * E;
     typename R::Raw rx, rf, rg;
     float g1 = 0.f;
     const int64_t step = (int64_t)gridDim.x * RPB, first = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
@@ -157,11 +167,11 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_fwd_kernel(papr_join_d
         const bool live = at < d.rows;
         const int64_t row = live ? at : d.rows - 1;
         float y[E], f[E], ga[E], st[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, slope;
-        R::values(y, rx, width, j);
+        R::values(y, rx, width, j, whole);
         if (d.f) {
-            R::values(f, rf, width, j);
+            R::values(f, rf, width, j, whole);
             if (d.gate_form == PAPR_GATE_FULL) {
-                R::values(ga, rg, width, j);
+                R::values(ga, rg, width, j, whole);
 #pragma unroll
                 for (int i = 0; i < E; ++i) gate_of(ga[i], d.gate_act, ga[i], slope);
             } else {
@@ -197,54 +207,78 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_fwd_kernel(papr_join_d
 }
 
 template <typename T, int V, int G>
-__global__ __launch_bounds__(G > 256 ? G : 256) void join_bwd_kernel(papr_join_desc d, const float* __restrict__ stats, const T* __restrict__ d_y, const T* __restrict__ d_h,
+__global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void join_bwd_kernel(papr_join_desc d, const float* __restrict__ stats, const T* __restrict__ d_y, const T* __restrict__ d_h,
                                                                      T* __restrict__ d_x, T* __restrict__ d_f, T* __restrict__ d_g, float* __restrict__ part) {
     typedef Row<T, V, G> R;
     constexpr int THREADS = G > 256 ? G : 256, RPB = THREADS / G;
-    __shared__ float lds[2][3][16];
+    __shared__ float lds[2][3][16], lds2[2][2][16];
     __shared__ float fold[RPB > 1 ? RPB * G * E : 1];
     int turn = 0;
     const int j = threadIdx.x % G, width = d.width;
     const float rw = 1.f / (float)width;
+    // What a compute unit has on its way is what bounds this kernel (eight waves with a row's operands each, 3.2 TB/s): two rows ahead of the arithmetic, with the
+    // parameters read again from LDS row by row instead of sitting in 32 registers.  float32 rows (twice the bytes) and odd ones: one row ahead; the widest rows: none.
+    constexpr int AHEAD = G > 512 ? 0 : G == 512 || V < 8 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) float par[G <= 256 ? 4 : 1][G <= 256 ? G * E : 1];
     float pa[E], pb[E], qa[E], sc[E];
     R::param(pa, d.post.gain, d.post.type, width, j, 1.f);
     R::param(pb, d.post.shift, d.post.type, width, j, 0.f);
     R::param(qa, d.pre.gain, d.pre.type, width, j, 1.f);
     R::param(sc, d.scale_cols, d.scale_type, width, j, d.scale);
+    auto param = [&](int q, float (&v)[E], bool put) __attribute__((always_inline)) {
+        if constexpr (G <= 256) {
+#pragma unroll
+            for (int i = 0; i < E; i += 4) {
+                float4* at = (float4*)&par[q][(i / 4 * G + j) * 4];
+                if (put) *at = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                else { const float4 t = *at; v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w; }
+            }
+        }
+    };
+    if (threadIdx.x < G) { param(0, pa, true); param(1, pb, true); param(2, qa, true); param(3, sc, true); }
+    __syncthreads();
     float acc[5][E];                              // column sums: d(pre gain), d(pre shift), d(post gain), d(post shift), d(scale)
 #pragma unroll
     for (int a = 0; a < 5; ++a)
 #pragma unroll
         for (int i = 0; i < E; ++i) acc[a][i] = 0.f;
-    typename R::Raw rx, rf, rg, ry, rh;
-    float raw_gate = 0.f, rst[6];
+    struct Operands { typename R::Raw x, f, g, y, h; T gate; float st[6]; } w0, w1;
     const int64_t step = (int64_t)gridDim.x * RPB, first = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
-    auto fetch = [&](int64_t at) {
+    auto fetch = [&](Operands& w, int64_t at) __attribute__((always_inline)) {
         const int64_t row = at < d.rows ? at : d.rows - 1;
-        R::fetch(rx, reinterpret_cast<const T*>(d.x) + row * d.ldx, width, j);
-        if (d.f) R::fetch(rf, reinterpret_cast<const T*>(d.f) + row * d.ldf, width, j);
-        if (d.gate_form == PAPR_GATE_FULL) R::fetch(rg, reinterpret_cast<const T*>(d.gate) + row * d.ldg, width, j);
-        if (d.gate_form == PAPR_GATE_ROW) raw_gate = (float)reinterpret_cast<const T*>(d.gate)[row * d.ldg];
-        if (d_y) R::fetch(ry, d_y + row * width, width, j);
-        if (d_h) R::fetch(rh, d_h + row * width, width, j);
+        R::fetch(w.x, reinterpret_cast<const T*>(d.x) + row * d.ldx, width, j);
+        if (d.f) R::fetch(w.f, reinterpret_cast<const T*>(d.f) + row * d.ldf, width, j);
+        if (d.gate_form == PAPR_GATE_FULL) R::fetch(w.g, reinterpret_cast<const T*>(d.gate) + row * d.ldg, width, j);
+        if (d.gate_form == PAPR_GATE_ROW) w.gate = reinterpret_cast<const T*>(d.gate)[row * d.ldg];
+        if (d_y) R::fetch(w.y, d_y + row * width, width, j);
+        if (d_h) R::fetch(w.h, d_h + row * width, width, j);
 #pragma unroll
-        for (int i = 0; i < 6; ++i) rst[i] = stats[row * 6 + i];
+        for (int i = 0; i < 6; ++i) w.st[i] = stats[row * 6 + i];
     };
-    fetch(first);
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB, at = first; r0 < d.rows; r0 += step, at += step) {
+    const bool whole = width == G * E;
+    auto one_row = [&](Operands& w, int64_t r0, int64_t at) __attribute__((always_inline)) {
         const bool live = at < d.rows;
         const int64_t row = live ? at : d.rows - 1;
+        if (AHEAD == 0) fetch(w, at);
         float x[E], f[E], g[E], dy[E], dh[E];
+        const bool all_live = r0 + RPB <= d.rows;      // (uniform)
         const int seen = live ? width : 0;        // (a row past the end: zero gradients, nothing reaches the sums)
-        R::values(x, rx, width, j);
-        if (d.f) R::values(f, rf, width, j);
-        if (d.gate_form == PAPR_GATE_FULL) R::values(g, rg, width, j);
-        if (d_y) R::values(dy, ry, seen, j);
-        if (d_h) R::values(dh, rh, seen, j);
-        const float g1 = raw_gate, m1 = rst[0], r1 = rst[1], c1 = rst[2], m2 = rst[3], r2 = rst[4], c2 = rst[5];
-        if (r0 + step < d.rows) fetch(at + step);
+        R::values(x, w.x, width, j, whole);
+        if (d.f) R::values(f, w.f, width, j, whole);
+        if (d.gate_form == PAPR_GATE_FULL) R::values(g, w.g, width, j, whole);
+        if (d_y) R::values(dy, w.y, seen, j, whole && all_live);
+        if (d_h) R::values(dh, w.h, seen, j, whole && all_live);
+        const float g1 = d.gate_form == PAPR_GATE_ROW ? (float)w.gate : 0.f, m1 = w.st[0], r1 = w.st[1], c1 = w.st[2], m2 = w.st[3], r2 = w.st[4], c2 = w.st[5];
+        if (AHEAD > 0) fetch(w, at + AHEAD * step);
         __builtin_amdgcn_sched_barrier(0);
-        float ga[E], gs[E], p[E];
+        asm volatile("" ::: "memory");            // (the parameters are read where they are used, row by row)
+        param(0, pa, false);
+        param(1, pb, false);
+        param(3, sc, false);
+        // (columns past the end need no care here: their gains, scale and incoming gradients are zero, so nothing of them reaches a row's sums, and their own results are
+        // never stored)
+        const bool post = d.post.kind != PAPR_NORM_NONE;
+        float ga[E], gn[E], gs[E], p[E];
         if (d.f) {
             if (d.gate_form == PAPR_GATE_FULL) {
 #pragma unroll
@@ -255,18 +289,23 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_bwd_kernel(papr_join_d
 #pragma unroll
                 for (int i = 0; i < E; ++i) { ga[i] = gv; gs[i] = sv; }
             }
+            if (post)
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[i] = (f[i] - m1) * r1;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const bool in = (i / V * G + j) * V < width;
-                if (d.post.kind != PAPR_NORM_NONE) f[i] = in ? (f[i] - m1) * r1 : 0.f;
                 p[i] = __builtin_fmaf(f[i], pa[i], pb[i]);
-                x[i] += sc[i] * ga[i] * p[i];
+                gn[i] = ga[i];
+                ga[i] *= sc[i];
+                x[i] = __builtin_fmaf(ga[i], p[i], x[i]);
             }
         }
         if (!d_y)
 #pragma unroll
             for (int i = 0; i < E; ++i) dy[i] = 0.f;
         if (d_h) {
+            asm volatile("" ::: "memory");
+            param(2, qa, false);
             if (d.pre.kind == PAPR_NORM_NONE) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
@@ -275,51 +314,59 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_bwd_kernel(papr_join_d
                     dy[i] = __builtin_fmaf(dh[i], qa[i], dy[i]);
                 }
             } else {
-                float s[3] = {0.f, 0.f, 0.f};
+                float s[2] = {0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const bool in = (i / V * G + j) * V < width;
-                    x[i] = in ? (x[i] - m2) * r2 : 0.f;
+                    x[i] = (x[i] - m2) * r2;
                     acc[0][i] = __builtin_fmaf(dh[i], x[i], acc[0][i]);
                     acc[1][i] += dh[i];
                     dh[i] *= qa[i];
                     s[0] = __builtin_fmaf(dh[i], x[i], s[0]);
                     s[1] += dh[i];
                 }
-                group_sum<G, 3>(s, lds, turn);
-                const float t = s[0] * c2, m = d.pre.kind == PAPR_NORM_LAYER ? s[1] * rw : 0.f;
+                group_sum<G, 2>(s, lds2, turn);
+                const float t = s[0] * c2 * r2, m = d.pre.kind == PAPR_NORM_LAYER ? s[1] * rw * r2 : 0.f;
 #pragma unroll
-                for (int i = 0; i < E; ++i) dy[i] += (dh[i] - x[i] * t - m) * r2;
+                for (int i = 0; i < E; ++i) dy[i] += __builtin_fmaf(dh[i], r2, -__builtin_fmaf(x[i], t, m));
             }
         }
         if (live && d_x) R::store(dy, d_x + row * width, width, j);
-        if (!d.f) continue;
+        if (!d.f) return;
         float s[3] = {0.f, 0.f, 0.f}, dp[E];
+        asm volatile("" ::: "memory");
+        param(0, pa, false);
+        param(3, sc, false);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const bool in = (i / V * G + j) * V < width;
-            const float dyi = in ? dy[i] : 0.f;
-            acc[4][i] = __builtin_fmaf(dyi * ga[i], p[i], acc[4][i]);
-            g[i] = dyi * sc[i] * p[i] * gs[i];
+            const float w = dy[i] * p[i];
+            dp[i] = dy[i] * ga[i];
+            acc[4][i] = __builtin_fmaf(gn[i], w, acc[4][i]);
+            g[i] = sc[i] * w * gs[i];
             s[2] += g[i];
-            dp[i] = dyi * sc[i] * ga[i];
             acc[2][i] = __builtin_fmaf(dp[i], f[i], acc[2][i]);
             acc[3][i] += dp[i];
             dp[i] *= pa[i];
             s[0] = __builtin_fmaf(dp[i], f[i], s[0]);
             s[1] += dp[i];
         }
-        group_sum<G, 3>(s, lds, turn);
+        if (post || d.gate_form == PAPR_GATE_ROW) group_sum<G, 3>(s, lds, turn);
         if (d_g) {
             if (d.gate_form == PAPR_GATE_FULL) { if (live) R::store(g, d_g + row * width, width, j); }
             else if (live && j == 0) d_g[row] = (T)s[2];
         }
-        if (d.post.kind != PAPR_NORM_NONE) {
-            const float t = s[0] * c1, m = d.post.kind == PAPR_NORM_LAYER ? s[1] * rw : 0.f;
+        if (post) {
+            const float t = s[0] * c1 * r1, m = d.post.kind == PAPR_NORM_LAYER ? s[1] * rw * r1 : 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) dp[i] = (dp[i] - f[i] * t - m) * r1;
+            for (int i = 0; i < E; ++i) dp[i] = __builtin_fmaf(dp[i], r1, -__builtin_fmaf(f[i], t, m));
         }
         if (live && d_f) R::store(dp, d_f + row * width, width, j);
+    };
+    if (AHEAD > 0) fetch(w0, first);
+    if (AHEAD > 1) fetch(w1, first + step);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB, at = first; r0 < d.rows; r0 += AHEAD * step, at += AHEAD * step) {
+        one_row(w0, r0, at);
+        if (AHEAD > 1 && r0 + step < d.rows) one_row(w1, r0 + step, at + step);
+        if (AHEAD == 0) { r0 += step; at += step; }
     }
     if (!part) return;
     // the workgroup's row groups meet in LDS, in group order; one partial row per workgroup and array
