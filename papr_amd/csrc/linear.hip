@@ -262,10 +262,12 @@ __device__ __forceinline__ Place place_of(unsigned id, unsigned total, unsigned 
     return p;
 }
 
-// Tile shapes: waves WM x WN, each IM x IN blocks of 32 x 32.
-template <int WM_, int WN_, int IM_, int IN_>
+// Tile shapes: waves WM x WN, each IM x IN blocks of 32 x 32; DEPTH stages of a streaming kernel.
+template <int WM_, int WN_, int IM_, int IN_, int DEPTH_>
 struct Shape {
-    static constexpr int WM = WM_, WN = WN_, IM = IM_, IN = IN_, THREADS = 64 * WM * WN, TM = WM * IM * 32, TN = WN * IN * 32;
+    static constexpr int DEPTH = DEPTH_, WM = WM_, WN = WN_, IM = IM_, IN = IN_, THREADS = 64 * WM * WN, TM = WM * IM * 32, TN = WN * IN * 32;
+    static constexpr int EPI_STRIDE = IN * 32 + 8;                                // floats: rows four apart lie on the other half of the banks
+    static constexpr size_t EPI = (size_t)WM * WN * 32 * EPI_STRIDE * 4;
 };
 
 template <typename T, int LA, int LB, int FMT, bool VEC, typename S>
@@ -274,9 +276,7 @@ struct Plan {
     typedef Tile<T, LA, 0, VEC, S::TM, BK, S::THREADS> TA;
     typedef Tile<T, LB, FMT, VEC, S::TN, BK, S::THREADS> TB;
     static constexpr int BUF = TA::HALFS + TB::HALFS;
-    static constexpr int EPI_STRIDE = S::IN * 32 + 8;                             // floats: rows four apart lie on the other half of the banks
-    static constexpr size_t EPI = (size_t)S::WM * S::WN * 32 * EPI_STRIDE * 4, LOOP = (size_t)2 * BUF * 2;
-    static constexpr size_t LDS = EPI > LOOP ? EPI : LOOP;
+    static constexpr size_t LOOP = (size_t)2 * BUF * 2, LDS = S::EPI > LOOP ? S::EPI : LOOP;
 };
 
 // E consecutive results of row m from column n on
@@ -300,6 +300,86 @@ __device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int6
 #pragma unroll
     for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
     *reinterpret_cast<papr_pack<T, E>*>(reinterpret_cast<T*>(ep.out) + m * N + n) = t;
+}
+
+// The results of a workgroup's tile, from the accumulators of its waves.  smem: Shape::EPI bytes, free of earlier readers.
+template <typename T, int OUT, typename S>
+__device__ __forceinline__ void write_tile(const f32x16 (&acc)[S::IM][S::IN], short* smem, int64_t m0, int64_t n0, int64_t M, int64_t N, int part, const Epilogue& ep) {
+    constexpr int IM = S::IM, IN = S::IN, EPI_STRIDE = S::EPI_STRIDE;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+    if (OUT == OUT_SLAB) {
+        // float32, as it lies: a lane holds column lane & 31 of a 32 x 32 block, rows (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
+        float* out = reinterpret_cast<float*>(ep.out) + (int64_t)part * M * N;
+#pragma unroll
+        for (int j = 0; j < IN; ++j) {
+            const int64_t n = n0 + (wn * IN + j) * 32 + (lane & 31);
+#pragma unroll
+            for (int i = 0; i < IM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int64_t m = m0 + (wm * IM + i) * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+                    if (n < N && m < M) out[m * N + n] = acc[i][j][e];
+                }
+        }
+        return;
+    }
+    // Through LDS, 32 rows of the wave's own at a time (no barrier), so that a lane takes 16 bytes of a row: 16-byte loads and stores of whole lines.  Rows that do not
+    // start on 16 bytes: a lane takes single columns, 64 (32) lanes a row.
+    float* epi = reinterpret_cast<float*>(smem) + wave * 32 * EPI_STRIDE;
+    constexpr int COLS = IN * 32, E = 16 / sizeof(T), LPR = COLS / E, RPP = 64 / LPR;
+    const int64_t nw = n0 + wn * COLS;
+    const bool wide = ep.wide;
+    const int64_t n = nw + (wide ? lane % LPR * E : lane % COLS);
+    float bias[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) bias[i] = 0.f;
+    if (OUT == OUT_FORWARD && ep.bias && n < N) {
+        const T* src = reinterpret_cast<const T*>(ep.bias) + n;
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) bias[i] = (float)src[i];
+        } else bias[0] = (float)src[0];
+    }
+#pragma unroll
+    for (int i = 0; i < IM; ++i) {
+        const int64_t mw = m0 + (wm * IM + i) * 32;
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) epi[((e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * EPI_STRIDE + j * 32 + (lane & 31)] = acc[i][j][e];
+        if (wide) {
+            papr_pack<T, E> res[32 / RPP];
+#pragma unroll
+            for (int r = 0; r < 32 / RPP; ++r) {
+                const int64_t m = mw + r * RPP + lane / LPR;
+                if (OUT == OUT_FORWARD && ep.res && m < M && n < N) res[r] = *reinterpret_cast<const papr_pack<T, E>*>(reinterpret_cast<const T*>(ep.res) + m * ep.ld_res + n);
+            }
+#pragma unroll
+            for (int r = 0; r < 32 / RPP; ++r) {
+                const int64_t m = mw + r * RPP + lane / LPR;
+                float v[E];
+#pragma unroll
+                for (int c = 0; c < E; c += 4) {
+                    const float4 t = *reinterpret_cast<const float4*>(epi + (r * RPP + lane / LPR) * EPI_STRIDE + lane % LPR * E + c);
+                    v[c] = t.x; v[c + 1] = t.y; v[c + 2] = t.z; v[c + 3] = t.w;
+                }
+                if (m < M && n < N) finish<T, OUT, E>(v, m, n, N, bias, res[r], ep);
+            }
+        } else {
+            constexpr int ROWS = 64 / COLS;
+#pragma unroll 4
+            for (int r = 0; r < 32; r += ROWS) {
+                const int64_t m = mw + r + lane / COLS;
+                float v[1] = {epi[(r + lane / COLS) * EPI_STRIDE + lane % COLS]};
+                const float b1[1] = {bias[0]};
+                if (m < M && n < N) {
+                    papr_pack<T, 1> res;
+                    if (OUT == OUT_FORWARD && ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
+                    finish<T, OUT, 1>(v, m, n, N, b1, res, ep);
+                }
+            }
+        }
+    }
 }
 
 template <typename T, int LA, int LB, int FMT, bool VEC, int OUT, typename S>
@@ -365,80 +445,269 @@ __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Opera
         }
         __syncthreads();
     }
-    const int64_t M = A.rows, N = B.rows;
-    if (OUT == OUT_SLAB) {
-        // float32, as it lies: a lane holds column lane & 31 of a 32 x 32 block, rows (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
-        float* out = reinterpret_cast<float*>(ep.out) + (int64_t)at.part * M * N;
+    write_tile<T, OUT, S>(acc, smem, m0, n0, A.rows, B.rows, at.part, ep);
+}
+
+// The same product for 16-bit rows that start on 16 bytes: operands go straight from memory into LDS (global_load_lds, 16 bytes a lane), DEPTH stages of 32 terms, three
+// of them on their way while one is multiplied -- with one stage on its way in registers (product_kernel) half of a wave's time was waiting for it (256 x 256 tiles:
+// the matrix pipe 34 % busy).  An instruction fills 1 KB in lane order, so the images are made by which address a lane asks for:
+//   K_RUNS:   16 rows of 32 halfs, pieces exchanged by the row number as in Tile;
+//   ROWS_RUN: one "line" = the k rows q, q + LINES, q + 2 LINES, ... of R halfs one behind the other (1 KB), lines 1,088 bytes apart: the four consecutive k that a
+//             16-lane group of a transposing read wants lie on different quarters of the banks.
+// Rows past the operand's end: some row of it (never stored); terms past the part's end: a block of zeros.
+// The fragments of a 16-term step are read under the matrix instructions of the step before, and the stage's one barrier stands between its two steps: in front of
+// it a wave has read all of its stage (whose buffer the requests behind the barrier overwrite), behind it the next stage, requested three stages earlier, is there.
+__device__ const uint4 zero_block[4] = {};
+
+__device__ __forceinline__ void request16(const void* src, unsigned lds) {         // 64 lanes x 16 bytes -> LDS [lds, +1 KB) in lane order
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(src), "s"(lds) : "memory");
+}
+
+template <typename T, int LAYOUT, int R, int WAVES>
+struct Stage {
+    static constexpr int BK = 32, LINE = LAYOUT == K_RUNS ? 1024 : 1088, LINES = R * BK * 2 / 1024, BYTES = LINES * LINE, N = LINES / WAVES;
+    static_assert(LINES % WAVES == 0 && R * 2 <= 1024, "whole requests per wave");
+    typedef typename Matrix<T>::frag frag;
+    const char* src[N];                                                            // this lane's address of the next stage's requests
+    int k[N];                                                                      // its term inside the stage
+    int64_t step;
+
+    __device__ __forceinline__ void start(const Operand& o, int64_t r0, int64_t k0, int wave) {
+        const int lane = threadIdx.x & 63;
+        const int64_t left = o.rows - r0;
 #pragma unroll
-        for (int j = 0; j < IN; ++j) {
-            const int64_t n = n0 + (wn * IN + j) * 32 + (lane & 31);
-#pragma unroll
-            for (int i = 0; i < IM; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int64_t m = m0 + (wm * IM + i) * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
-                    if (n < N && m < M) out[m * N + n] = acc[i][j][e];
-                }
+        for (int q = 0; q < N; ++q) {
+            const int line = wave * N + q;
+            int r;
+            if (LAYOUT == K_RUNS) {
+                r = line * 16 + lane / 4;
+                k[q] = 8 * ((lane & 3) ^ ((r >> 2) & 3));
+                if (r >= left) r = (int)left - 1;
+                src[q] = reinterpret_cast<const char*>(o.p) + ((r0 + r) * o.ld + k0 + k[q]) * 2;
+            } else {
+                r = 8 * (lane % (R / 8));
+                k[q] = line + lane / (R / 8) * LINES;
+                if (r >= left) r = 0;
+                src[q] = reinterpret_cast<const char*>(o.p) + ((k0 + k[q]) * o.ld + r0 + r) * 2;
+            }
         }
-        return;
+        step = (LAYOUT == K_RUNS ? (int64_t)BK : BK * o.ld) * 2;
     }
-    // Through LDS, 32 rows of the wave's own at a time (no barrier), so that a lane takes 16 bytes of a row: 16-byte loads and stores of whole lines.  Rows that do not
-    // start on 16 bytes: a lane takes single columns, 64 (32) lanes a row.
-    float* epi = reinterpret_cast<float*>(smem) + wave * 32 * P::EPI_STRIDE;
-    constexpr int COLS = IN * 32, E = 16 / sizeof(T), LPR = COLS / E, RPP = 64 / LPR;
-    const int64_t nw = n0 + wn * COLS;
-    const bool wide = ep.wide;
-    const int64_t n = nw + (wide ? lane % LPR * E : lane % COLS);
-    float bias[E];
+    // requests of the next stage; `left`: terms from its first on
+    __device__ __forceinline__ void request(unsigned lds, int64_t left, int wave) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) bias[i] = 0.f;
-    if (OUT == OUT_FORWARD && ep.bias && n < N) {
-        const T* src = reinterpret_cast<const T*>(ep.bias) + n;
-        if (wide) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) bias[i] = (float)src[i];
-        } else bias[0] = (float)src[0];
+        for (int q = 0; q < N; ++q) {
+            const void* p = k[q] < left ? (const void*)src[q] : (const void*)zero_block;
+            request16(p, lds + (unsigned)(wave * N + q) * LINE);
+            src[q] += step;
+        }
     }
+    // this lane's corner of the fragments (bytes): rows `row` .. + 31, step 0
+    static __device__ __forceinline__ unsigned corner(int row) {
+        const int lane = threadIdx.x & 63;
+        if (LAYOUT == K_RUNS) { const int r = row + (lane & 31); return (unsigned)(r * 64 + (((lane >> 5) ^ ((r >> 2) & 3)) << 4)); }
+        const int c = 8 * (lane >> 5) + ((lane & 15) >> 2);
+        return (unsigned)(c % LINES * LINE + c / LINES * R * 2 + (row + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2);
+    }
+    // LINES is 16 (R = 256) or 8 (R = 128): the second step's k + 16 is one half of a line on, or two quarters; four k on is four lines (LINES > 4, c < 12)
+    static __device__ __forceinline__ frag read(unsigned stage, unsigned corner, int ks) {
+        s16x8 v;
+        if (LAYOUT == K_RUNS) {
+            // (piece c of step 1 is piece c + 2: the exchange turns + 2 into ^ 2)
+            v = *reinterpret_cast<const __attribute__((address_space(3))) s16x8*>(stage + (corner ^ (unsigned)(ks * 32)));
+        } else {
+            const unsigned a = stage + corner + (unsigned)(ks * 16 / LINES * R * 2);
+            const s16x4 lo = read_tr4(a), hi = read_tr4(a + 4 * LINE);
+            v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return __builtin_bit_cast(frag, v);
+    }
+};
+
+template <typename T, int LA, int LB, typename S>
+struct Stream {
+    static constexpr int DEPTH = S::DEPTH;
+    typedef Stage<T, LA, S::TM, S::WM * S::WN> SA;
+    typedef Stage<T, LB, S::TN, S::WM * S::WN> SB;
+    static constexpr unsigned BYTES = SA::BYTES + SB::BYTES;
+    static constexpr size_t LOOP = (size_t)DEPTH * BYTES, LDS = S::EPI > LOOP ? S::EPI : LOOP;
+};
+
+template <typename T, int LA, int LB, int OUT, typename S>
+__global__ __launch_bounds__(S::THREADS, 2) void stream_kernel(Operand A, Operand B, int64_t K, int64_t k_per_part, unsigned tiles_m, unsigned tiles_n, Epilogue ep) {
+    typedef Stream<T, LA, LB, S> P;
+    typedef typename P::SA SA;
+    typedef typename P::SB SB;
+    constexpr int IM = S::IM, IN = S::IN, WAITING = (P::DEPTH - 2) * (SA::N + SB::N);          // requests of the stages behind the next one
+    extern __shared__ __attribute__((aligned(16))) short smem[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+    const Place at = place_of(blockIdx.x, gridDim.x, tiles_m, tiles_n);
+    const int64_t m0 = (int64_t)at.m * S::TM, n0 = (int64_t)at.n * S::TN;
+    const int64_t kb = at.part * k_per_part, ke = kb + k_per_part < K ? kb + k_per_part : K;
+    const int stages = (int)((ke - kb + 31) / 32);
+    const unsigned lds = (unsigned)(size_t)smem;
+    f32x16 acc[IM][IN];
 #pragma unroll
-    for (int i = 0; i < IM; ++i) {
-        const int64_t mw = m0 + (wm * IM + i) * 32;
+    for (int i = 0; i < IM; ++i)
 #pragma unroll
         for (int j = 0; j < IN; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) epi[((e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * P::EPI_STRIDE + j * 32 + (lane & 31)] = acc[i][j][e];
-        if (wide) {
-            papr_pack<T, E> res[32 / RPP];
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    SA a;
+    SB b;
+    a.start(A, m0, kb, wave);
+    b.start(B, n0, kb, wave);
+    int64_t left = ke - kb;
+    auto request = [&](int st) {
+        const unsigned to = lds + (unsigned)(st % P::DEPTH) * P::BYTES;
+        a.request(to, left, wave);
+        b.request(to + SA::BYTES, left, wave);
+        left -= 32;
+    };
+    unsigned ca[IM], cb[IN];
 #pragma unroll
-            for (int r = 0; r < 32 / RPP; ++r) {
-                const int64_t m = mw + r * RPP + lane / LPR;
-                if (OUT == OUT_FORWARD && ep.res && m < M && n < N) res[r] = *reinterpret_cast<const papr_pack<T, E>*>(reinterpret_cast<const T*>(ep.res) + m * ep.ld_res + n);
-            }
+    for (int i = 0; i < IM; ++i) ca[i] = SA::corner((wm * IM + i) * 32);
 #pragma unroll
-            for (int r = 0; r < 32 / RPP; ++r) {
-                const int64_t m = mw + r * RPP + lane / LPR;
-                float v[E];
+    for (int j = 0; j < IN; ++j) cb[j] = SA::BYTES + SB::corner((wn * IN + j) * 32);
+    struct Frags { typename SA::frag a[IM]; typename SB::frag b[IN]; } f0, f1;
+    auto read = [&](Frags& f, int st, int ks) {
+        const unsigned from = lds + (unsigned)(st % P::DEPTH) * P::BYTES;
 #pragma unroll
-                for (int c = 0; c < E; c += 4) {
-                    const float4 t = *reinterpret_cast<const float4*>(epi + (r * RPP + lane / LPR) * P::EPI_STRIDE + lane % LPR * E + c);
-                    v[c] = t.x; v[c + 1] = t.y; v[c + 2] = t.z; v[c + 3] = t.w;
-                }
-                if (m < M && n < N) finish<T, OUT, E>(v, m, n, N, bias, res[r], ep);
-            }
+        for (int j = 0; j < IN; ++j) f.b[j] = SB::read(from, cb[j], ks);
+#pragma unroll
+        for (int i = 0; i < IM; ++i) f.a[i] = SA::read(from, ca[i], ks);
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+        for (int i = 0; i < IM; ++i)
+#pragma unroll
+            for (int j = 0; j < IN; ++j) acc[i][j] = mfma(f.a[i], f.b[j], acc[i][j]);
+    };
+#pragma unroll
+    for (int st = 0; st < P::DEPTH - 1; ++st) request(st);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WAITING) : "memory");     // stage 0 is there (every wave's part of it)
+    request(P::DEPTH - 1);
+    read(f0, 0, 0);
+    for (int st = 0; st < stages; ++st) {
+        read(f1, st, 1);
+        multiply(f0);
+        // stage st is read (its reads are waited for), stage st + 1 is there: the two stages behind it may be on their way
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WAITING) : "memory");
+        request(st + P::DEPTH);
+        read(f0, st + 1, 0);                       // (behind the last stage: a stage of zeros, not multiplied)
+        multiply(f1);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    write_tile<T, OUT, S>(acc, smem, m0, n0, A.rows, B.rows, at.part, ep);
+}
+
+// Few rows (one token, a handful): the weight is read once and that is the time.  A workgroup takes 16 columns of the result, its waves a part of the sum each,
+// straight from memory into the operands of 16 x 16 x 32 matrix instructions (rows of x come from the caches); the parts meet in LDS, in wave order.
+template <typename T, int MT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand B, int64_t K, bool aligned, Epilogue ep) {
+    constexpr int PARTS = sizeof(T) == 4 ? 3 : 1, AHEAD = 8 / MT / (sizeof(T) / 2);
+    typedef typename Matrix<T>::frag frag;
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    __shared__ float lds[WAVES][MT * 16][17];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, k8 = lane >> 4 << 3;
+    const int64_t M = A.rows, N = B.rows, n0 = (int64_t)blockIdx.x * 16;
+    const int steps = (int)((K + 31) / 32), per = (steps + WAVES - 1) / WAVES, beg = wave * per, end = beg + per < steps ? beg + per : steps;
+    struct Eight { papr_pack<T, 8> t; };
+    auto fetch = [&](Eight& v, const Operand& o, int64_t row, int step) __attribute__((always_inline)) {
+        row = row < o.rows ? row : o.rows - 1;
+        const int64_t k = (int64_t)step * 32 + k8;
+        const T* src = reinterpret_cast<const T*>(o.p) + row * o.ld + k;
+        if ((int64_t)step * 32 + 32 <= K) {
+            if (aligned) {
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(&v.t)[i] = reinterpret_cast<const uint4*>(src)[i];
+            } else __builtin_memcpy(&v.t, src, sizeof(v.t));
         } else {
-            constexpr int ROWS = 64 / COLS;
-#pragma unroll 4
-            for (int r = 0; r < 32; r += ROWS) {
-                const int64_t m = mw + r + lane / COLS;
-                float v[1] = {epi[(r + lane / COLS) * P::EPI_STRIDE + lane % COLS]};
-                const float b1[1] = {bias[0]};
-                if (m < M && n < N) {
-                    papr_pack<T, 1> res;
-                    if (OUT == OUT_FORWARD && ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
-                    finish<T, OUT, 1>(v, m, n, N, b1, res, ep);
-                }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v.t.v[i] = k + i < K ? src[i] : (T)0.f;
+        }
+    };
+    auto parts = [&](frag (&f)[PARTS], const Eight& v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (PARTS == 1) f[0][i] = v.t.v[i];
+            else {
+                f[0][i] = (bf16)v.t.v[i];
+                const float rest = v.t.v[i] - (float)f[0][i];
+                f[1][i] = (bf16)rest;
+                f[2][i] = (bf16)(rest - (float)f[1][i]);
+            }
+        }
+    };
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = beg; s0 < end; s0 += AHEAD) {
+        Eight wv[AHEAD], xv[AHEAD][MT];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (s0 + a >= end) break;
+            fetch(wv[a], B, n0 + r, s0 + a);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) fetch(xv[a][t], A, t * 16 + r, s0 + a);
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (s0 + a >= end) break;
+            frag wf[PARTS];
+            parts(wf, wv[a]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                frag xf[PARTS];
+                parts(xf, xv[a][t]);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q)
+                        if (p + q < 3) {
+                            if constexpr (__is_same(T, f16)) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[p], wf[q], acc[t], 0, 0, 0);
+                            else acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[p], wf[q], acc[t], 0, 0, 0);
+                        }
             }
         }
     }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lds[wave][t * 16 + 4 * (lane >> 4) + e][r] = acc[t][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 256; i += 64 * WAVES) {
+        const int64_t m = i >> 4, n = n0 + (i & 15);
+        if (m >= M || n >= N) continue;
+        float v[1] = {0.f}, bias[1] = {0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v[0] += lds[w][m][i & 15];
+        if (ep.bias) bias[0] = (float)reinterpret_cast<const T*>(ep.bias)[n];
+        papr_pack<T, 1> res;
+        if (ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
+        finish<T, OUT_FORWARD, 1>(v, m, n, N, bias, res, ep);
+    }
+}
+
+// Up to here the few-rows kernel is the faster one: 1 x 1024 -> 4096 bf16 3.8 us against 10.1 of 64 x 64 tiles, 32 x 4096 -> 1024 26.8 against 29.6, 64 x 4096 -> 1024 48 against 30.
+constexpr int FEW_ROWS = 32;
+
+template <typename T>
+int launch_few_rows(const Operand& A, const Operand& B, int64_t K, bool vec, const Epilogue& ep, hipStream_t s) {
+    // (sixteen waves where there are fewer workgroups than compute units and steps enough: 16 x 4096 -> 1024 in bf16 16.6 us with eight)
+    const dim3 grid((unsigned)((B.rows + 15) / 16));
+    const bool many = B.rows <= 16 * papr_cu_count() / 2 && K >= 1024;
+    if (A.rows <= 16) {
+        if (many) few_rows_kernel<T, 1, 16><<<grid, 1024, 0, s>>>(A, B, K, vec, ep);
+        else few_rows_kernel<T, 1, 8><<<grid, 512, 0, s>>>(A, B, K, vec, ep);
+    } else {
+        if (many) few_rows_kernel<T, 2, 16><<<grid, 1024, 0, s>>>(A, B, K, vec, ep);
+        else few_rows_kernel<T, 2, 8><<<grid, 512, 0, s>>>(A, B, K, vec, ep);
+    }
+    PAPR_CHECK_LAUNCH("papr_linear_fwd");
+    return 0;
 }
 
 // The slabs of a sum in parts: a workgroup takes 64 results, its four waves a quarter of the parts each, quarters added in order.
@@ -505,72 +774,94 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
     }
 }
 
-typedef Shape<2, 4, 4, 2> Large;                   // 256 x 256, eight waves
-typedef Shape<2, 2, 2, 2> Middle;                  // 128 x 128, four waves
-typedef Shape<2, 2, 1, 1> Small;                   // 64 x 64, four waves
+typedef Shape<2, 4, 4, 2, 4> Large;                // 256 x 256, eight waves
+typedef Shape<2, 2, 4, 2, 3> Wide;                 // 256 x 128, four waves
+typedef Shape<2, 2, 2, 2, 4> Middle;               // 128 x 128, four waves
+typedef Shape<2, 2, 1, 1, 4> Small;                // 64 x 64, four waves
 
-// Which tile, and into how many parts the sum is cut: the least estimated time.  A tile's time is its area times the steps of its part over the rate its shape
-// reaches, the launch as many of them in turn as a compute unit gets; parts cost their slabs' way to memory and back.
+// Which tile shape, and into how many parts the sum is cut: the least estimated time.  A compute unit gets q = ceil(tiles x parts / compute units) tiles; a tile costs
+// its 64-term steps and a fixed part (filling the pipeline, writing the results), both measured per shape with the unit's resident workgroups sharing it; fewer
+// tiles than that leave a unit waiting more (`lone`: a single tile against a full unit).  Parts cost their slabs' way to memory and back and one more launch.
+//   streaming 16-bit (8192 x 4096 x 1024 and 65,536 x 1024 x 1024):  256 x 256 1.5 us a step, 256 x 128 0.87, 128 x 128 0.55, 64 x 64 0.24
+//   16-bit through registers (8191 x 1001 x 1003, 8-bit rows):                          3.5         4.0             1.6          0.55
+//   float32 (512,000 x 256 x 256, 25,600 x 256 x 142):                                  11          6               3.2          1.3
+enum { PATH_STREAM, PATH_REGISTERS, PATH_F32 };
 struct Choice { int shape; int64_t parts, per; };      // per: terms of a part
-int step_of(int type) { return type == PAPR_TYPE_F32 ? 32 : 64; }
-Choice choose(int64_t M, int64_t N, int64_t K, int type, bool may_split) {
-    const int bk = step_of(type);
-    const int64_t cus = papr_cu_count(), steps = (K + bk - 1) / bk;
-    static const int side[3] = {256, 128, 64}, resident[3] = {1, 2, 4};
-    static const double rate[3] = {1.0, 0.8, 0.45};
+Choice choose(int64_t M, int64_t N, int64_t K, int path, bool may_split) {
+    static const int rows[4] = {256, 256, 128, 64}, cols[4] = {256, 128, 128, 64}, resident[4] = {1, 2, 2, 4};
+    static const double step_us[3][4] = {{1.5, 0.87, 0.55, 0.24}, {3.5, 4.0, 1.6, 0.55}, {11.0, 6.0, 3.2, 1.3}};
+    static const double fixed_us[4] = {9.0, 5.0, 2.5, 1.0};
+    static const double lone[3][4] = {{1.0, 1.4, 1.2, 2.0}, {1.0, 1.4, 1.8, 1.5}, {1.0, 1.6, 1.4, 1.0}};
+    const int64_t cus = papr_cu_count(), steps = (K + 63) / 64;
     Choice best = {0, 1, 0};
     double least = 0;
-    for (int s = 0; s < 3; ++s) {
-        const int64_t tiles = ((M + side[s] - 1) / side[s]) * ((N + side[s] - 1) / side[s]), slots = cus * resident[s];
-        int64_t tried[3] = {1, slots / tiles, 2 * slots / tiles};
+    for (int s = 0; s < 4; ++s) {
+        const int64_t tiles = ((M + rows[s] - 1) / rows[s]) * ((N + cols[s] - 1) / cols[s]);
+        const int64_t tried[4] = {1, cus / tiles, 2 * cus / tiles, 4 * cus / tiles};
         for (int64_t parts : tried) {
-            if (parts > steps / 4) parts = steps / 4;
+            if (parts > 1 && !may_split) continue;
+            if (parts > steps / 2) parts = steps / 2;
             if (parts > 1024) parts = 1024;
-            if (parts < 1 || !may_split) parts = 1;
+            if (parts < 1) parts = 1;
             const int64_t per = (steps + parts - 1) / parts;
             parts = (steps + per - 1) / per;
-            const int64_t turns = (tiles * parts + slots - 1) / slots;
-            // (in matrix instruction time of one compute unit: 4096 products of a 16-bit type a cycle; slabs at 2 KB a cycle over the chip; 3 us a launch)
-            double t = (double)turns * resident[s] * ((double)side[s] * side[s] * (per + 3) * bk / (4096 * rate[s]));
-            if (parts > 1) t += 2.0 * parts * M * N * 4 / 2048 + 7000;
-            if (least == 0 || t < least) { least = t; best = {s, parts, per * bk}; }
+            const int64_t q = (tiles * parts + cus - 1) / cus;
+            const double share = q < resident[s] ? 1 + (lone[path][s] - 1) * (double)(resident[s] - q) / (resident[s] > 1 ? resident[s] - 1 : 1) : 1;
+            double t = (double)q * (step_us[path][s] * per * share + fixed_us[s]);
+            if (parts > 1) t += (double)parts * M * N * 8 / 5e6 + 4;
+            if (least == 0 || t < least) { least = t; best = {s, parts, per * 64}; }
         }
     }
     return best;
 }
+int path_of(int type, bool vec, int keep) { return type == PAPR_TYPE_F32 ? PATH_F32 : vec && !keep ? PATH_STREAM : PATH_REGISTERS; }
 
-template <typename T, int LA, int LB, int FMT, bool VEC, int OUT, typename S>
-int launch_shape(const Operand& A, const Operand& B, int64_t K, const Choice& c, const Epilogue& ep, hipStream_t s) {
-    typedef Plan<T, LA, LB, FMT, VEC, S> P;
-    static_assert(P::LDS <= 160 * 1024, "a compute unit's LDS");
-    auto kernel = product_kernel<T, LA, LB, FMT, VEC, OUT, S>;
-    static_assert(32 % P::BK == 0 || 64 % P::BK == 0, "parts are whole steps");
+template <auto KERNEL, size_t LDS, typename S>
+int launch_kernel(const Operand& A, const Operand& B, int64_t K, const Choice& c, const Epilogue& ep, hipStream_t s) {
+    static_assert(LDS <= 160 * 1024, "a compute unit's LDS");
     const int64_t tm = (A.rows + S::TM - 1) / S::TM, tn = (B.rows + S::TN - 1) / S::TN, grid = tm * tn * c.parts;
     PAPR_REQUIRE(grid < (int64_t)1 << 31, "papr_linear: %lld tiles", (long long)grid);
-    static std::atomic<uint64_t> ready{0};            // (devices on which this kernel may already use more than 64 KB of LDS)
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (P::LDS > 65536 && !(ready.load(std::memory_order_relaxed) & bit)) {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)P::LDS);
-        ready.fetch_or(bit, std::memory_order_relaxed);
+    if (LDS > 65536) {
+        static std::atomic<uint64_t> ready{0};        // (devices on which this kernel may already use more than 64 KB of LDS)
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        const uint64_t bit = 1ull << (dev & 63);
+        if (dev > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
+            (void)hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
+            ready.fetch_or(bit, std::memory_order_relaxed);
+        }
     }
-    kernel<<<dim3((unsigned)grid), dim3(S::THREADS), P::LDS, s>>>(A, B, K, c.per, (unsigned)tm, (unsigned)tn, ep);
+    KERNEL<<<dim3((unsigned)grid), dim3(S::THREADS), LDS, s>>>(A, B, K, c.per, (unsigned)tm, (unsigned)tn, ep);
     PAPR_CHECK_LAUNCH("papr_linear product");
     return 0;
 }
 
+template <typename T, int LA, int LB, int FMT, bool VEC, int OUT, typename S>
+int launch_shape(const Operand& A, const Operand& B, int64_t K, const Choice& c, const Epilogue& ep, hipStream_t s) {
+    if constexpr (sizeof(T) == 2 && FMT == 0 && VEC && S::TM >= 128)
+        return launch_kernel<stream_kernel<T, LA, LB, OUT, S>, Stream<T, LA, LB, S>::LDS, S>(A, B, K, c, ep, s);
+    else
+        return launch_kernel<product_kernel<T, LA, LB, FMT, VEC, OUT, S>, Plan<T, LA, LB, FMT, VEC, S>::LDS, S>(A, B, K, c, ep, s);
+}
+
+template <typename T, int LA, int LB, int FMT, bool VEC, int OUT>
+int launch_choice(const Choice& c, const Operand& A, const Operand& B, int64_t K, const Epilogue& ep, hipStream_t s) {
+    switch (c.shape) {
+        case 0: return launch_shape<T, LA, LB, FMT, VEC, OUT, Large>(A, B, K, c, ep, s);
+        case 1: return launch_shape<T, LA, LB, FMT, VEC, OUT, Wide>(A, B, K, c, ep, s);
+        case 2: return launch_shape<T, LA, LB, FMT, VEC, OUT, Middle>(A, B, K, c, ep, s);
+        default: return launch_shape<T, LA, LB, FMT, VEC, OUT, Small>(A, B, K, c, ep, s);
+    }
+}
 template <typename T, int LA, int LB, int FMT, int OUT>
 int launch_product(const Choice& c, bool vec, const Operand& A, const Operand& B, int64_t K, const Epilogue& ep, hipStream_t s) {
-    if (c.shape == 0) return vec ? launch_shape<T, LA, LB, FMT, true, OUT, Large>(A, B, K, c, ep, s) : launch_shape<T, LA, LB, FMT, false, OUT, Large>(A, B, K, c, ep, s);
-    if (c.shape == 1) return vec ? launch_shape<T, LA, LB, FMT, true, OUT, Middle>(A, B, K, c, ep, s) : launch_shape<T, LA, LB, FMT, false, OUT, Middle>(A, B, K, c, ep, s);
-    return vec ? launch_shape<T, LA, LB, FMT, true, OUT, Small>(A, B, K, c, ep, s) : launch_shape<T, LA, LB, FMT, false, OUT, Small>(A, B, K, c, ep, s);
+    return vec ? launch_choice<T, LA, LB, FMT, true, OUT>(c, A, B, K, ep, s) : launch_choice<T, LA, LB, FMT, false, OUT>(c, A, B, K, ep, s);
 }
 
 // C = A B^T into contiguous rows of type T, the sum in parts where the tiles alone do not fill the chip
 template <typename T, int LA, int LB, int FMT>
 int rows_product(bool vec, const Operand& A, const Operand& B, int64_t K, void* out, float* slab, hipStream_t s) {
-    const Choice c = choose(A.rows, B.rows, K, sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, true);
+    const Choice c = choose(A.rows, B.rows, K, path_of(sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, vec, FMT), true);
     Epilogue ep = {};
     if (c.parts == 1) {
         ep.out = out;
@@ -587,8 +878,12 @@ int rows_product(bool vec, const Operand& A, const Operand& B, int64_t K, void* 
 
 // float32 slabs of one product
 size_t slab_floats(int type, int64_t M, int64_t N, int64_t K) {
-    const int64_t parts = choose(M, N, K, type, true).parts;
-    return parts > 1 ? (size_t)(parts * M * N) : 0;
+    size_t most = 0;                                  // (the path, and with it the choice, depends on alignments that the workspace's size does not know)
+    for (int path = type == PAPR_TYPE_F32 ? PATH_F32 : PATH_STREAM; path <= (type == PAPR_TYPE_F32 ? PATH_F32 : PATH_REGISTERS); ++path) {
+        const int64_t parts = choose(M, N, K, path, true).parts;
+        if (parts > 1 && (size_t)(parts * M * N) > most) most = (size_t)(parts * M * N);
+    }
+    return most;
 }
 
 struct SlopeGrid { int lanes; int64_t blocks, rows_per_block; unsigned cols; };
@@ -630,7 +925,8 @@ extern "C" int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t
     const Operand A = {x, ldx, d->M, nullptr}, B = {w, ldw, d->N, nullptr};
     const Epilogue ep = {y, bias, res, ld_res, z, d->act,
                          papr_rows_aligned(y, d->N, d->N, b) && (!z || ((uintptr_t)z & 15) == 0) && (!res || papr_rows_aligned(res, ld_res, d->N, b))};
-    const Choice c = choose(d->M, d->N, d->K, d->type, false);
+    if (d->M <= FEW_ROWS) PAPR_TYPE_SWITCH(d->type, return launch_few_rows<T>(A, B, d->K, vec, ep, as_stream(stream)));
+    const Choice c = choose(d->M, d->N, d->K, path_of(d->type, vec, 0), false);
     PAPR_TYPE_SWITCH(d->type, return (launch_product<T, K_RUNS, K_RUNS, 0, OUT_FORWARD>(c, vec, A, B, d->K, ep, as_stream(stream))));
 }
 
