@@ -11,7 +11,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libpapr_hip.so")
-SOURCES = ["error.hip", "knn.hip", "cloud.hip", "features.hip", "pairs.hip", "rowops.hip", "gemm.hip", "chain4.hip", "conv.hip", "unet.hip", "small_unet.hip", "adam.hip", "linear.hip", "join.hip", "rows8.hip"]
+SOURCES = ["error.hip", "knn.hip", "cloud.hip", "features.hip", "pairs.hip", "rowops.hip", "gemm.hip", "chain4.hip", "conv.hip", "unet.hip", "small_unet.hip", "adam.hip", "linear.hip", "linear_f32.hip", "linear_f16.hip", "linear_bf16.hip", "join.hip", "rows8.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics",
          "-Wall", "-Wno-unused-function", "-Wno-inline-asm"]
 # chain4.hip: no packed-fp32 VALU (v_pk_mul_f32 / v_pk_add_f32 come from the SLP vectoriser).  Measured on MI355X (round 2,
@@ -21,7 +21,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
 # (MI355X_MICROARCH.md, "price of one filler beside MFMAs").
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]      # (the same caution by target feature: the host pass warns that it does not know it)
 EXTRA_FLAGS = {"chain4.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-spill-vgpr-to-agpr=0"],
-               "linear.hip": NO_PACKED_FP32, "join.hip": NO_PACKED_FP32, "rows8.hip": NO_PACKED_FP32}
+               "join.hip": NO_PACKED_FP32, "rows8.hip": NO_PACKED_FP32, "linear.hip": NO_PACKED_FP32, "linear_f32.hip": NO_PACKED_FP32, "linear_f16.hip": NO_PACKED_FP32,
+               "linear_bf16.hip": NO_PACKED_FP32}
 # chain4.hip keeps its weight fragments in a[0:127] by name, from inline asm; the compiler does not know they are taken in between
 # and moves values of its own into AGPRs when it runs out of VGPRs.  A build whose device code holds any v_accvgpr_* is wrong.
 NO_ACCVGPR = ["chain4.hip"]
@@ -88,6 +89,9 @@ def _register_metadata_ok(asm, kernel_substr="mlp_chain4_kernel"):
     return problems
 
 
+ROW_BLOCKS = ["join.hip", "rows8.hip", "linear.hip", "linear_f32.hip", "linear_f16.hip", "linear_bf16.hip"]      # (headers of their own)
+
+
 def _stale(target, deps):
     if not os.path.exists(target):
         return True
@@ -97,7 +101,7 @@ def _stale(target, deps):
 
 def build_library(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    headers = [os.path.join(CSRC, h) for h in ("papr_common.h", "block_types.h", "h3_common.h", "unet_parts.h", "chain.h", "chain4_kloop.inc", "chain4_fused.inc", "chain4_krun.inc")] + [os.path.join(os.path.dirname(PKG), "include", "papr_hip.h")]
+    headers = [os.path.join(CSRC, h) for h in ("papr_common.h", "h3_common.h", "unet_parts.h", "chain.h", "chain4_kloop.inc", "chain4_fused.inc", "chain4_krun.inc")] + [os.path.join(os.path.dirname(PKG), "include", "papr_hip.h")]
     objdir = os.path.join(PKG, "build")
     os.makedirs(objdir, exist_ok=True)
     objs, procs = [], []
@@ -105,7 +109,7 @@ def build_library(force=False, verbose=True):
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src.replace(".hip", ".o"))
         objs.append(o)
-        if force or _stale(o, [s] + headers):
+        if force or _stale(o, [s] + headers + ([os.path.join(CSRC, h) for h in ("block_types.h", "linear.h", "linear_kernels.h")] if src in ROW_BLOCKS else [])):
             cmd = [hipcc] + FLAGS + EXTRA_FLAGS.get(src, []) + ["-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)

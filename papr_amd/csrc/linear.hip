@@ -1,892 +1,21 @@
-// Linear layers over rows with their epilogue, and their backward pass, on the matrix pipe:
-//     z = x W^T + b,  y = act(z) + r          d_z = d_y act'(z),  d_x = d_z W,  d_W = d_z^T x,  d_b = sum of the rows of d_z
-// x (M, K), W (N, K) in float32, float16 or bfloat16; sums in float32.  One kernel, C(m, n) = sum_k A(m, k) B(n, k), serves the three products; an operand
-// lies with k contiguous (x and W forward, d_z in d_x) or with its rows contiguous (W in d_x, both in d_W), or it is a set of 8-bit rows (rows8.hip: d_W).
-//   * float16 / bfloat16: the values themselves are the matrix operands.
-//   * float32: every value is cut into three bfloat16 parts (8 + 8 + 8 bits, rounded to nearest: exact for every normal number) on its way into LDS, and the six
-//     products of weight 2^-18 and more are summed -- what is left out is below 2^-26 of a term, less than float32's own rounding.  2.5 PFLOP/s / 6 = 416 TFLOP/s
-//     against 157 of the float32 matrix instructions.  Infinities and NaN give NaN (inf - inf), magnitudes above 2^128 (1 - 2^-9) count as infinite.
-//   * d_z is an operand of two products and is kept in the rows' type (rounded once, to nearest): float32 for float32 rows; for 16-bit rows its rounding is of the
-//     size of the gradients' own.  d_b sums it in float32 before that rounding.
-#include "block_types.h"
-#include <atomic>
+// The C entry points of the linear layers (the mathematics and the kernels: linear_kernels.h).
+#include "linear.h"
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef f16 f16x8 __attribute__((ext_vector_type(8)));
-typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+using namespace papr_linear;
 
 namespace {
-
-// Phi(z) and phi(z) of the erf form of gelu.  float32 rows: the library's erf and exp.  16-bit rows: erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2), t = 1 / (1 + p x)
-// (Abramowitz and Stegun 7.1.26, 1.5e-7 absolute), a sixteenth of the rows' own rounding and a third of erf's instructions: erf in the epilogue of an
-// 8192 x 1024 -> 4096 layer took longer than its matrix instructions.
-template <bool EXACT>
-__device__ __forceinline__ void gauss(float z, float& cdf, float& pdf) {
-    if (EXACT) {
-        cdf = 0.5f * erfcf(z * -0.70710678f);
-        pdf = 0.39894228f * expf(-0.5f * z * z);
-    } else {
-        const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
-        const float e = __builtin_amdgcn_exp2f(x * x * -1.44269504f);
-        const float q = 0.5f * t * e * __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, __builtin_fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-        cdf = z < 0.f ? q : 1.f - q;
-        pdf = 0.39894228f * e;
-    }
-}
-// v <- act(v)
-template <bool EXACT, int N>
-__device__ __forceinline__ void act_values(float (&v)[N], int act) {
-    if (act == PAPR_ACT_RELU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = v[i] > 0.f ? v[i] : (v[i] == v[i] ? 0.f : v[i]);
-    } else if (act == PAPR_ACT_LEAKY_RELU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = v[i] > 0.f ? v[i] : 0.2f * v[i];
-    } else if (act == PAPR_ACT_GELU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float cdf, pdf;
-            gauss<EXACT>(v[i], cdf, pdf);
-            v[i] *= cdf;
-        }
-    } else if (act == PAPR_ACT_SILU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] *= papr_sigmoid(v[i]);
-    }
-}
-// g <- g act'(z)
-template <bool EXACT, int N>
-__device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], int act) {
-    if (act == PAPR_ACT_RELU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = z[i] > 0.f ? g[i] : 0.f;
-    } else if (act == PAPR_ACT_LEAKY_RELU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = z[i] > 0.f ? g[i] : 0.2f * g[i];
-    } else if (act == PAPR_ACT_GELU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float cdf, pdf;
-            gauss<EXACT>(z[i], cdf, pdf);
-            g[i] *= __builtin_fmaf(z[i], pdf, cdf);
-        }
-    } else if (act == PAPR_ACT_SILU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float p = papr_sigmoid(z[i]);
-            g[i] *= p * __builtin_fmaf(z[i], 1.f - p, 1.f);
-        }
-    }
-}
-
-enum { K_RUNS = 0, ROWS_RUN = 1 };                // which index of an operand is contiguous in memory
-enum { OUT_FORWARD = 0, OUT_ROWS = 1, OUT_SLAB = 2 };
-
-struct Operand { const void* p; int64_t ld; int64_t rows; const uint8_t* exps; };       // exps: 8-bit rows only (ld in codes)
-struct Epilogue {                                  // out and z (M, N) contiguous
-    void* out;
-    const void* bias; const void* res; int64_t ld_res; void* z;
-    int act;
-    int wide;                                      // whole 16-byte vectors in every row of out, z and res
-};
-
-template <typename T> struct Matrix { typedef bf16x8 frag; };
-template <> struct Matrix<f16> { typedef f16x8 frag; };
-__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Wint-to-pointer-cast"      // (an LDS address is a 32-bit offset: the host pass sees a 64-bit pointer type)
-__device__ __forceinline__ s16x4 read_tr4(unsigned a) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a); }
-#pragma clang diagnostic pop
-
-// One operand's tile of R rows x BK in LDS, `PLANES` of them, and the registers its next tile waits in.
-//   K_RUNS:   image [R][BK] halfs, 16-byte pieces exchanged by the row number so that 16 rows' reads of one piece cover all 64 banks.
-//   ROWS_RUN: image [BK][R + pad] halfs as it lies in memory; the transposing LDS read hands a lane 8 consecutive k of its row.  The row stride is
-//             64 bytes modulo 256: the four k a 16-lane group reads lie on different quarters of the banks.
-// FMT: 0 rows of type T, else 8-bit rows (ROWS_RUN only).  A thread's pieces sit at fixed 32-bit offsets from a uniform tile address that advances with k.
-template <typename T, int LAYOUT, int FMT, bool VEC, int R, int BK, int THREADS>
-struct Tile {
-    static constexpr bool SPLIT = sizeof(T) == 4 && FMT == 0;
-    static constexpr int PLANES = SPLIT ? 3 : 1;
-    static constexpr int PIECE = SPLIT ? 4 : 8;                                   // elements of one load
-    static constexpr int BYTES = FMT ? 1 : sizeof(T);
-    static constexpr int N = R * BK / PIECE / THREADS;
-    static constexpr int STRIDE = LAYOUT == K_RUNS ? BK : (R * 2 % 256 == 64 ? R : R + 32);
-    static constexpr int PLANE = (LAYOUT == K_RUNS ? R : BK) * STRIDE;            // halfs
-    static constexpr int HALFS = PLANES * PLANE;
-    static_assert(R * BK % (PIECE * THREADS) == 0, "whole pieces per thread");
-    typedef typename Matrix<T>::frag frag;
-
-    uint4 reg[N];
-    unsigned off[N];                                                              // bytes from the tile's address
-    uint8_t ex[FMT ? N : 1];
-    unsigned exo[FMT ? N : 1];
-    const char* base;                                                             // (uniform) rows r0, the next k
-    const uint8_t* exb;
-    int64_t ld;
-
-    // piece q of this thread: (row, k) of its first element inside the tile
-    static __device__ __forceinline__ void where(int q, int& r, int& k) {
-        const int id = q * THREADS + threadIdx.x;
-        if (LAYOUT == K_RUNS) { r = id / (BK / PIECE); k = id % (BK / PIECE) * PIECE; }
-        else { k = id / (R / PIECE); r = id % (R / PIECE) * PIECE; }
-    }
-    // swizzled place of 16-byte piece c of row r (halfs)
-    static __device__ __forceinline__ int place(int r, int c) {
-        const int sw = BK == 64 ? (r >> 1) & 7 : BK == 32 ? (r >> 2) & 3 : (r >> 3) & 1;
-        return r * STRIDE + ((c ^ sw) << 3);
-    }
-
-    __device__ __forceinline__ void start(const Operand& o, int64_t r0, int64_t k0) {
-        ld = o.ld;
-        base = reinterpret_cast<const char*>(o.p) + (LAYOUT == K_RUNS ? r0 * ld + k0 : k0 * ld + r0) * BYTES;
-        if (FMT) exb = o.exps + k0 * (ld >> 5) + (r0 >> 5);
-        const int64_t left = (FMT ? ld : o.rows) - r0;
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            int r, k;
-            where(q, r, k);
-            if (r >= left) r = LAYOUT == K_RUNS ? (int)left - 1 : 0;              // (rows past the end: some row of the operand, its results are never stored)
-            off[q] = (unsigned)((LAYOUT == K_RUNS ? (int64_t)r * ld + k : (int64_t)k * ld + r) * BYTES);
-            if (FMT) exo[q] = (unsigned)(k * (ld >> 5) + (r >> 5));
-        }
-    }
-    // the next tile: k0 .. k0 + BK of K terms.  `inside`: every piece may be read whole.  A piece that crosses the end of a contiguous row of rows reads the start
-    // of the next one (those rows of the product are never stored), but behind the last k there is no next one.
-    __device__ __forceinline__ void load(const Operand& o, int64_t r0, int64_t k0, int64_t K) {
-        bool inside = k0 + BK <= K;
-        if (LAYOUT == ROWS_RUN && !VEC && FMT == 0) inside = k0 + BK < K && o.rows >= PIECE;
-        if (inside) {
-#pragma unroll
-            for (int q = 0; q < N; ++q) {
-                const char* src = base + off[q];
-                if (FMT) {
-                    const uint2 c = *reinterpret_cast<const uint2*>(src);
-                    reg[q].x = c.x; reg[q].y = c.y;
-                    ex[q] = exb[exo[q]];
-                } else if (VEC) reg[q] = *reinterpret_cast<const uint4*>(src);
-                else __builtin_memcpy(&reg[q], __builtin_assume_aligned(src, sizeof(T)), 16);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < N; ++q) {
-                int r, k;
-                where(q, r, k);
-                const bool in = k0 + k < K;
-                const char* src = in ? base + off[q] : base;                      // (base: rows r0, the tile's first k < K)
-                if (FMT) {
-                    const uint2 c = *reinterpret_cast<const uint2*>(src);
-                    reg[q].x = in ? c.x : 0u; reg[q].y = in ? c.y : 0u;
-                    ex[q] = exb[in ? exo[q] : 0u];
-                } else if (VEC) {
-                    const uint4 t = *reinterpret_cast<const uint4*>(src);
-                    reg[q].x = in ? t.x : 0u; reg[q].y = in ? t.y : 0u; reg[q].z = in ? t.z : 0u; reg[q].w = in ? t.w : 0u;
-                } else {
-                    papr_pack<T, PIECE> t;
-                    if (LAYOUT == ROWS_RUN && r0 + r >= o.rows) r = 0;
-#pragma unroll
-                    for (int i = 0; i < PIECE; ++i) {
-                        const bool ok = LAYOUT == K_RUNS ? k0 + k + i < K : in && r0 + r + i < o.rows;
-                        t.v[i] = ok ? reinterpret_cast<const T*>(src)[i] : (T)0.f;
-                    }
-                    __builtin_memcpy(&reg[q], &t, 16);
-                }
-            }
-        }
-        base += (LAYOUT == K_RUNS ? (int64_t)BK : BK * ld) * BYTES;
-        if (FMT) exb += BK * (ld >> 5);
-    }
-
-    __device__ __forceinline__ void store(short* lds) const {
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            int r, k;
-            where(q, r, k);
-            const int at = LAYOUT == K_RUNS ? place(r, k >> 3) + (k & 7) : k * STRIDE + r;
-            if (FMT) {
-                float v[4], w[4];
-                const float scale = __uint_as_float((unsigned)ex[q] << 23);
-                papr_codes_to_float<FMT>(reg[q].x, scale, v);
-                papr_codes_to_float<FMT>(reg[q].y, scale, w);
-                frag h;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { h[i] = v[i]; h[4 + i] = w[i]; }     // (exact: at most 8 significant bits)
-                *reinterpret_cast<frag*>(lds + at) = h;
-            } else if (SPLIT) {
-                const float f[4] = {__uint_as_float(reg[q].x), __uint_as_float(reg[q].y), __uint_as_float(reg[q].z), __uint_as_float(reg[q].w)};
-                papr_pack<bf16, 4> p[3];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[0].v[i] = (bf16)f[i];
-                    const float rest = f[i] - (float)p[0].v[i];
-                    p[1].v[i] = (bf16)rest;
-                    p[2].v[i] = (bf16)(rest - (float)p[1].v[i]);
-                }
-#pragma unroll
-                for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<bf16, 4>*>(lds + n * PLANE + at) = p[n];
-            } else *reinterpret_cast<uint4*>(lds + at) = reg[q];
-        }
-    }
-
-    // this lane's operand of the 16-term step ks: row base + (lane & 31), k = 8 (lane >> 5) + 0 .. 7
-    static __device__ __forceinline__ frag read(const short* lds, int plane, int row, int ks) {
-        const int lane = threadIdx.x & 63;
-        s16x8 v;
-        if (LAYOUT == K_RUNS) {
-            v = *reinterpret_cast<const s16x8*>(lds + plane * PLANE + place(row + (lane & 31), ks * 2 + (lane >> 5)));
-        } else {
-            const unsigned a = (unsigned)(size_t)(lds + plane * PLANE) +
-                               2u * (unsigned)((ks * 16 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * STRIDE + row + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
-            const s16x4 lo = read_tr4(a), hi = read_tr4(a + 8 * STRIDE);
-            v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-        return __builtin_bit_cast(frag, v);
-    }
-};
-
-// Workgroup -> (row tile, column tile, part of the sum).  Workgroups go to the eight XCDs in turn: each takes a contiguous run of tiles, and the run walks
-// GROUP row tiles down before it steps to the next column tile, so that an XCD's workgroups of one moment share operand tiles in its L2.
-struct Place { int m, n, part; };
-__device__ __forceinline__ Place place_of(unsigned id, unsigned total, unsigned tm, unsigned tn) {
-    constexpr unsigned XCDS = 8, GROUP = 8;
-    const unsigned x = id % XCDS, q = id / XCDS, per = total / XCDS, rem = total % XCDS;
-    const unsigned t = x * per + (x < rem ? x : rem) + q;
-    Place p;
-    p.part = (int)(t / (tm * tn));
-    const unsigned r = t % (tm * tn), g = r / (GROUP * tn), in = r % (GROUP * tn), high = tm - g * GROUP < GROUP ? tm - g * GROUP : GROUP;
-    p.m = (int)(g * GROUP + in % high);
-    p.n = (int)(in / high);
-    return p;
-}
-
-// Tile shapes: waves WM x WN, each IM x IN blocks of 32 x 32; DEPTH stages of a streaming kernel.
-template <int WM_, int WN_, int IM_, int IN_, int DEPTH_>
-struct Shape {
-    static constexpr int DEPTH = DEPTH_, WM = WM_, WN = WN_, IM = IM_, IN = IN_, THREADS = 64 * WM * WN, TM = WM * IM * 32, TN = WN * IN * 32;
-    static constexpr int EPI_STRIDE = IN * 32 + 8;                                // floats: rows four apart lie on the other half of the banks
-    static constexpr size_t EPI = (size_t)WM * WN * 32 * EPI_STRIDE * 4;
-};
-
-template <typename T, int LA, int LB, int FMT, bool VEC, typename S>
-struct Plan {
-    static constexpr int BK = sizeof(T) == 2 ? 64 : S::TM > 64 ? 16 : 32;       // (divides step_of)
-    typedef Tile<T, LA, 0, VEC, S::TM, BK, S::THREADS> TA;
-    typedef Tile<T, LB, FMT, VEC, S::TN, BK, S::THREADS> TB;
-    static constexpr int BUF = TA::HALFS + TB::HALFS;
-    static constexpr size_t LOOP = (size_t)2 * BUF * 2, LDS = S::EPI > LOOP ? S::EPI : LOOP;
-};
-
-// E consecutive results of row m from column n on
-template <typename T, int OUT, int E>
-__device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int64_t N, const float (&bias)[E], const papr_pack<T, E>& res, const Epilogue& ep) {
-    if (OUT == OUT_FORWARD) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) v[i] += bias[i];
-        if (ep.z) {
-            papr_pack<T, E> t;
-#pragma unroll
-            for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
-            *reinterpret_cast<papr_pack<T, E>*>(reinterpret_cast<T*>(ep.z) + m * N + n) = t;
-        }
-        act_values<sizeof(T) == 4>(v, ep.act);
-        if (ep.res)
-#pragma unroll
-            for (int i = 0; i < E; ++i) v[i] += (float)res.v[i];
-    }
-    papr_pack<T, E> t;
-#pragma unroll
-    for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
-    *reinterpret_cast<papr_pack<T, E>*>(reinterpret_cast<T*>(ep.out) + m * N + n) = t;
-}
-
-// The results of a workgroup's tile, from the accumulators of its waves.  smem: Shape::EPI bytes, free of earlier readers.
-template <typename T, int OUT, typename S>
-__device__ __forceinline__ void write_tile(const f32x16 (&acc)[S::IM][S::IN], short* smem, int64_t m0, int64_t n0, int64_t M, int64_t N, int part, const Epilogue& ep) {
-    constexpr int IM = S::IM, IN = S::IN, EPI_STRIDE = S::EPI_STRIDE;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
-    if (OUT == OUT_SLAB) {
-        // float32, as it lies: a lane holds column lane & 31 of a 32 x 32 block, rows (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
-        float* out = reinterpret_cast<float*>(ep.out) + (int64_t)part * M * N;
-#pragma unroll
-        for (int j = 0; j < IN; ++j) {
-            const int64_t n = n0 + (wn * IN + j) * 32 + (lane & 31);
-#pragma unroll
-            for (int i = 0; i < IM; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int64_t m = m0 + (wm * IM + i) * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
-                    if (n < N && m < M) out[m * N + n] = acc[i][j][e];
-                }
-        }
-        return;
-    }
-    // Through LDS, 32 rows of the wave's own at a time (no barrier), so that a lane takes 16 bytes of a row: 16-byte loads and stores of whole lines.  Rows that do not
-    // start on 16 bytes: a lane takes single columns, 64 (32) lanes a row.
-    float* epi = reinterpret_cast<float*>(smem) + wave * 32 * EPI_STRIDE;
-    constexpr int COLS = IN * 32, E = 16 / sizeof(T), LPR = COLS / E, RPP = 64 / LPR;
-    const int64_t nw = n0 + wn * COLS;
-    const bool wide = ep.wide;
-    const int64_t n = nw + (wide ? lane % LPR * E : lane % COLS);
-    float bias[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) bias[i] = 0.f;
-    if (OUT == OUT_FORWARD && ep.bias && n < N) {
-        const T* src = reinterpret_cast<const T*>(ep.bias) + n;
-        if (wide) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) bias[i] = (float)src[i];
-        } else bias[0] = (float)src[0];
-    }
-#pragma unroll
-    for (int i = 0; i < IM; ++i) {
-        const int64_t mw = m0 + (wm * IM + i) * 32;
-#pragma unroll
-        for (int j = 0; j < IN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) epi[((e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * EPI_STRIDE + j * 32 + (lane & 31)] = acc[i][j][e];
-        if (wide) {
-            papr_pack<T, E> res[32 / RPP];
-#pragma unroll
-            for (int r = 0; r < 32 / RPP; ++r) {
-                const int64_t m = mw + r * RPP + lane / LPR;
-                if (OUT == OUT_FORWARD && ep.res && m < M && n < N) res[r] = *reinterpret_cast<const papr_pack<T, E>*>(reinterpret_cast<const T*>(ep.res) + m * ep.ld_res + n);
-            }
-#pragma unroll
-            for (int r = 0; r < 32 / RPP; ++r) {
-                const int64_t m = mw + r * RPP + lane / LPR;
-                float v[E];
-#pragma unroll
-                for (int c = 0; c < E; c += 4) {
-                    const float4 t = *reinterpret_cast<const float4*>(epi + (r * RPP + lane / LPR) * EPI_STRIDE + lane % LPR * E + c);
-                    v[c] = t.x; v[c + 1] = t.y; v[c + 2] = t.z; v[c + 3] = t.w;
-                }
-                if (m < M && n < N) finish<T, OUT, E>(v, m, n, N, bias, res[r], ep);
-            }
-        } else {
-            constexpr int ROWS = 64 / COLS;
-#pragma unroll 4
-            for (int r = 0; r < 32; r += ROWS) {
-                const int64_t m = mw + r + lane / COLS;
-                float v[1] = {epi[(r + lane / COLS) * EPI_STRIDE + lane % COLS]};
-                const float b1[1] = {bias[0]};
-                if (m < M && n < N) {
-                    papr_pack<T, 1> res;
-                    if (OUT == OUT_FORWARD && ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
-                    finish<T, OUT, 1>(v, m, n, N, b1, res, ep);
-                }
-            }
-        }
-    }
-}
-
-template <typename T, int LA, int LB, int FMT, bool VEC, int OUT, typename S>
-__global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Operand B, int64_t K, int64_t k_per_part, unsigned tiles_m, unsigned tiles_n, Epilogue ep) {
-    typedef Plan<T, LA, LB, FMT, VEC, S> P;
-    typedef typename P::TA TA;
-    typedef typename P::TB TB;
-    constexpr int IM = S::IM, IN = S::IN, BK = P::BK;
-    extern __shared__ __attribute__((aligned(16))) short smem[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
-    const Place at = place_of(blockIdx.x, gridDim.x, tiles_m, tiles_n);
-    const int64_t m0 = (int64_t)at.m * S::TM, n0 = (int64_t)at.n * S::TN;
-    const int64_t kb = at.part * k_per_part, ke = kb + k_per_part < K ? kb + k_per_part : K;
-    f32x16 acc[IM][IN];
-#pragma unroll
-    for (int i = 0; i < IM; ++i)
-#pragma unroll
-        for (int j = 0; j < IN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    TA a;
-    TB b;
-    a.start(A, m0, kb);
-    b.start(B, n0, kb);
-    a.load(A, m0, kb, K);
-    b.load(B, n0, kb, K);
-    a.store(smem);
-    b.store(smem + TA::HALFS);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t k0 = kb; k0 < ke; k0 += BK, buf ^= 1) {
-        const bool more = k0 + BK < ke;
-        if (more) {
-            a.load(A, m0, k0 + BK, K);
-            b.load(B, n0, k0 + BK, K);
-        }
-        const short *la = smem + buf * P::BUF, *lb = la + TA::HALFS;
-#pragma unroll
-        for (int ks = 0; ks < BK / 16; ++ks) {
-            typename TA::frag fa[TA::PLANES][IM];
-            typename TB::frag fb[TB::PLANES][IN];
-#pragma unroll
-            for (int p = 0; p < TA::PLANES; ++p)
-#pragma unroll
-                for (int i = 0; i < IM; ++i) fa[p][i] = TA::read(la, p, (wm * IM + i) * 32, ks);
-#pragma unroll
-            for (int p = 0; p < TB::PLANES; ++p)
-#pragma unroll
-                for (int j = 0; j < IN; ++j) fb[p][j] = TB::read(lb, p, (wn * IN + j) * 32, ks);
-#pragma unroll
-            for (int p = 0; p < TA::PLANES; ++p)
-#pragma unroll
-                for (int q = 0; q < TB::PLANES; ++q)
-                    if (p + q < 3)                // (the parts' products below 2^-26 are left out)
-#pragma unroll
-                        for (int i = 0; i < IM; ++i)
-#pragma unroll
-                            for (int j = 0; j < IN; ++j) acc[i][j] = mfma(fa[p][i], fb[q][j], acc[i][j]);
-        }
-        if (more) {
-            a.store(smem + (buf ^ 1) * P::BUF);
-            b.store(smem + (buf ^ 1) * P::BUF + TA::HALFS);
-        }
-        __syncthreads();
-    }
-    write_tile<T, OUT, S>(acc, smem, m0, n0, A.rows, B.rows, at.part, ep);
-}
-
-// The same product for 16-bit rows that start on 16 bytes: operands go straight from memory into LDS (global_load_lds, 16 bytes a lane), DEPTH stages of 32 terms, three
-// of them on their way while one is multiplied -- with one stage on its way in registers (product_kernel) half of a wave's time was waiting for it (256 x 256 tiles:
-// the matrix pipe 34 % busy).  An instruction fills 1 KB in lane order, so the images are made by which address a lane asks for:
-//   K_RUNS:   16 rows of 32 halfs, pieces exchanged by the row number as in Tile;
-//   ROWS_RUN: one "line" = the k rows q, q + LINES, q + 2 LINES, ... of R halfs one behind the other (1 KB), lines 1,088 bytes apart: the four consecutive k that a
-//             16-lane group of a transposing read wants lie on different quarters of the banks.
-// Rows past the operand's end: some row of it (never stored); terms past the part's end: a block of zeros.
-// The fragments of a 16-term step are read under the matrix instructions of the step before, and the stage's one barrier stands between its two steps: in front of
-// it a wave has read all of its stage (whose buffer the requests behind the barrier overwrite), behind it the next stage, requested three stages earlier, is there.
-__device__ const uint4 zero_block[4] = {};
-
-__device__ __forceinline__ void request16(const void* src, unsigned lds) {         // 64 lanes x 16 bytes -> LDS [lds, +1 KB) in lane order
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(src), "s"(lds) : "memory");
-}
-
-template <typename T, int LAYOUT, int R, int WAVES>
-struct Stage {
-    static constexpr int BK = 32, LINE = LAYOUT == K_RUNS ? 1024 : 1088, LINES = R * BK * 2 / 1024, BYTES = LINES * LINE, N = LINES / WAVES;
-    static_assert(LINES % WAVES == 0 && R * 2 <= 1024, "whole requests per wave");
-    typedef typename Matrix<T>::frag frag;
-    const char* src[N];                                                            // this lane's address of the next stage's requests
-    int k[N];                                                                      // its term inside the stage
-    int64_t step;
-
-    __device__ __forceinline__ void start(const Operand& o, int64_t r0, int64_t k0, int wave) {
-        const int lane = threadIdx.x & 63;
-        const int64_t left = o.rows - r0;
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const int line = wave * N + q;
-            int r;
-            if (LAYOUT == K_RUNS) {
-                r = line * 16 + lane / 4;
-                k[q] = 8 * ((lane & 3) ^ ((r >> 2) & 3));
-                if (r >= left) r = (int)left - 1;
-                src[q] = reinterpret_cast<const char*>(o.p) + ((r0 + r) * o.ld + k0 + k[q]) * 2;
-            } else {
-                r = 8 * (lane % (R / 8));
-                k[q] = line + lane / (R / 8) * LINES;
-                if (r >= left) r = 0;
-                src[q] = reinterpret_cast<const char*>(o.p) + ((k0 + k[q]) * o.ld + r0 + r) * 2;
-            }
-        }
-        step = (LAYOUT == K_RUNS ? (int64_t)BK : BK * o.ld) * 2;
-    }
-    // requests of the next stage; `left`: terms from its first on
-    __device__ __forceinline__ void request(unsigned lds, int64_t left, int wave) {
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const void* p = k[q] < left ? (const void*)src[q] : (const void*)zero_block;
-            request16(p, lds + (unsigned)(wave * N + q) * LINE);
-            src[q] += step;
-        }
-    }
-    // this lane's corner of the fragments (bytes): rows `row` .. + 31, step 0
-    static __device__ __forceinline__ unsigned corner(int row) {
-        const int lane = threadIdx.x & 63;
-        if (LAYOUT == K_RUNS) { const int r = row + (lane & 31); return (unsigned)(r * 64 + (((lane >> 5) ^ ((r >> 2) & 3)) << 4)); }
-        const int c = 8 * (lane >> 5) + ((lane & 15) >> 2);
-        return (unsigned)(c % LINES * LINE + c / LINES * R * 2 + (row + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2);
-    }
-    // LINES is 16 (R = 256) or 8 (R = 128): the second step's k + 16 is one half of a line on, or two quarters; four k on is four lines (LINES > 4, c < 12)
-    static __device__ __forceinline__ frag read(unsigned stage, unsigned corner, int ks) {
-        s16x8 v;
-        if (LAYOUT == K_RUNS) {
-            // (piece c of step 1 is piece c + 2: the exchange turns + 2 into ^ 2)
-            v = *reinterpret_cast<const __attribute__((address_space(3))) s16x8*>(stage + (corner ^ (unsigned)(ks * 32)));
-        } else {
-            const unsigned a = stage + corner + (unsigned)(ks * 16 / LINES * R * 2);
-            const s16x4 lo = read_tr4(a), hi = read_tr4(a + 4 * LINE);
-            v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-        return __builtin_bit_cast(frag, v);
-    }
-};
-
-template <typename T, int LA, int LB, typename S>
-struct Stream {
-    static constexpr int DEPTH = S::DEPTH;
-    typedef Stage<T, LA, S::TM, S::WM * S::WN> SA;
-    typedef Stage<T, LB, S::TN, S::WM * S::WN> SB;
-    static constexpr unsigned BYTES = SA::BYTES + SB::BYTES;
-    static constexpr size_t LOOP = (size_t)DEPTH * BYTES, LDS = S::EPI > LOOP ? S::EPI : LOOP;
-};
-
-template <typename T, int LA, int LB, int OUT, typename S>
-__global__ __launch_bounds__(S::THREADS, 2) void stream_kernel(Operand A, Operand B, int64_t K, int64_t k_per_part, unsigned tiles_m, unsigned tiles_n, Epilogue ep) {
-    typedef Stream<T, LA, LB, S> P;
-    typedef typename P::SA SA;
-    typedef typename P::SB SB;
-    constexpr int IM = S::IM, IN = S::IN, WAITING = (P::DEPTH - 2) * (SA::N + SB::N);          // requests of the stages behind the next one
-    extern __shared__ __attribute__((aligned(16))) short smem[];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
-    const Place at = place_of(blockIdx.x, gridDim.x, tiles_m, tiles_n);
-    const int64_t m0 = (int64_t)at.m * S::TM, n0 = (int64_t)at.n * S::TN;
-    const int64_t kb = at.part * k_per_part, ke = kb + k_per_part < K ? kb + k_per_part : K;
-    const int stages = (int)((ke - kb + 31) / 32);
-    const unsigned lds = (unsigned)(size_t)smem;
-    f32x16 acc[IM][IN];
-#pragma unroll
-    for (int i = 0; i < IM; ++i)
-#pragma unroll
-        for (int j = 0; j < IN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    SA a;
-    SB b;
-    a.start(A, m0, kb, wave);
-    b.start(B, n0, kb, wave);
-    int64_t left = ke - kb;
-    auto request = [&](int st) {
-        const unsigned to = lds + (unsigned)(st % P::DEPTH) * P::BYTES;
-        a.request(to, left, wave);
-        b.request(to + SA::BYTES, left, wave);
-        left -= 32;
-    };
-    unsigned ca[IM], cb[IN];
-#pragma unroll
-    for (int i = 0; i < IM; ++i) ca[i] = SA::corner((wm * IM + i) * 32);
-#pragma unroll
-    for (int j = 0; j < IN; ++j) cb[j] = SA::BYTES + SB::corner((wn * IN + j) * 32);
-    struct Frags { typename SA::frag a[IM]; typename SB::frag b[IN]; } f0, f1;
-    auto read = [&](Frags& f, int st, int ks) {
-        const unsigned from = lds + (unsigned)(st % P::DEPTH) * P::BYTES;
-#pragma unroll
-        for (int j = 0; j < IN; ++j) f.b[j] = SB::read(from, cb[j], ks);
-#pragma unroll
-        for (int i = 0; i < IM; ++i) f.a[i] = SA::read(from, ca[i], ks);
-    };
-    auto multiply = [&](const Frags& f) {
-#pragma unroll
-        for (int i = 0; i < IM; ++i)
-#pragma unroll
-            for (int j = 0; j < IN; ++j) acc[i][j] = mfma(f.a[i], f.b[j], acc[i][j]);
-    };
-#pragma unroll
-    for (int st = 0; st < P::DEPTH - 1; ++st) request(st);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WAITING) : "memory");     // stage 0 is there (every wave's part of it)
-    request(P::DEPTH - 1);
-    read(f0, 0, 0);
-    for (int st = 0; st < stages; ++st) {
-        read(f1, st, 1);
-        multiply(f0);
-        // stage st is read (its reads are waited for), stage st + 1 is there: the two stages behind it may be on their way
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WAITING) : "memory");
-        request(st + P::DEPTH);
-        read(f0, st + 1, 0);                       // (behind the last stage: a stage of zeros, not multiplied)
-        multiply(f1);
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    write_tile<T, OUT, S>(acc, smem, m0, n0, A.rows, B.rows, at.part, ep);
-}
-
-// Few rows (one token, a handful): the weight is read once and that is the time.  A workgroup takes 16 columns of the result, its waves a part of the sum each,
-// straight from memory into the operands of 16 x 16 x 32 matrix instructions (rows of x come from the caches); the parts meet in LDS, in wave order.
-template <typename T, int MT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand B, int64_t K, bool aligned, Epilogue ep) {
-    constexpr int PARTS = sizeof(T) == 4 ? 3 : 1, AHEAD = 8 / MT / (sizeof(T) / 2);
-    typedef typename Matrix<T>::frag frag;
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
-    __shared__ float lds[WAVES][MT * 16][17];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, k8 = lane >> 4 << 3;
-    const int64_t M = A.rows, N = B.rows, n0 = (int64_t)blockIdx.x * 16;
-    const int steps = (int)((K + 31) / 32), per = (steps + WAVES - 1) / WAVES, beg = wave * per, end = beg + per < steps ? beg + per : steps;
-    struct Eight { papr_pack<T, 8> t; };
-    auto fetch = [&](Eight& v, const Operand& o, int64_t row, int step) __attribute__((always_inline)) {
-        row = row < o.rows ? row : o.rows - 1;
-        const int64_t k = (int64_t)step * 32 + k8;
-        const T* src = reinterpret_cast<const T*>(o.p) + row * o.ld + k;
-        if ((int64_t)step * 32 + 32 <= K) {
-            if (aligned) {
-#pragma unroll
-                for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(&v.t)[i] = reinterpret_cast<const uint4*>(src)[i];
-            } else __builtin_memcpy(&v.t, src, sizeof(v.t));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v.t.v[i] = k + i < K ? src[i] : (T)0.f;
-        }
-    };
-    auto parts = [&](frag (&f)[PARTS], const Eight& v) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (PARTS == 1) f[0][i] = v.t.v[i];
-            else {
-                f[0][i] = (bf16)v.t.v[i];
-                const float rest = v.t.v[i] - (float)f[0][i];
-                f[1][i] = (bf16)rest;
-                f[2][i] = (bf16)(rest - (float)f[1][i]);
-            }
-        }
-    };
-    f32x4 acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s0 = beg; s0 < end; s0 += AHEAD) {
-        Eight wv[AHEAD], xv[AHEAD][MT];
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            if (s0 + a >= end) break;
-            fetch(wv[a], B, n0 + r, s0 + a);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) fetch(xv[a][t], A, t * 16 + r, s0 + a);
-        }
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            if (s0 + a >= end) break;
-            frag wf[PARTS];
-            parts(wf, wv[a]);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                frag xf[PARTS];
-                parts(xf, xv[a][t]);
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                    for (int q = 0; q < PARTS; ++q)
-                        if (p + q < 3) {
-                            if constexpr (__is_same(T, f16)) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[p], wf[q], acc[t], 0, 0, 0);
-                            else acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[p], wf[q], acc[t], 0, 0, 0);
-                        }
-            }
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) lds[wave][t * 16 + 4 * (lane >> 4) + e][r] = acc[t][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * 256; i += 64 * WAVES) {
-        const int64_t m = i >> 4, n = n0 + (i & 15);
-        if (m >= M || n >= N) continue;
-        float v[1] = {0.f}, bias[1] = {0.f};
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) v[0] += lds[w][m][i & 15];
-        if (ep.bias) bias[0] = (float)reinterpret_cast<const T*>(ep.bias)[n];
-        papr_pack<T, 1> res;
-        if (ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
-        finish<T, OUT_FORWARD, 1>(v, m, n, N, bias, res, ep);
-    }
-}
-
-// Up to here the few-rows kernel is the faster one: 1 x 1024 -> 4096 bf16 3.8 us against 10.1 of 64 x 64 tiles, 32 x 4096 -> 1024 26.8 against 29.6, 64 x 4096 -> 1024 48 against 30.
-constexpr int FEW_ROWS = 32;
-
-template <typename T>
-int launch_few_rows(const Operand& A, const Operand& B, int64_t K, bool vec, const Epilogue& ep, hipStream_t s) {
-    // (sixteen waves where there are fewer workgroups than compute units and steps enough: 16 x 4096 -> 1024 in bf16 16.6 us with eight)
-    const dim3 grid((unsigned)((B.rows + 15) / 16));
-    const bool many = B.rows <= 16 * papr_cu_count() / 2 && K >= 1024;
-    if (A.rows <= 16) {
-        if (many) few_rows_kernel<T, 1, 16><<<grid, 1024, 0, s>>>(A, B, K, vec, ep);
-        else few_rows_kernel<T, 1, 8><<<grid, 512, 0, s>>>(A, B, K, vec, ep);
-    } else {
-        if (many) few_rows_kernel<T, 2, 16><<<grid, 1024, 0, s>>>(A, B, K, vec, ep);
-        else few_rows_kernel<T, 2, 8><<<grid, 512, 0, s>>>(A, B, K, vec, ep);
-    }
-    PAPR_CHECK_LAUNCH("papr_linear_fwd");
-    return 0;
-}
-
-// The slabs of a sum in parts: a workgroup takes 64 results, its four waves a quarter of the parts each, quarters added in order.
-template <typename T>
-__global__ __launch_bounds__(256) void join_slabs_kernel(const float* __restrict__ slab, int64_t n, int parts, T* __restrict__ out) {
-    __shared__ float lds[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (parts + 3) / 4;
-    for (int64_t i0 = (int64_t)blockIdx.x * 64; i0 < n; i0 += (int64_t)gridDim.x * 64) {
-        const int64_t i = i0 + lane < n ? i0 + lane : n - 1;
-        const int end = (wave + 1) * per < parts ? (wave + 1) * per : parts;
-        float s = 0.f;
-#pragma unroll 8
-        for (int k = wave * per; k < end; ++k) s += slab[k * n + i];
-        lds[wave][lane] = s;
-        __syncthreads();
-        if (wave == 0 && i0 + lane < n) out[i] = (T)((lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]));
-        __syncthreads();
-    }
-}
-
-// d_z = d_y act'(z) in the rows' type (none: d_y as it is, nothing is written) and the column sums of it in float32, one partial row per workgroup.
-// A thread holds PIECE columns; the threads of a workgroup beyond one row's take further rows.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, int64_t ld, const T* __restrict__ z, int64_t M, int N, int act, int lanes, T* __restrict__ d_z,
-                                                    float* __restrict__ part, int64_t rows_per_block) {
-    constexpr int V = VEC ? 16 / sizeof(T) : 1;
-    __shared__ float fold[256 * V];
-    const int per = 256 / lanes, cg = threadIdx.x % lanes, rl = threadIdx.x / lanes;
-    const int c = (blockIdx.y * lanes + cg) * V;
-    const int64_t beg = (int64_t)blockIdx.x * rows_per_block, end = beg + rows_per_block < M ? beg + rows_per_block : M;
-    float sum[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = 0.f;
-    if (c < N)
-#pragma unroll 4
-        for (int64_t m = beg + rl; m < end; m += per) {
-            auto g = *reinterpret_cast<const papr_pack<T, V>*>(d_y + m * ld + c);
-            if (d_z) {
-                const auto t = *reinterpret_cast<const papr_pack<T, V>*>(z + m * N + c);
-                float v[V], zv[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) { v[i] = (float)g.v[i]; zv[i] = (float)t.v[i]; }
-                act_slopes<sizeof(T) == 4>(v, zv, act);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    sum[i] += v[i];
-                    g.v[i] = (T)v[i];
-                }
-                *reinterpret_cast<papr_pack<T, V>*>(d_z + m * N + c) = g;
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) sum[i] += (float)g.v[i];
-            }
-        }
-    if (!part) return;
-#pragma unroll
-    for (int i = 0; i < V; ++i) fold[threadIdx.x * V + i] = sum[i];
-    __syncthreads();
-    for (int q = threadIdx.x; q < lanes * V; q += 256) {
-        const int col = blockIdx.y * lanes * V + q;
-        float s = 0.f;
-        for (int k = 0; k < per; ++k) s += fold[k * lanes * V + q];
-        if (col < N) part[(int64_t)blockIdx.x * N + col] = s;
-    }
-}
-
-typedef Shape<2, 4, 4, 2, 4> Large;                // 256 x 256, eight waves
-typedef Shape<2, 2, 4, 2, 3> Wide;                 // 256 x 128, four waves
-typedef Shape<2, 2, 2, 2, 4> Middle;               // 128 x 128, four waves
-typedef Shape<2, 2, 1, 1, 4> Small;                // 64 x 64, four waves
-
-// Which tile shape, and into how many parts the sum is cut: the least estimated time.  A compute unit gets q = ceil(tiles x parts / compute units) tiles; a tile costs
-// its 64-term steps and a fixed part (filling the pipeline, writing the results), both measured per shape with the unit's resident workgroups sharing it; fewer
-// tiles than that leave a unit waiting more (`lone`: a single tile against a full unit).  Parts cost their slabs' way to memory and back and one more launch.
-//   streaming 16-bit (8192 x 4096 x 1024 and 65,536 x 1024 x 1024):  256 x 256 1.5 us a step, 256 x 128 0.87, 128 x 128 0.55, 64 x 64 0.24
-//   16-bit through registers (8191 x 1001 x 1003, 8-bit rows):                          3.5         4.0             1.6          0.55
-//   float32 (512,000 x 256 x 256, 25,600 x 256 x 142):                                  11          6               3.2          1.3
-enum { PATH_STREAM, PATH_REGISTERS, PATH_F32 };
-struct Choice { int shape; int64_t parts, per; };      // per: terms of a part
-Choice choose(int64_t M, int64_t N, int64_t K, int path, bool may_split) {
-    static const int rows[4] = {256, 256, 128, 64}, cols[4] = {256, 128, 128, 64}, resident[4] = {1, 2, 2, 4};
-    static const double step_us[3][4] = {{1.5, 0.87, 0.55, 0.24}, {3.5, 4.0, 1.6, 0.55}, {11.0, 6.0, 3.2, 1.3}};
-    static const double fixed_us[4] = {9.0, 5.0, 2.5, 1.0};
-    static const double lone[3][4] = {{1.0, 1.4, 1.2, 2.0}, {1.0, 1.4, 1.8, 1.5}, {1.0, 1.6, 1.4, 1.0}};
-    const int64_t cus = papr_cu_count(), steps = (K + 63) / 64;
-    Choice best = {0, 1, 0};
-    double least = 0;
-    for (int s = 0; s < 4; ++s) {
-        const int64_t tiles = ((M + rows[s] - 1) / rows[s]) * ((N + cols[s] - 1) / cols[s]);
-        const int64_t tried[4] = {1, cus / tiles, 2 * cus / tiles, 4 * cus / tiles};
-        for (int64_t parts : tried) {
-            if (parts > 1 && !may_split) continue;
-            if (parts > steps / 2) parts = steps / 2;
-            if (parts > 1024) parts = 1024;
-            if (parts < 1) parts = 1;
-            const int64_t per = (steps + parts - 1) / parts;
-            parts = (steps + per - 1) / per;
-            const int64_t q = (tiles * parts + cus - 1) / cus;
-            const double share = q < resident[s] ? 1 + (lone[path][s] - 1) * (double)(resident[s] - q) / (resident[s] > 1 ? resident[s] - 1 : 1) : 1;
-            double t = (double)q * (step_us[path][s] * per * share + fixed_us[s]);
-            if (parts > 1) t += (double)parts * M * N * 8 / 5e6 + 4;
-            if (least == 0 || t < least) { least = t; best = {s, parts, per * 64}; }
-        }
-    }
-    return best;
-}
-int path_of(int type, bool vec, int keep) { return type == PAPR_TYPE_F32 ? PATH_F32 : vec && !keep ? PATH_STREAM : PATH_REGISTERS; }
-
-template <auto KERNEL, size_t LDS, typename S>
-int launch_kernel(const Operand& A, const Operand& B, int64_t K, const Choice& c, const Epilogue& ep, hipStream_t s) {
-    static_assert(LDS <= 160 * 1024, "a compute unit's LDS");
-    const int64_t tm = (A.rows + S::TM - 1) / S::TM, tn = (B.rows + S::TN - 1) / S::TN, grid = tm * tn * c.parts;
-    PAPR_REQUIRE(grid < (int64_t)1 << 31, "papr_linear: %lld tiles", (long long)grid);
-    if (LDS > 65536) {
-        static std::atomic<uint64_t> ready{0};        // (devices on which this kernel may already use more than 64 KB of LDS)
-        int dev = 0;
-        (void)hipGetDevice(&dev);
-        const uint64_t bit = 1ull << (dev & 63);
-        if (dev > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
-            (void)hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
-            ready.fetch_or(bit, std::memory_order_relaxed);
-        }
-    }
-    KERNEL<<<dim3((unsigned)grid), dim3(S::THREADS), LDS, s>>>(A, B, K, c.per, (unsigned)tm, (unsigned)tn, ep);
-    PAPR_CHECK_LAUNCH("papr_linear product");
-    return 0;
-}
-
-template <typename T, int LA, int LB, int FMT, bool VEC, int OUT, typename S>
-int launch_shape(const Operand& A, const Operand& B, int64_t K, const Choice& c, const Epilogue& ep, hipStream_t s) {
-    if constexpr (sizeof(T) == 2 && FMT == 0 && VEC && S::TM >= 128)
-        return launch_kernel<stream_kernel<T, LA, LB, OUT, S>, Stream<T, LA, LB, S>::LDS, S>(A, B, K, c, ep, s);
-    else
-        return launch_kernel<product_kernel<T, LA, LB, FMT, VEC, OUT, S>, Plan<T, LA, LB, FMT, VEC, S>::LDS, S>(A, B, K, c, ep, s);
-}
-
-template <typename T, int LA, int LB, int FMT, bool VEC, int OUT>
-int launch_choice(const Choice& c, const Operand& A, const Operand& B, int64_t K, const Epilogue& ep, hipStream_t s) {
-    switch (c.shape) {
-        case 0: return launch_shape<T, LA, LB, FMT, VEC, OUT, Large>(A, B, K, c, ep, s);
-        case 1: return launch_shape<T, LA, LB, FMT, VEC, OUT, Wide>(A, B, K, c, ep, s);
-        case 2: return launch_shape<T, LA, LB, FMT, VEC, OUT, Middle>(A, B, K, c, ep, s);
-        default: return launch_shape<T, LA, LB, FMT, VEC, OUT, Small>(A, B, K, c, ep, s);
-    }
-}
-template <typename T, int LA, int LB, int FMT, int OUT>
-int launch_product(const Choice& c, bool vec, const Operand& A, const Operand& B, int64_t K, const Epilogue& ep, hipStream_t s) {
-    return vec ? launch_choice<T, LA, LB, FMT, true, OUT>(c, A, B, K, ep, s) : launch_choice<T, LA, LB, FMT, false, OUT>(c, A, B, K, ep, s);
-}
-
-// C = A B^T into contiguous rows of type T, the sum in parts where the tiles alone do not fill the chip
-template <typename T, int LA, int LB, int FMT>
-int rows_product(bool vec, const Operand& A, const Operand& B, int64_t K, void* out, float* slab, hipStream_t s) {
-    const Choice c = choose(A.rows, B.rows, K, path_of(sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, vec, FMT), true);
-    Epilogue ep = {};
-    if (c.parts == 1) {
-        ep.out = out;
-        ep.wide = ((uintptr_t)out & 15) == 0 && (B.rows * sizeof(T)) % 16 == 0;
-        return launch_product<T, LA, LB, FMT, OUT_ROWS>(c, vec, A, B, K, ep, s);
-    }
-    ep.out = slab;
-    if (int rc = launch_product<T, LA, LB, FMT, OUT_SLAB>(c, vec, A, B, K, ep, s)) return rc;
-    const int64_t n = A.rows * B.rows, need = (n + 63) / 64, cap = (int64_t)papr_cu_count() * 16;
-    join_slabs_kernel<T><<<dim3((unsigned)(need < cap ? need : cap)), dim3(256), 0, s>>>(slab, n, (int)c.parts, (T*)out);
-    PAPR_CHECK_LAUNCH("papr_linear slabs");
-    return 0;
-}
 
 // float32 slabs of one product
 size_t slab_floats(int type, int64_t M, int64_t N, int64_t K) {
     size_t most = 0;                                  // (the path, and with it the choice, depends on alignments that the workspace's size does not know)
-    for (int path = type == PAPR_TYPE_F32 ? PATH_F32 : PATH_STREAM; path <= (type == PAPR_TYPE_F32 ? PATH_F32 : PATH_REGISTERS); ++path) {
+    for (int path = 0; path < PATHS; ++path) {
+        if ((type == PAPR_TYPE_F32) != (path == PATH_F32 || path == PATH_F32_ODD)) continue;
         const int64_t parts = choose(M, N, K, path, true).parts;
         if (parts > 1 && (size_t)(parts * M * N) > most) most = (size_t)(parts * M * N);
     }
     return most;
 }
 
-struct SlopeGrid { int lanes; int64_t blocks, rows_per_block; unsigned cols; };
 SlopeGrid slope_grid(int64_t M, int N, int piece) {
     SlopeGrid g;
     const int groups = (N + piece - 1) / piece;
@@ -903,6 +32,13 @@ SlopeGrid slope_grid(int64_t M, int N, int piece) {
 }
 
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+// d_z of 16-bit rows is rounded to their type in front of its two products, an error of the gradients' own rounding's size (together 1.4 times it).  Where the products
+// are over in a few microseconds whatever they multiply (2^28 terms: 5 us at a fifth of the matrix pipe's rate) that is not paid for: d_z stays in float32 and the
+// products take it as the sum of two 16-bit values.  (none and relu: d_z is d_y or zero and needs no rounding.)
+bool keeps_wide(const papr_linear_desc* d) {
+    return d->type != PAPR_TYPE_F32 && d->act != PAPR_ACT_NONE && d->act != PAPR_ACT_RELU && (double)d->M * (double)d->N * (double)d->K <= 268435456.0;
+}
 
 int linear_check(const char* who, int type, int64_t M, int64_t N, int64_t K, int act) {
     PAPR_REQUIRE(papr_type_ok(type), "%s: unknown row type %d", who, type);
@@ -925,14 +61,12 @@ extern "C" int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t
     const Operand A = {x, ldx, d->M, nullptr}, B = {w, ldw, d->N, nullptr};
     const Epilogue ep = {y, bias, res, ld_res, z, d->act,
                          papr_rows_aligned(y, d->N, d->N, b) && (!z || ((uintptr_t)z & 15) == 0) && (!res || papr_rows_aligned(res, ld_res, d->N, b))};
-    if (d->M <= FEW_ROWS) PAPR_TYPE_SWITCH(d->type, return launch_few_rows<T>(A, B, d->K, vec, ep, as_stream(stream)));
-    const Choice c = choose(d->M, d->N, d->K, path_of(d->type, vec, 0), false);
-    PAPR_TYPE_SWITCH(d->type, return (launch_product<T, K_RUNS, K_RUNS, 0, OUT_FORWARD>(c, vec, A, B, d->K, ep, as_stream(stream))));
+    PAPR_TYPE_SWITCH(d->type, return forward<T>(A, B, d->K, vec, ep, as_stream(stream)));
 }
 
 extern "C" size_t papr_linear_bwd_workspace_bytes(const papr_linear_desc* d) {
     if (!d || d->M <= 0 || d->N <= 0 || d->K <= 0 || !papr_type_ok(d->type)) return 0;
-    const size_t dz = d->act == PAPR_ACT_NONE ? 0 : up16((size_t)d->M * d->N * papr_type_bytes(d->type));
+    const size_t dz = d->act == PAPR_ACT_NONE ? 0 : up16((size_t)d->M * d->N * (keeps_wide(d) ? 4 : papr_type_bytes(d->type)));
     size_t part = 0;
     for (int piece = 1; piece <= 8; piece *= 2) {
         const size_t p = (size_t)slope_grid(d->M, (int)d->N, piece).blocks * d->N * sizeof(float);
@@ -954,20 +88,17 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
     PAPR_REQUIRE(!d_x || w, "papr_linear_bwd: d_x needs the weight");
     PAPR_REQUIRE(!d_w || (x && (!d->keep || exps)), "papr_linear_bwd: d_w needs the rows");
     const int b = papr_type_bytes(d->type);
-    const bool slope = d->act != PAPR_ACT_NONE;
+    const bool slope = d->act != PAPR_ACT_NONE, wide = keeps_wide(d);
     char* ws = reinterpret_cast<char*>(workspace);
     void* dz = slope ? ws : nullptr;
-    if (slope) ws += up16((size_t)M * N * b);
+    if (slope) ws += up16((size_t)M * N * (wide ? 4 : b));
     float* part = reinterpret_cast<float*>(ws);
     if (slope || d_b) {
         const bool vec = papr_rows_aligned(d_y, ld_dy, N, b) && ((uintptr_t)z & 15) == 0;
         const SlopeGrid g = slope_grid(M, (int)N, vec ? 16 / b : 1);
-        const dim3 grid((unsigned)g.blocks, g.cols);
-        PAPR_TYPE_SWITCH(d->type, {
-            if (vec) slope_kernel<T, true><<<grid, 256, 0, s>>>((const T*)d_y, ld_dy, (const T*)z, M, (int)N, d->act, g.lanes, (T*)dz, d_b ? part : nullptr, g.rows_per_block);
-            else slope_kernel<T, false><<<grid, 256, 0, s>>>((const T*)d_y, ld_dy, (const T*)z, M, (int)N, d->act, g.lanes, (T*)dz, d_b ? part : nullptr, g.rows_per_block);
-        });
-        PAPR_CHECK_LAUNCH("papr_linear_bwd");
+        int rc = 0;
+        PAPR_TYPE_SWITCH(d->type, rc = slopes<T>(wide, vec, g, d_y, ld_dy, z, M, (int)N, d->act, dz, d_b ? part : nullptr, s));
+        if (rc) return rc;
         if (d_b) {
             papr_colsum_out out = {};
             out.p[0] = d_b;
@@ -983,23 +114,19 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
     float* slab = reinterpret_cast<float*>(ws + up16(most));
     const void* g = slope ? dz : d_y;
     const int64_t ldg = slope ? N : ld_dy;
-    const bool vg = papr_rows_aligned(g, ldg, N, b);
+    const bool vg = papr_rows_aligned(g, ldg, N, wide ? 4 : b);
     if (d_x) {
         const Operand A = {g, ldg, M, nullptr}, B = {w, ldw, K, nullptr};
         const bool vec = vg && papr_rows_aligned(w, ldw, K, b);
         int rc = 0;
-        PAPR_TYPE_SWITCH(d->type, rc = (rows_product<T, K_RUNS, ROWS_RUN, 0>(vec, A, B, N, d_x, slab, s)));
+        PAPR_TYPE_SWITCH(d->type, rc = grad_rows<T>(wide, vec, A, B, N, d_x, slab, s));
         if (rc) return rc;
     }
     if (d_w) {
         const Operand A = {g, ldg, N, nullptr}, B = {x, ldx, K, (const uint8_t*)exps};
         const bool vec = vg && (d->keep || papr_rows_aligned(x, ldx, K, b));
         int rc = 0;
-        PAPR_TYPE_SWITCH(d->type, {
-            if (d->keep == PAPR_KEEP_E4M3) rc = rows_product<T, ROWS_RUN, ROWS_RUN, PAPR_KEEP_E4M3>(vec, A, B, M, d_w, slab, s);
-            else if (d->keep == PAPR_KEEP_INT8) rc = rows_product<T, ROWS_RUN, ROWS_RUN, PAPR_KEEP_INT8>(vec, A, B, M, d_w, slab, s);
-            else rc = rows_product<T, ROWS_RUN, ROWS_RUN, 0>(vec, A, B, M, d_w, slab, s);
-        });
+        PAPR_TYPE_SWITCH(d->type, rc = grad_weight<T>(wide, d->keep, vec, A, B, M, d_w, slab, s));
         if (rc) return rc;
     }
     return 0;
