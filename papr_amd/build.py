@@ -142,6 +142,28 @@ def build_library(force=False, verbose=True):
     return LIB
 
 
+GLUE = os.path.join(PKG, "_blocks.so")
+
+
+def build_glue(force=False, verbose=True):
+    """papr_amd/_blocks.so: the native host side of papr_amd/blocks.py (host code only, against the installed torch's headers)."""
+    import sysconfig
+    import torch
+    src = os.path.join(CSRC, "blocks_glue.cpp")
+    if not (force or _stale(GLUE, [src, os.path.join(os.path.dirname(PKG), "include", "papr_hip.h")])):
+        return GLUE
+    root = os.path.dirname(torch.__file__)
+    inc = os.path.join(root, "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM=1", "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], "-I/opt/rocm/include", src, "-o", GLUE,
+           "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return GLUE
+
+
 if __name__ == "__main__":
+    build_glue(force="--force" in sys.argv)
     build_library(force="--force" in sys.argv)
     print(LIB)
