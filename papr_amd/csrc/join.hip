@@ -470,18 +470,18 @@ __global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ 
     const int64_t step = (int64_t)n_arrays * width, per = (n_blocks + 15) / 16;
     int64_t b = wave * per, end = b + per < n_blocks ? b + per : n_blocks;
     const float* p = part + (int64_t)a * width + (c < width ? c : 0);
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-    for (; b + 4 <= end; b += 4) {
-        s0 += p[b * step]; s1 += p[(b + 1) * step]; s2 += p[(b + 2) * step]; s3 += p[(b + 3) * step];
-    }
-    for (; b < end; ++b) s0 += p[b * step];
-    lds[wave][lane] = (s0 + s1) + (s2 + s3);
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (; b + 8 <= end; b += 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] += p[(b + i) * step];
+    for (; b < end; ++b) s[0] += p[b * step];
+    lds[wave][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (wave == 0 && c < width) {
-        float s = 0.f;
+        float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) s += lds[w][lane];
-        store_param(out.p[a], out.type[a], c, s);
+        for (int w = 0; w < 16; ++w) sum += lds[w][lane];
+        store_param(out.p[a], out.type[a], c, sum);
     }
 }
 

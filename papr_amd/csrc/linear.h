@@ -18,14 +18,15 @@ struct Epilogue {                                  // out and z (M, N) contiguou
 //                                                                                              256 x 256      128 x 128      64 x 64
 //   streaming 16-bit (8192 x 4096 x 1024 and 65,536 x 1024 x 1024), us a step                    1.5            0.55          0.24
 //   16-bit through registers (8191 x 1001 x 1003, 8-bit rows)                                    (slower)       1.6           0.55
-//   float32 (512,000 x 256 x 256, 25,600 x 256 x 142)                                            11             3.2           1.3
+//   float32 (512,000 x 256 x 256, 8192 x 4096 x 1024; 8-bit rows 1.8 / 0.9)                      10.6           2.9           1.1
 //   float32 d_z of a 16-bit layer                                                                                             0.8
-enum { PATH_STREAM, PATH_REGISTERS, PATH_F32, PATH_F32_ODD, PATH_WIDE, PATHS };
+enum { PATH_STREAM, PATH_REGISTERS, PATH_F32, PATH_F32_ODD, PATH_F32_KEPT, PATH_WIDE, PATHS };
 struct Choice { int shape; int64_t parts, per; };      // per: terms of a part
 inline Choice choose(int64_t M, int64_t N, int64_t K, int path, bool may_split) {
-    static const int side[3] = {256, 128, 64}, resident[3] = {1, 2, 4}, first[PATHS] = {0, 1, 0, 1, 2};
-    static const double step_us[PATHS][3] = {{1.5, 0.55, 0.24}, {0, 1.6, 0.55}, {11.0, 3.2, 1.3}, {0, 3.2, 1.3}, {0, 0, 0.8}};
-    static const double fixed_us[3] = {9.0, 2.5, 1.0}, lone[PATHS][3] = {{1.0, 1.2, 2.0}, {1.0, 1.8, 1.5}, {1.0, 1.4, 1.0}, {1.0, 1.4, 1.0}, {1.0, 1.0, 1.2}};
+    static const int side[3] = {256, 128, 64}, resident[3] = {1, 2, 4}, first[PATHS] = {0, 1, 0, 1, 1, 2};
+    static const double step_us[PATHS][3] = {{1.5, 0.55, 0.24}, {0, 1.6, 0.55}, {10.6, 2.9, 1.1}, {0, 2.9, 1.1}, {0, 1.8, 0.9}, {0, 0, 0.8}};
+    static const double fixed_us[3] = {9.0, 2.5, 1.5};
+    static const double lone[PATHS][3] = {{1.0, 1.2, 2.0}, {1.0, 1.8, 1.5}, {1.0, 1.5, 1.4}, {1.0, 1.5, 1.4}, {1.0, 1.5, 1.9}, {1.0, 1.0, 1.2}};
     const int64_t cus = papr_cu_count(), steps = (K + 63) / 64;
     Choice best = {0, 1, 0};
     double least = 0;
@@ -42,14 +43,14 @@ inline Choice choose(int64_t M, int64_t N, int64_t K, int path, bool may_split) 
             const int64_t q = (tiles * parts + cus - 1) / cus;
             const double share = q < resident[s] ? 1 + (lone[path][s] - 1) * (double)(resident[s] - q) / (resident[s] - 1) : 1;
             double t = (double)q * (step_us[path][s] * per * share + fixed_us[s]);
-            if (parts > 1) t += (double)parts * M * N * 8 / 5e6 + 4;
+            if (parts > 1) t += (double)parts * M * N * 8 / 5e6 + 3;
             if (least == 0 || t < least) { least = t; best = {s, parts, per * 64}; }
         }
     }
     return best;
 }
 inline int path_of(int type, bool vec, int keep, bool wide) {
-    if (type == PAPR_TYPE_F32) return vec && !keep ? PATH_F32 : PATH_F32_ODD;
+    if (type == PAPR_TYPE_F32) return keep ? PATH_F32_KEPT : vec ? PATH_F32 : PATH_F32_ODD;
     return wide ? PATH_WIDE : vec && !keep ? PATH_STREAM : PATH_REGISTERS;
 }
 

@@ -9,7 +9,7 @@ namespace {
 size_t slab_floats(int type, int64_t M, int64_t N, int64_t K) {
     size_t most = 0;                                  // (the path, and with it the choice, depends on alignments that the workspace's size does not know)
     for (int path = 0; path < PATHS; ++path) {
-        if ((type == PAPR_TYPE_F32) != (path == PATH_F32 || path == PATH_F32_ODD)) continue;
+        if ((type == PAPR_TYPE_F32) != (path == PATH_F32 || path == PATH_F32_ODD || path == PATH_F32_KEPT)) continue;
         const int64_t parts = choose(M, N, K, path, true).parts;
         if (parts > 1 && (size_t)(parts * M * N) > most) most = (size_t)(parts * M * N);
     }
@@ -23,7 +23,7 @@ SlopeGrid slope_grid(int64_t M, int N, int piece) {
     while (g.lanes < groups && g.lanes < 256) g.lanes *= 2;
     g.cols = (unsigned)((groups + g.lanes - 1) / g.lanes);
     const int64_t per = 256 / g.lanes;
-    int64_t blocks = (M + 8 * per - 1) / (8 * per), cap = (int64_t)papr_cu_count() * 8 / g.cols;
+    int64_t blocks = (M + 8 * per - 1) / (8 * per), cap = (int64_t)papr_cu_count() * 4 / g.cols;
     if (cap < 1) cap = 1;
     if (blocks > cap) blocks = cap;
     g.rows_per_block = (M + blocks - 1) / blocks;

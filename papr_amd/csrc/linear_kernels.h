@@ -118,9 +118,8 @@ struct Tile {
     static_assert(R * BK % (PIECE * THREADS) == 0, "whole pieces per thread");
     typedef typename Matrix<T>::frag frag;
 
-    uint4 reg[N];
+    struct Held { uint4 reg[N]; uint8_t ex[PACKED ? N : 1]; };                    // a tile on its way
     unsigned off[N];                                                              // bytes from the tile's address
-    uint8_t ex[PACKED ? N : 1];
     unsigned exo[PACKED ? N : 1];
     const char* base;                                                             // (uniform) rows r0, the next k
     const uint8_t* exb;
@@ -154,7 +153,7 @@ struct Tile {
     }
     // the next tile: k0 .. k0 + BK of K terms.  `inside`: every piece may be read whole.  A piece that crosses the end of a contiguous row of rows reads the start
     // of the next one (those rows of the product are never stored), but behind the last k there is no next one.
-    __device__ __forceinline__ void load(const Operand& o, int64_t r0, int64_t k0, int64_t K) {
+    __device__ __forceinline__ void load(Held& h, const Operand& o, int64_t r0, int64_t k0, int64_t K) {
         bool inside = k0 + BK <= K;
         if (LAYOUT == ROWS_RUN && !VEC && !PACKED) inside = k0 + BK < K && o.rows >= PIECE;
         if (inside) {
@@ -163,10 +162,10 @@ struct Tile {
                 const char* src = base + off[q];
                 if (PACKED) {
                     const uint2 c = *reinterpret_cast<const uint2*>(src);
-                    reg[q].x = c.x; reg[q].y = c.y;
-                    ex[q] = exb[exo[q]];
-                } else if (VEC) reg[q] = *reinterpret_cast<const uint4*>(src);
-                else __builtin_memcpy(&reg[q], __builtin_assume_aligned(src, sizeof(Source)), 16);
+                    h.reg[q].x = c.x; h.reg[q].y = c.y;
+                    h.ex[q] = exb[exo[q]];
+                } else if (VEC) h.reg[q] = *reinterpret_cast<const uint4*>(src);
+                else __builtin_memcpy(&h.reg[q], __builtin_assume_aligned(src, sizeof(Source)), 16);
             }
         } else {
 #pragma unroll
@@ -177,11 +176,11 @@ struct Tile {
                 const char* src = in ? base + off[q] : base;                      // (base: rows r0, the tile's first k < K)
                 if (PACKED) {
                     const uint2 c = *reinterpret_cast<const uint2*>(src);
-                    reg[q].x = in ? c.x : 0u; reg[q].y = in ? c.y : 0u;
-                    ex[q] = exb[in ? exo[q] : 0u];
+                    h.reg[q].x = in ? c.x : 0u; h.reg[q].y = in ? c.y : 0u;
+                    h.ex[q] = exb[in ? exo[q] : 0u];
                 } else if (VEC) {
                     const uint4 t = *reinterpret_cast<const uint4*>(src);
-                    reg[q].x = in ? t.x : 0u; reg[q].y = in ? t.y : 0u; reg[q].z = in ? t.z : 0u; reg[q].w = in ? t.w : 0u;
+                    h.reg[q].x = in ? t.x : 0u; h.reg[q].y = in ? t.y : 0u; h.reg[q].z = in ? t.z : 0u; h.reg[q].w = in ? t.w : 0u;
                 } else {
                     papr_pack<Source, PIECE> t;
                     if (LAYOUT == ROWS_RUN && r0 + r >= o.rows) r = 0;
@@ -190,7 +189,7 @@ struct Tile {
                         const bool ok = LAYOUT == K_RUNS ? k0 + k + i < K : in && r0 + r + i < o.rows;
                         t.v[i] = ok ? reinterpret_cast<const Source*>(src)[i] : (Source)0.f;
                     }
-                    __builtin_memcpy(&reg[q], &t, 16);
+                    __builtin_memcpy(&h.reg[q], &t, 16);
                 }
             }
         }
@@ -198,7 +197,7 @@ struct Tile {
         if (PACKED) exb += BK * (ld >> 5);
     }
 
-    __device__ __forceinline__ void store(short* lds) const {
+    __device__ __forceinline__ void store(const Held& h, short* lds) const {
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             int r, k;
@@ -206,15 +205,15 @@ struct Tile {
             const int at = LAYOUT == K_RUNS ? place(r, k >> 3) + (k & 7) : k * STRIDE + r;
             if constexpr (PACKED) {
                 float v[4], w[4];
-                const float scale = __uint_as_float((unsigned)ex[q] << 23);
-                papr_codes_to_float<FMT>(reg[q].x, scale, v);
-                papr_codes_to_float<FMT>(reg[q].y, scale, w);
-                frag h;
+                const float scale = __uint_as_float((unsigned)h.ex[q] << 23);
+                papr_codes_to_float<FMT>(h.reg[q].x, scale, v);
+                papr_codes_to_float<FMT>(h.reg[q].y, scale, w);
+                frag to;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { h[i] = v[i]; h[4 + i] = w[i]; }     // (exact: at most 8 significant bits)
-                *reinterpret_cast<frag*>(lds + at) = h;
+                for (int i = 0; i < 4; ++i) { to[i] = v[i]; to[4 + i] = w[i]; }     // (exact: at most 8 significant bits)
+                *reinterpret_cast<frag*>(lds + at) = to;
             } else if (SPLIT) {
-                const float f[4] = {__uint_as_float(reg[q].x), __uint_as_float(reg[q].y), __uint_as_float(reg[q].z), __uint_as_float(reg[q].w)};
+                const float f[4] = {__uint_as_float(h.reg[q].x), __uint_as_float(h.reg[q].y), __uint_as_float(h.reg[q].z), __uint_as_float(h.reg[q].w)};
                 papr_pack<Part, 4> p[PLANES];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -227,7 +226,7 @@ struct Tile {
                 }
 #pragma unroll
                 for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<Part, 4>*>(lds + n * PLANE + at) = p[n];
-            } else *reinterpret_cast<uint4*>(lds + at) = reg[q];
+            } else *reinterpret_cast<uint4*>(lds + at) = h.reg[q];
         }
     }
 
@@ -272,11 +271,11 @@ struct Shape {
 
 template <typename T, int LA, int LB, int FA, int FMT, bool VEC, typename S>
 struct Plan {
-    static constexpr int BK = sizeof(T) == 2 ? 64 : S::TM > 64 ? 16 : 32;       // (divides step_of)
+    static constexpr int BK = sizeof(T) == 2 ? 64 : 32, BUFFERS = sizeof(T) == 4 && S::TM > 64 ? 1 : 2;
     typedef Tile<T, LA, FA, VEC, S::TM, BK, S::THREADS> TA;
     typedef Tile<T, LB, FMT, VEC, S::TN, BK, S::THREADS> TB;
     static constexpr int BUF = TA::HALFS + TB::HALFS;
-    static constexpr size_t LOOP = (size_t)2 * BUF * 2, LDS = S::EPI > LOOP ? S::EPI : LOOP;
+    static constexpr size_t LOOP = (size_t)BUFFERS * BUF * 2, LDS = S::EPI > LOOP ? S::EPI : LOOP;
 };
 
 // E consecutive results of row m from column n on
@@ -404,18 +403,21 @@ __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Opera
     TB b;
     a.start(A, m0, kb);
     b.start(B, n0, kb);
-    a.load(A, m0, kb, K);
-    b.load(B, n0, kb, K);
-    a.store(smem);
-    b.store(smem + TA::HALFS);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t k0 = kb; k0 < ke; k0 += BK, buf ^= 1) {
-        const bool more = k0 + BK < ke;
-        if (more) {
-            a.load(A, m0, k0 + BK, K);
-            b.load(B, n0, k0 + BK, K);
-        }
+    // The next tile is on its way in registers while one is multiplied.  float32 (three parts of every value: three times the LDS and six times the matrix instructions of
+    // a step) has one buffer and two barriers a step of 32 terms instead of two buffers of 16: half as many steps shorter than the way to memory.
+    typename TA::Held ha;
+    typename TB::Held hb;
+    auto load = [&](int64_t k) __attribute__((always_inline)) {
+        if (k >= ke) return;
+        a.load(ha, A, m0, k, K);
+        b.load(hb, B, n0, k, K);
+    };
+    auto store = [&](int64_t k, int buf) __attribute__((always_inline)) {
+        if (k >= ke) return;
+        a.store(ha, smem + buf * P::BUF);
+        b.store(hb, smem + buf * P::BUF + TA::HALFS);
+    };
+    auto multiply = [&](int buf) __attribute__((always_inline)) {
         const short *la = smem + buf * P::BUF, *lb = la + TA::HALFS;
 #pragma unroll
         for (int ks = 0; ks < BK / 16; ++ks) {
@@ -439,11 +441,26 @@ __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Opera
 #pragma unroll
                             for (int j = 0; j < IN; ++j) acc[i][j] = mfma(fa[p][i], fb[q][j], acc[i][j]);
         }
-        if (more) {
-            a.store(smem + (buf ^ 1) * P::BUF);
-            b.store(smem + (buf ^ 1) * P::BUF + TA::HALFS);
+    };
+    load(kb);
+    if constexpr (P::BUFFERS == 1) {
+        for (int64_t k = kb; k < ke; k += BK) {
+            store(k, 0);
+            __syncthreads();
+            load(k + BK);
+            multiply(0);
+            __syncthreads();
         }
+    } else {
+        store(kb, 0);
         __syncthreads();
+        int buf = 0;
+        for (int64_t k = kb; k < ke; k += BK, buf ^= 1) {
+            load(k + BK);
+            multiply(buf);
+            store(k + BK, buf ^ 1);
+            __syncthreads();
+        }
     }
     write_tile<T, OUT, S>(acc, smem, m0, n0, A.rows, B.rows, at.part, ep);
 }
@@ -710,22 +727,56 @@ int launch_few_rows(const Operand& A, const Operand& B, int64_t K, bool vec, con
     return 0;
 }
 
-// The slabs of a sum in parts: a workgroup takes 64 results, its four waves a quarter of the parts each, quarters added in order.
-template <typename T>
+// The slabs of a sum in parts, V results a lane.  SPREAD: the four waves of a workgroup take a quarter of the parts each (many parts: their loads are a chain), quarters
+// added in order; otherwise a lane adds all parts of its results.
+template <typename T, int V, bool SPREAD>
 __global__ __launch_bounds__(256) void join_slabs_kernel(const float* __restrict__ slab, int64_t n, int parts, T* __restrict__ out) {
-    __shared__ float lds[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (parts + 3) / 4;
-    for (int64_t i0 = (int64_t)blockIdx.x * 64; i0 < n; i0 += (int64_t)gridDim.x * 64) {
-        const int64_t i = i0 + lane < n ? i0 + lane : n - 1;
-        const int end = (wave + 1) * per < parts ? (wave + 1) * per : parts;
-        float s = 0.f;
+    __shared__ float lds[SPREAD ? 4 : 1][SPREAD ? 64 * V : 1];
+    const int lane = SPREAD ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6, per = SPREAD ? (parts + 3) / 4 : parts;
+    constexpr int SPAN = (SPREAD ? 64 : 256) * V;
+    const int beg = SPREAD ? wave * per : 0, end = beg + per < parts ? beg + per : parts;
+    for (int64_t i0 = (int64_t)blockIdx.x * SPAN; i0 < n; i0 += (int64_t)gridDim.x * SPAN) {
+        const int64_t at = i0 + lane * V, i = at < n ? at : 0;
+        papr_pack<float, V> s;
+#pragma unroll
+        for (int v = 0; v < V; ++v) s.v[v] = 0.f;
 #pragma unroll 8
-        for (int k = wave * per; k < end; ++k) s += slab[k * n + i];
-        lds[wave][lane] = s;
-        __syncthreads();
-        if (wave == 0 && i0 + lane < n) out[i] = (T)((lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane]));
-        __syncthreads();
+        for (int k = beg; k < end; ++k) {
+            const auto t = *reinterpret_cast<const papr_pack<float, V>*>(slab + k * n + i);
+#pragma unroll
+            for (int v = 0; v < V; ++v) s.v[v] += t.v[v];
+        }
+        if constexpr (SPREAD) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) lds[wave][lane * V + v] = s.v[v];
+            __syncthreads();
+            if (wave == 0)
+#pragma unroll
+                for (int v = 0; v < V; ++v) s.v[v] = (s.v[v] + lds[1][lane * V + v]) + (lds[2][lane * V + v] + lds[3][lane * V + v]);
+        }
+        if (at < n && (!SPREAD || wave == 0)) {
+            papr_pack<T, V> t;
+#pragma unroll
+            for (int v = 0; v < V; ++v) t.v[v] = (T)s.v[v];
+            *reinterpret_cast<papr_pack<T, V>*>(out + at) = t;
+        }
+        if constexpr (SPREAD) __syncthreads();
     }
+}
+template <typename T>
+int join_slabs(const float* slab, int64_t n, int parts, T* out, hipStream_t s) {
+    const bool spread = parts >= 16, wide = n % 4 == 0 && ((uintptr_t)out & 15) == 0;
+    const int64_t span = (spread ? 64 : 256) * (wide ? 4 : 1), need = (n + span - 1) / span, cap = (int64_t)papr_cu_count() * 16;
+    const dim3 grid((unsigned)(need < cap ? need : cap));
+    if (spread) {
+        if (wide) join_slabs_kernel<T, 4, true><<<grid, 256, 0, s>>>(slab, n, parts, out);
+        else join_slabs_kernel<T, 1, true><<<grid, 256, 0, s>>>(slab, n, parts, out);
+    } else {
+        if (wide) join_slabs_kernel<T, 4, false><<<grid, 256, 0, s>>>(slab, n, parts, out);
+        else join_slabs_kernel<T, 1, false><<<grid, 256, 0, s>>>(slab, n, parts, out);
+    }
+    PAPR_CHECK_LAUNCH("papr_linear slabs");
+    return 0;
 }
 
 // d_z = d_y act'(z) in the rows' type (none: d_y as it is, nothing is written) and the column sums of it in float32, one partial row per workgroup.
@@ -833,10 +884,7 @@ int rows_product(bool vec, const Operand& A, const Operand& B, int64_t K, void* 
     }
     ep.out = slab;
     if (int rc = launch_product<T, LA, LB, FA, FMT, OUT_SLAB>(c, vec, A, B, K, ep, s)) return rc;
-    const int64_t n = A.rows * B.rows, need = (n + 63) / 64, cap = (int64_t)papr_cu_count() * 16;
-    join_slabs_kernel<T><<<dim3((unsigned)(need < cap ? need : cap)), dim3(256), 0, s>>>(slab, n, (int)c.parts, (T*)out);
-    PAPR_CHECK_LAUNCH("papr_linear slabs");
-    return 0;
+    return join_slabs<T>(slab, A.rows * B.rows, (int)c.parts, (T*)out, s);
 }
 
 template <typename T, int FA>
