@@ -575,11 +575,13 @@ enum { PAPR_TYPE_F32 = 0, PAPR_TYPE_F16 = 1, PAPR_TYPE_BF16 = 2 };
  * Backward: with d_z = d_y act'(z):  d_x = d_z W (M, K),  d_w = d_z^T x (N, K),  d_b = column sums of d_z (N); each optional (NULL).  d_z is rounded to the
  * rows' type in front of the two products.  keep != 0: x is rows kept in 8 bits (papr_rows8_pack; ldx in codes, exps its exponents) and d_w = d_z^T of the
  * values they stand for.  M = 0: the forward call does nothing, the backward call is an error (the gradients are zero: the caller's).
- * float32 rows: infinities give NaN.  workspace: papr_linear_bwd_workspace_bytes(desc) bytes. */
+ * float32 rows: infinities give NaN.  workspace: papr_linear_fwd_workspace_bytes(desc) (mostly none: NULL) and
+ * papr_linear_bwd_workspace_bytes(desc) bytes, 16-byte aligned. */
 enum { PAPR_KEEP_ROWS = 0, PAPR_KEEP_E4M3 = 1, PAPR_KEEP_INT8 = 2 };
 typedef struct { int32_t type, act, keep, reserved; int64_t M, N, K; } papr_linear_desc;
 int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ld_res,
-                    void* y, void* z, papr_stream_t stream);
+                    void* y, void* z, void* workspace, papr_stream_t stream);
+size_t papr_linear_fwd_workspace_bytes(const papr_linear_desc* d);
 size_t papr_linear_bwd_workspace_bytes(const papr_linear_desc* d);
 int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64_t ld_dy, const void* z, const void* x, int64_t ldx, const void* exps, const void* w, int64_t ldw,
                     void* d_x, void* d_w, void* d_b, void* workspace, papr_stream_t stream);

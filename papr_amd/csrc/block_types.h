@@ -23,9 +23,13 @@ static inline bool papr_rows_aligned(const void* p, int64_t ld, int64_t width, i
     return ((uintptr_t)p & 15) == 0 && (ld * bytes) % 16 == 0 && (width * bytes) % 16 == 0;
 }
 
-// 1 / (1 + exp(-z)): the exponent's product with log2(e) in two parts (a relative error of a few ulp for every z), hardware exp2 and reciprocal.
+// 1 / (1 + exp(-z)), hardware exp2 and reciprocal.  EXACT (float32 rows): the exponent's product with log2(e) in two parts, a relative error of a few ulp for every z.
+// Otherwise one product: |z| 2^-24 relative, far below a 16-bit type's rounding, and half the instructions (they are what an epilogue of short sums waits for).
+template <bool EXACT>
 __device__ __forceinline__ float papr_sigmoid(float z) {
-    const float a = z * -1.44269504f, rest = fabsf(a) < 126.f ? __builtin_fmaf(z, -1.44269504f, -a) + z * -1.92596299e-8f : 0.f;
+    const float a = z * -1.44269504f;
+    if (!EXACT) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a));
+    const float rest = fabsf(a) < 126.f ? __builtin_fmaf(z, -1.44269504f, -a) + z * -1.92596299e-8f : 0.f;
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a) * __builtin_fmaf(rest, 0.693147181f, 1.f));
 }
 

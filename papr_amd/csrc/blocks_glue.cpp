@@ -31,6 +31,7 @@ namespace {
 PAPR_ENTRY(papr_last_error);
 PAPR_ENTRY(papr_linear_fwd);
 PAPR_ENTRY(papr_linear_bwd);
+PAPR_ENTRY(papr_linear_fwd_workspace_bytes);
 PAPR_ENTRY(papr_linear_bwd_workspace_bytes);
 PAPR_ENTRY(papr_rows8_pack);
 PAPR_ENTRY(papr_rows8_unpack);
@@ -44,6 +45,7 @@ void bind(const py::dict& at) {
     take(papr_last_error_, "papr_last_error");
     take(papr_linear_fwd_, "papr_linear_fwd");
     take(papr_linear_bwd_, "papr_linear_bwd");
+    take(papr_linear_fwd_workspace_bytes_, "papr_linear_fwd_workspace_bytes");
     take(papr_linear_bwd_workspace_bytes_, "papr_linear_bwd_workspace_bytes");
     take(papr_rows8_pack_, "papr_rows8_pack");
     take(papr_rows8_unpack_, "papr_rows8_unpack");
@@ -192,9 +194,11 @@ py::object linear(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe&
     auto shape = x.sizes().vec();                  // (outputs in their final shape: contiguous, so the same rows)
     shape.back() = N;
     Tensor y = fresh(rows, shape), z = slopes ? fresh(rows, {d.M, N}) : Tensor();
+    const size_t aside = papr_linear_fwd_workspace_bytes_(&d);
+    Tensor ws = aside ? bytes_like(rows, {(int64_t)aside}) : Tensor();
     {
         On on(rows);
-        check(papr_linear_fwd_(&d, ptr(rows), ld_of(rows), ptr(w2), ld_of(w2), ptr(b1), ptr(r2), ld_of(r2), ptr(y), ptr(z), on.stream), "papr_linear_fwd");
+        check(papr_linear_fwd_(&d, ptr(rows), ld_of(rows), ptr(w2), ld_of(w2), ptr(b1), ptr(r2), ld_of(r2), ptr(y), ptr(z), ptr(ws), on.stream), "papr_linear_fwd");
     }
     if (tracked) {
         auto node = std::shared_ptr<LinearBackward>(new LinearBackward(), torch::autograd::deleteNode);

@@ -98,9 +98,10 @@ struct Row {
 };
 
 // a(g) and a'(g)
+template <bool EXACT>
 __device__ __forceinline__ void gate_of(float g, int act, float& value, float& slope) {
     if (act == PAPR_GATE_NONE) { value = g; slope = 1.f; return; }
-    const float p = papr_sigmoid(g);
+    const float p = papr_sigmoid<EXACT>(g);
     value = act == PAPR_GATE_SIGMOID ? p : g * p;
     slope = act == PAPR_GATE_SIGMOID ? p * (1.f - p) : p * __builtin_fmaf(g, 1.f - p, 1.f);
 }
@@ -173,10 +174,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void join_fwd_kernel(papr_join_d
             if (d.gate_form == PAPR_GATE_FULL) {
                 R::values(ga, rg, width, j, whole);
 #pragma unroll
-                for (int i = 0; i < E; ++i) gate_of(ga[i], d.gate_act, ga[i], slope);
+                for (int i = 0; i < E; ++i) gate_of<sizeof(T) == 4>(ga[i], d.gate_act, ga[i], slope);
             } else {
                 float g = 1.f;
-                if (d.gate_form == PAPR_GATE_ROW) gate_of(g1, d.gate_act, g, slope);
+                if (d.gate_form == PAPR_GATE_ROW) gate_of<sizeof(T) == 4>(g1, d.gate_act, g, slope);
 #pragma unroll
                 for (int i = 0; i < E; ++i) ga[i] = g;
             }
@@ -282,10 +283,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void join_bwd_k
         if (d.f) {
             if (d.gate_form == PAPR_GATE_FULL) {
 #pragma unroll
-                for (int i = 0; i < E; ++i) gate_of(g[i], d.gate_act, ga[i], gs[i]);
+                for (int i = 0; i < E; ++i) gate_of<sizeof(T) == 4>(g[i], d.gate_act, ga[i], gs[i]);
             } else {
                 float gv = 1.f, sv = 0.f;
-                if (d.gate_form == PAPR_GATE_ROW) gate_of(g1, d.gate_act, gv, sv);
+                if (d.gate_form == PAPR_GATE_ROW) gate_of<sizeof(T) == 4>(g1, d.gate_act, gv, sv);
 #pragma unroll
                 for (int i = 0; i < E; ++i) { ga[i] = gv; gs[i] = sv; }
             }

@@ -55,7 +55,7 @@ __device__ __forceinline__ void act_values(float (&v)[N], int act) {
         }
     } else if (act == PAPR_ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] *= papr_sigmoid(v[i]);
+        for (int i = 0; i < N; ++i) v[i] *= papr_sigmoid<EXACT>(v[i]);
     }
 }
 // g <- g act'(z)
@@ -77,14 +77,14 @@ __device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], i
     } else if (act == PAPR_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float p = papr_sigmoid(z[i]);
+            const float p = papr_sigmoid<EXACT>(z[i]);
             g[i] *= p * __builtin_fmaf(z[i], 1.f - p, 1.f);
         }
     }
 }
 
 enum { K_RUNS = 0, ROWS_RUN = 1 };                // which index of an operand is contiguous in memory
-enum { OUT_FORWARD = 0, OUT_ROWS = 1, OUT_SLAB = 2 };
+enum { OUT_FORWARD = 0, OUT_ROWS = 1, OUT_SLAB = 2, OUT_FORWARD_LOOSE = 3 };      // (loose: rows of the results that start anywhere)
 
 template <typename T> struct Matrix { typedef bf16x8 frag; };
 template <> struct Matrix<f16> { typedef f16x8 frag; };
@@ -278,8 +278,13 @@ struct Plan {
     static constexpr size_t LOOP = (size_t)BUFFERS * BUF * 2, LDS = S::EPI > LOOP ? S::EPI : LOOP;
 };
 
-// E consecutive results of row m from column n on
-template <typename T, int OUT, int E>
+// E consecutive results of row m from column n on.  LOOSE: rows that start anywhere (the hardware takes 16 bytes at any address, in two requests).
+template <typename T, int E, bool LOOSE>
+__device__ __forceinline__ void put(T* to, const papr_pack<T, E>& t) {
+    if (LOOSE) __builtin_memcpy(to, &t, sizeof(t));
+    else *reinterpret_cast<papr_pack<T, E>*>(to) = t;
+}
+template <typename T, int OUT, int E, bool LOOSE>
 __device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int64_t N, const float (&bias)[E], const papr_pack<T, E>& res, const Epilogue& ep) {
     if (OUT == OUT_FORWARD) {
 #pragma unroll
@@ -288,7 +293,7 @@ __device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int6
             papr_pack<T, E> t;
 #pragma unroll
             for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
-            *reinterpret_cast<papr_pack<T, E>*>(reinterpret_cast<T*>(ep.z) + m * N + n) = t;
+            put<T, E, LOOSE>(reinterpret_cast<T*>(ep.z) + m * N + n, t);
         }
         act_values<sizeof(T) == 4>(v, ep.act);
         if (ep.res)
@@ -298,7 +303,49 @@ __device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int6
     papr_pack<T, E> t;
 #pragma unroll
     for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
-    *reinterpret_cast<papr_pack<T, E>*>(reinterpret_cast<T*>(ep.out) + m * N + n) = t;
+    put<T, E, LOOSE>(reinterpret_cast<T*>(ep.out) + m * N + n, t);
+}
+// 32 rows of a wave's part, from its LDS: 16 bytes of a row a lane
+template <typename T, int OUT, typename S, bool LOOSE>
+__device__ __forceinline__ void write_block(const float* epi, int64_t mw, int64_t n, int64_t M, int64_t N, const float (&bias)[16 / sizeof(T)], const Epilogue& ep) {
+    constexpr int COLS = S::IN * 32, E = 16 / sizeof(T), LPR = COLS / E, RPP = 64 / LPR;
+    const int lane = threadIdx.x & 63;
+    const bool whole = LOOSE ? n + E <= N : n < N, with_res = OUT == OUT_FORWARD && ep.res;
+    papr_pack<T, E> res[32 / RPP];
+    if (with_res)
+#pragma unroll
+        for (int r = 0; r < 32 / RPP; ++r) {
+            const int64_t m = mw + r * RPP + lane / LPR;
+            if (m >= M || !whole) continue;
+            const T* src = reinterpret_cast<const T*>(ep.res) + m * ep.ld_res + n;
+            if (LOOSE) __builtin_memcpy(&res[r], src, sizeof(res[r]));
+            else res[r] = *reinterpret_cast<const papr_pack<T, E>*>(src);
+        }
+#pragma unroll
+    for (int r = 0; r < 32 / RPP; ++r) {
+        const int64_t m = mw + r * RPP + lane / LPR;
+        const float* at = epi + (r * RPP + lane / LPR) * S::EPI_STRIDE + lane % LPR * E;
+        float v[E];
+#pragma unroll
+        for (int c = 0; c < E; c += 4) {
+            const float4 t = *reinterpret_cast<const float4*>(at + c);
+            v[c] = t.x; v[c + 1] = t.y; v[c + 2] = t.z; v[c + 3] = t.w;
+        }
+        if (m < M && whole) finish<T, OUT, E, LOOSE>(v, m, n, N, bias, res[r], ep);
+    }
+    if (LOOSE && !whole)                           // (the last columns of the rows)
+#pragma unroll 1
+        for (int r = 0; r < 32 / RPP; ++r) {
+            const int64_t m = mw + r * RPP + lane / LPR;
+            const float* at = epi + (r * RPP + lane / LPR) * S::EPI_STRIDE + lane % LPR * E;
+#pragma unroll 1
+            for (int i = 0; m < M && n + i < N; ++i) {
+                float v1[1] = {at[i]}, b1[1] = {OUT == OUT_FORWARD && ep.bias ? (float)reinterpret_cast<const T*>(ep.bias)[n + i] : 0.f};
+                papr_pack<T, 1> r1;
+                if (with_res) r1.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n + i];
+                finish<T, OUT, 1, false>(v1, m, n + i, N, b1, r1, ep);
+            }
+        }
 }
 
 // The results of a workgroup's tile, from the accumulators of its waves.  smem: Shape::EPI bytes, free of earlier readers.
@@ -322,23 +369,14 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[S::IM][S::IN], sh
         }
         return;
     }
-    // Through LDS, 32 rows of the wave's own at a time (no barrier), so that a lane takes 16 bytes of a row: 16-byte loads and stores of whole lines.  Rows that do not
-    // start on 16 bytes: a lane takes single columns, 64 (32) lanes a row.
+    // Through LDS, 32 rows of the wave's own at a time (no barrier), so that a lane takes 16 bytes of a row: whole lines in and out.
     float* epi = reinterpret_cast<float*>(smem) + wave * 32 * EPI_STRIDE;
-    constexpr int COLS = IN * 32, E = 16 / sizeof(T), LPR = COLS / E, RPP = 64 / LPR;
-    const int64_t nw = n0 + wn * COLS;
-    const bool wide = ep.wide;
-    const int64_t n = nw + (wide ? lane % LPR * E : lane % COLS);
+    constexpr int COLS = IN * 32, E = 16 / sizeof(T);
+    constexpr bool FORWARD = OUT == OUT_FORWARD || OUT == OUT_FORWARD_LOOSE;
+    const int64_t n = n0 + wn * COLS + lane % (COLS / E) * E;
     float bias[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) bias[i] = 0.f;
-    if (OUT == OUT_FORWARD && ep.bias && n < N) {
-        const T* src = reinterpret_cast<const T*>(ep.bias) + n;
-        if (wide) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) bias[i] = (float)src[i];
-        } else bias[0] = (float)src[0];
-    }
+    for (int i = 0; i < E; ++i) bias[i] = FORWARD && ep.bias && n + i < N ? (float)reinterpret_cast<const T*>(ep.bias)[n + i] : 0.f;
 #pragma unroll
     for (int i = 0; i < IM; ++i) {
         const int64_t mw = m0 + (wm * IM + i) * 32;
@@ -346,38 +384,11 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[S::IM][S::IN], sh
         for (int j = 0; j < IN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) epi[((e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * EPI_STRIDE + j * 32 + (lane & 31)] = acc[i][j][e];
-        if (wide) {
-            papr_pack<T, E> res[32 / RPP];
-#pragma unroll
-            for (int r = 0; r < 32 / RPP; ++r) {
-                const int64_t m = mw + r * RPP + lane / LPR;
-                if (OUT == OUT_FORWARD && ep.res && m < M && n < N) res[r] = *reinterpret_cast<const papr_pack<T, E>*>(reinterpret_cast<const T*>(ep.res) + m * ep.ld_res + n);
-            }
-#pragma unroll
-            for (int r = 0; r < 32 / RPP; ++r) {
-                const int64_t m = mw + r * RPP + lane / LPR;
-                float v[E];
-#pragma unroll
-                for (int c = 0; c < E; c += 4) {
-                    const float4 t = *reinterpret_cast<const float4*>(epi + (r * RPP + lane / LPR) * EPI_STRIDE + lane % LPR * E + c);
-                    v[c] = t.x; v[c + 1] = t.y; v[c + 2] = t.z; v[c + 3] = t.w;
-                }
-                if (m < M && n < N) finish<T, OUT, E>(v, m, n, N, bias, res[r], ep);
-            }
-        } else {
-            constexpr int ROWS = 64 / COLS;
-#pragma unroll 4
-            for (int r = 0; r < 32; r += ROWS) {
-                const int64_t m = mw + r + lane / COLS;
-                float v[1] = {epi[(r + lane / COLS) * EPI_STRIDE + lane % COLS]};
-                const float b1[1] = {bias[0]};
-                if (m < M && n < N) {
-                    papr_pack<T, 1> res;
-                    if (OUT == OUT_FORWARD && ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
-                    finish<T, OUT, 1>(v, m, n, N, b1, res, ep);
-                }
-            }
-        }
+        // (the forward pass's two forms are kernels of their own: an activation's five forms times a tile's passes, twice, do not fit the instruction cache -- with both
+        // in one kernel 65,536 x 1024 -> 1024 took 345 us for 235)
+        if constexpr (FORWARD) write_block<T, OUT_FORWARD, S, OUT == OUT_FORWARD_LOOSE>(epi, mw, n, M, N, bias, ep);
+        else if (ep.wide) write_block<T, OUT, S, false>(epi, mw, n, M, N, bias, ep);
+        else write_block<T, OUT, S, true>(epi, mw, n, M, N, bias, ep);
     }
 }
 
@@ -704,7 +715,7 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand
         if (ep.bias) bias[0] = (float)reinterpret_cast<const T*>(ep.bias)[n];
         papr_pack<T, 1> res;
         if (ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
-        finish<T, OUT_FORWARD, 1>(v, m, n, N, bias, res, ep);
+        finish<T, OUT_FORWARD, 1, false>(v, m, n, N, bias, res, ep);
     }
 }
 
@@ -782,7 +793,7 @@ int join_slabs(const float* slab, int64_t n, int parts, T* out, hipStream_t s) {
 // d_z = d_y act'(z) in the rows' type (none: d_y as it is, nothing is written) and the column sums of it in float32, one partial row per workgroup.
 // D: the rows' type, or float32 for a product of few terms (keeps_wide).  A thread holds whole vectors of columns; the threads of a workgroup beyond one row's take further rows.
 template <typename T, typename D, bool VEC>
-__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, int64_t ld, const T* __restrict__ z, int64_t M, int N, int act, int lanes, D* __restrict__ d_z,
+__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, int64_t ld, const T* __restrict__ z, int64_t M, int N, int act, int lanes, D* __restrict__ d_z, int64_t ldz,
                                                     float* __restrict__ part, int64_t rows_per_block) {
     constexpr int V = VEC ? 16 / sizeof(T) : 1;
     __shared__ float fold[256 * V];
@@ -792,6 +803,8 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    if (d_z && !VEC && c >= N && c < ldz)           // (zeros up to whole vectors)
+        for (int64_t m = beg + rl; m < end; m += per) d_z[m * ldz + c] = (D)0.f;
     if (c < N)
 #pragma unroll 4
         for (int64_t m = beg + rl; m < end; m += per) {
@@ -808,8 +821,8 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
                     sum[i] += v[i];
                     to.v[i] = (D)v[i];
                 }
-                if constexpr (VEC) *reinterpret_cast<decltype(to)*>(d_z + m * N + c) = to;
-                else d_z[m * N + c] = to.v[0];
+                if constexpr (VEC) *reinterpret_cast<decltype(to)*>(d_z + m * ldz + c) = to;
+                else d_z[m * ldz + c] = to.v[0];
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[i] += (float)g.v[i];
@@ -897,8 +910,8 @@ int weight_product(int keep, bool vec, const Operand& A, const Operand& B, int64
 template <typename T>
 int forward(const Operand& x, const Operand& w, int64_t K, bool vec, const Epilogue& ep, hipStream_t s) {
     if (x.rows <= FEW_ROWS) return launch_few_rows<T>(x, w, K, vec, ep, s);
-    const Choice c = choose(x.rows, w.rows, K, path_of(sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, vec, 0, false), false);
-    return launch_product<T, K_RUNS, K_RUNS, 0, 0, OUT_FORWARD>(c, vec, x, w, K, ep, s);
+    const Choice c = choose(x.rows, w.rows, K, path_of(sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, vec, 0, false), false, aside_of(ep.res, ep.z, sizeof(T)));
+    return ep.wide ? launch_product<T, K_RUNS, K_RUNS, 0, 0, OUT_FORWARD>(c, vec, x, w, K, ep, s) : launch_product<T, K_RUNS, K_RUNS, 0, 0, OUT_FORWARD_LOOSE>(c, vec, x, w, K, ep, s);
 }
 
 template <typename T>
@@ -916,14 +929,14 @@ int grad_weight(bool wide, int keep, bool vec, const Operand& d_z, const Operand
 }
 
 template <typename T>
-int slopes(bool wide, bool vec, const SlopeGrid& g, const void* d_y, int64_t ld, const void* z, int64_t M, int N, int act, void* d_z, float* part, hipStream_t s) {
+int slopes(bool wide, bool vec, const SlopeGrid& g, const void* d_y, int64_t ld, const void* z, int64_t M, int N, int act, void* d_z, int64_t ldz, float* part, hipStream_t s) {
     const dim3 grid((unsigned)g.blocks, g.cols);
     if (wide) {
-        if (vec) slope_kernel<T, float, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (float*)d_z, part, g.rows_per_block);
-        else slope_kernel<T, float, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (float*)d_z, part, g.rows_per_block);
+        if (vec) slope_kernel<T, float, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (float*)d_z, ldz, part, g.rows_per_block);
+        else slope_kernel<T, float, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (float*)d_z, ldz, part, g.rows_per_block);
     } else {
-        if (vec) slope_kernel<T, T, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (T*)d_z, part, g.rows_per_block);
-        else slope_kernel<T, T, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (T*)d_z, part, g.rows_per_block);
+        if (vec) slope_kernel<T, T, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (T*)d_z, ldz, part, g.rows_per_block);
+        else slope_kernel<T, T, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (T*)d_z, ldz, part, g.rows_per_block);
     }
     PAPR_CHECK_LAUNCH("papr_linear_bwd");
     return 0;
@@ -937,5 +950,5 @@ int slopes(bool wide, bool vec, const SlopeGrid& g, const void* d_y, int64_t ld,
     template int forward<T>(const Operand&, const Operand&, int64_t, bool, const Epilogue&, hipStream_t);                                                           \
     template int grad_rows<T>(bool, bool, const Operand&, const Operand&, int64_t, void*, float*, hipStream_t);                                                     \
     template int grad_weight<T>(bool, int, bool, const Operand&, const Operand&, int64_t, void*, float*, hipStream_t);                                              \
-    template int slopes<T>(bool, bool, const SlopeGrid&, const void*, int64_t, const void*, int64_t, int, int, void*, float*, hipStream_t);                         \
+    template int slopes<T>(bool, bool, const SlopeGrid&, const void*, int64_t, const void*, int64_t, int, int, void*, int64_t, float*, hipStream_t);                \
     }

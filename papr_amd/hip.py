@@ -27,7 +27,7 @@ EXPORTS = [
     "papr_rownorm_fwd", "papr_rownorm_bwd", "papr_row_dots", "papr_qk_bias_bwd_workspace_bytes", "papr_qk_bias_bwd", "papr_mse_workspace_bytes", "papr_mse_fwd", "papr_ln_fold_fwd", "papr_ln_fold_bwd", "papr_ln_fold_fwd_batch", "papr_ln_fold_bwd_batch", "papr_mlp_fwd_workspace_bytes", "papr_mlp_bwd_workspace_bytes", "papr_mlp_saved_floats", "papr_mlp_bwd_needs_weight_t", "papr_mlp_fwd",
     "papr_mlp_bwd", "papr_mlp_bwd_takes_f16_rows",
     "papr_attn_tail_fwd", "papr_attn_tail_bwd", "papr_conv3x3_weight_halfs", "papr_conv3x3_workspace_bytes", "papr_conv3x3_fwd", "papr_conv3x3_wgrad_workspace_bytes", "papr_conv3x3_wgrad", "papr_maxpool2_fwd", "papr_maxpool2_bwd", "papr_upconv2x2_fwd", "papr_upconv2x2_dgrad", "papr_upconv2x2_wgrad_workspace_bytes", "papr_upconv2x2_wgrad", "papr_conv1x1_fwd", "papr_conv1x1_bwd_workspace_bytes", "papr_conv1x1_bwd", "papr_small_unet_state_bytes", "papr_small_unet_bwd_workspace_bytes", "papr_small_unet_fwd", "papr_small_unet_bwd", "papr_adam_step", "papr_adam_step_scaled", "papr_composite_fwd", "papr_composite_bwd_workspace_bytes", "papr_composite_bwd", "papr_profile_enable", "papr_profile_collect", "papr_set_switch", "papr_get_switch",
-    "papr_linear_fwd", "papr_linear_bwd_workspace_bytes", "papr_linear_bwd", "papr_rows8_pack", "papr_rows8_unpack",
+    "papr_linear_fwd", "papr_linear_fwd_workspace_bytes", "papr_linear_bwd_workspace_bytes", "papr_linear_bwd", "papr_rows8_pack", "papr_rows8_unpack",
     "papr_join_fwd", "papr_join_bwd_workspace_bytes", "papr_join_bwd",
 ]
 
@@ -200,7 +200,9 @@ def lib():
     L.papr_attn_tail_fwd.argtypes = [C.POINTER(TailDesc), vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp]
     L.papr_attn_tail_bwd.argtypes = [C.POINTER(TailDesc), vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                      C.POINTER(F16Rows), C.POINTER(F16Rows), vp]
-    L.papr_linear_fwd.argtypes = [C.POINTER(LinearDesc), vp, i64, vp, i64, vp, vp, i64, vp, vp, vp]
+    L.papr_linear_fwd.argtypes = [C.POINTER(LinearDesc), vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, vp]
+    L.papr_linear_fwd_workspace_bytes.restype = C.c_size_t
+    L.papr_linear_fwd_workspace_bytes.argtypes = [C.POINTER(LinearDesc)]
     L.papr_linear_bwd_workspace_bytes.restype = C.c_size_t
     L.papr_linear_bwd_workspace_bytes.argtypes = [C.POINTER(LinearDesc)]
     L.papr_linear_bwd.argtypes = [C.POINTER(LinearDesc), vp, i64, vp, vp, i64, vp, vp, i64, vp, vp, vp, vp, vp]

@@ -73,13 +73,13 @@ def test_c_entry_points_refuse_before_touching_a_device():
     L = hip.lib()
     p = C.c_void_p(4096)                                 # (never read: the checks come first)
     D = hip.LinearDesc
-    refused(L.papr_linear_fwd(None, p, 8, p, 8, None, None, 0, p, None, None), "no descriptor")
-    refused(L.papr_linear_fwd(D(3, 0, 0, 0, 4, 6, 8), p, 8, p, 8, None, None, 0, p, None, None), "row type")
-    refused(L.papr_linear_fwd(D(0, 5, 0, 0, 4, 6, 8), p, 8, p, 8, None, None, 0, p, None, None), "activation")
-    refused(L.papr_linear_fwd(D(0, 0, 0, 0, -1, 6, 8), p, 8, p, 8, None, None, 0, p, None, None), "M -1")
-    refused(L.papr_linear_fwd(D(0, 0, 0, 0, 4, 6, 0), p, 8, p, 8, None, None, 0, p, None, None), "K 0")
-    refused(L.papr_linear_fwd(D(0, 0, 0, 0, 4, 6, 8), None, 8, p, 8, None, None, 0, p, None, None), "missing")
-    assert L.papr_linear_fwd(D(0, 0, 0, 0, 0, 6, 8), None, 8, p, 8, None, None, 0, None, None, None) == 0        # no rows: nothing to do
+    refused(L.papr_linear_fwd(None, p, 8, p, 8, None, None, 0, p, None, None, None), "no descriptor")
+    refused(L.papr_linear_fwd(D(3, 0, 0, 0, 4, 6, 8), p, 8, p, 8, None, None, 0, p, None, None, None), "row type")
+    refused(L.papr_linear_fwd(D(0, 5, 0, 0, 4, 6, 8), p, 8, p, 8, None, None, 0, p, None, None, None), "activation")
+    refused(L.papr_linear_fwd(D(0, 0, 0, 0, -1, 6, 8), p, 8, p, 8, None, None, 0, p, None, None, None), "M -1")
+    refused(L.papr_linear_fwd(D(0, 0, 0, 0, 4, 6, 0), p, 8, p, 8, None, None, 0, p, None, None, None), "K 0")
+    refused(L.papr_linear_fwd(D(0, 0, 0, 0, 4, 6, 8), None, 8, p, 8, None, None, 0, p, None, None, None), "missing")
+    assert L.papr_linear_fwd(D(0, 0, 0, 0, 0, 6, 8), None, 8, p, 8, None, None, 0, None, None, None, None) == 0        # no rows: nothing to do
     bwd = lambda d, dy=p, z=p, x=p, e=None, w=p, dx=p, dw=p, db=p, ws=p: L.papr_linear_bwd(d, dy, 6, z, x, 8, e, w, 8, dx, dw, db, ws, None)
     refused(bwd(D(0, 0, 0, 0, 0, 6, 8)), "no rows")
     refused(bwd(D(0, 0, 3, 0, 4, 6, 8)), "format")
