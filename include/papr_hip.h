@@ -578,6 +578,7 @@ enum { PAPR_TYPE_F32 = 0, PAPR_TYPE_F16 = 1, PAPR_TYPE_BF16 = 2 };
  * float32 rows: infinities give NaN.  workspace: papr_linear_fwd_workspace_bytes(desc) (mostly none: NULL) and
  * papr_linear_bwd_workspace_bytes(desc) bytes, 16-byte aligned. */
 enum { PAPR_KEEP_ROWS = 0, PAPR_KEEP_E4M3 = 1, PAPR_KEEP_INT8 = 2 };
+#define PAPR_LINEAR_MAX_STRIDE (1 << 22)      /* elements between rows of x, W and d_y; M < 2^31, N and K <= 2^20 */
 typedef struct { int32_t type, act, keep, reserved; int64_t M, N, K; } papr_linear_desc;
 int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ld_res,
                     void* y, void* z, void* workspace, papr_stream_t stream);

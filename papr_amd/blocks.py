@@ -129,6 +129,8 @@ def _explain_linear(x, weight, bias, residual, act, keep):
     if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1:
         _fail(who, "weight has shape %s, x %s" % (tuple(weight.shape), tuple(x.shape)))
     N = weight.shape[0]
+    if max(weight.shape) > 1 << 20:
+        _fail(who, "weight has shape %s (at most %d a side)" % (tuple(weight.shape), 1 << 20))
     for name, t, shape in (("bias", bias, (N,)), ("residual", residual, tuple(x.shape[:-1]) + (N,))):
         if t is None:
             continue

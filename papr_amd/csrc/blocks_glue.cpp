@@ -80,10 +80,10 @@ Tensor untracked(const Tensor& t) { return t.requires_grad() ? t.detach() : t; }
 Tensor rows_of(const Tensor& given, int64_t width) {
     Tensor t = untracked(given);
     if (t.dim() != 2) t = t.reshape({-1, width});
-    if ((width > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < width)) t = t.contiguous();
+    if ((width > 1 && t.stride(1) != 1) || (t.size(0) > 1 && (t.stride(0) < width || t.stride(0) > PAPR_LINEAR_MAX_STRIDE))) t = t.contiguous();
     return t;
 }
-int64_t ld_of(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }
+int64_t ld_of(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 int64_t ld_of(const Maybe& t) { return t ? ld_of(*t) : 0; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
@@ -171,7 +171,7 @@ struct LinearBackward : Node {
 bool linear_fits(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int act, int keep_fmt) {
     if (!x.is_cuda() || type_of(x) < 0 || x.dim() < 1 || w.dim() != 2 || w.scalar_type() != x.scalar_type() || w.device() != x.device() || act < 0 || keep_fmt < 0) return false;
     const int64_t K = w.size(1), N = w.size(0);
-    if (K < 1 || N < 1 || x.size(-1) != K) return false;
+    if (K < 1 || N < 1 || x.size(-1) != K || K > (1 << 20) || N > (1 << 20)) return false;
     if (b && (b->scalar_type() != x.scalar_type() || b->device() != x.device() || b->dim() != 1 || b->size(0) != N)) return false;
     if (!r) return true;
     if (r->scalar_type() != x.scalar_type() || r->device() != x.device() || r->dim() != x.dim() || r->size(-1) != N) return false;

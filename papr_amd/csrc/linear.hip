@@ -93,6 +93,8 @@ int linear_check(const char* who, int type, int64_t M, int64_t N, int64_t K, int
     PAPR_REQUIRE(act >= PAPR_ACT_NONE && act <= PAPR_ACT_SILU, "%s: unknown activation %d", who, act);
     return 0;
 }
+// (a tile's rows lie at 32-bit offsets from its first: 256 rows of float32)
+bool stride_ok(int64_t ld, int64_t width) { return ld >= width && ld <= PAPR_LINEAR_MAX_STRIDE; }
 
 }  // namespace
 
@@ -107,6 +109,8 @@ extern "C" int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t
     if (int rc = linear_check("papr_linear_fwd", d->type, d->M, d->N, d->K, d->act)) return rc;
     if (d->M == 0) return 0;
     PAPR_REQUIRE(x && w && y, "papr_linear_fwd: a pointer is missing");
+    PAPR_REQUIRE(stride_ok(ldx, d->K) && stride_ok(ldw, d->K), "papr_linear_fwd: row strides %lld, %lld (%lld .. %d)", (long long)ldx, (long long)ldw, (long long)d->K,
+                 PAPR_LINEAR_MAX_STRIDE);
     const int b = papr_type_bytes(d->type);
     bool vec = papr_rows_aligned(x, ldx, d->K, b) && papr_rows_aligned(w, ldw, d->K, b);
     Operand A = {x, ldx, d->M, nullptr}, B = {w, ldw, d->N, nullptr};
@@ -164,6 +168,9 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
     PAPR_REQUIRE(d_y && workspace && (d->act == PAPR_ACT_NONE || z), "papr_linear_bwd: a pointer is missing");
     PAPR_REQUIRE(!d_x || w, "papr_linear_bwd: d_x needs the weight");
     PAPR_REQUIRE(!d_w || (x && (!d->keep || exps)), "papr_linear_bwd: d_w needs the rows");
+    PAPR_REQUIRE(stride_ok(ld_dy, N) && (!d_x || stride_ok(ldw, K)) && (!d_w || d->keep || stride_ok(ldx, K)), "papr_linear_bwd: row strides (at most %d)", PAPR_LINEAR_MAX_STRIDE);
+    PAPR_REQUIRE(!d_w || !d->keep || (ldx == (K + 31) / 32 * 32 && ((uintptr_t)x & 7) == 0), "papr_linear_bwd: kept rows are whole blocks of 32 codes on 8 bytes");
+    PAPR_REQUIRE(((uintptr_t)workspace & 15) == 0, "papr_linear_bwd: the workspace starts on 16 bytes");
     const int b = papr_type_bytes(d->type);
     const bool slope = d->act != PAPR_ACT_NONE, wide = keeps_wide(d);
     const Layout l = layout_of(d);

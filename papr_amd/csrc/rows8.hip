@@ -125,6 +125,7 @@ extern "C" int papr_rows8_pack(int32_t type, int32_t fmt, const void* x, int64_t
     PAPR_REQUIRE(rows >= 0 && width >= 1, "papr_rows8_pack: rows %lld, width %d", (long long)rows, width);
     if (rows == 0) return 0;
     PAPR_REQUIRE(x && codes && exps, "papr_rows8_pack: a pointer is missing");
+    PAPR_REQUIRE(((uintptr_t)codes & 7) == 0, "papr_rows8_pack: the codes start on 8 bytes");
     const int blocks = (width + 31) / 32;
     const unsigned grid = rows8_grid(rows, blocks);
     hipStream_t s = as_stream(stream);
@@ -147,6 +148,7 @@ extern "C" int papr_rows8_unpack(int32_t type, int32_t fmt, const void* codes, c
     PAPR_REQUIRE(rows >= 0 && width >= 1, "papr_rows8_unpack: rows %lld, width %d", (long long)rows, width);
     if (rows == 0) return 0;
     PAPR_REQUIRE(x && codes && exps, "papr_rows8_unpack: a pointer is missing");
+    PAPR_REQUIRE(((uintptr_t)codes & 7) == 0, "papr_rows8_unpack: the codes start on 8 bytes");
     const int blocks = (width + 31) / 32;
     const unsigned grid = rows8_grid(rows, blocks);
     hipStream_t s = as_stream(stream);

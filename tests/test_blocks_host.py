@@ -19,6 +19,7 @@ def rows_norm(n=8, dtype=torch.float32, kind="rmsnorm"):
     (lambda: blocks.linear_rows(X, torch.zeros(6, 7)), "weight has shape"),
     (lambda: blocks.linear_rows(X, torch.zeros(0, 8)), "weight has shape"),
     (lambda: blocks.linear_rows(X, torch.zeros(8)), "weight has shape"),
+    (lambda: blocks.linear_rows(torch.zeros(1, 1), torch.zeros((1 << 20) + 1, 1)), "at most"),
     (lambda: blocks.linear_rows(X, W.half()), "weight is torch.float16"),
     (lambda: blocks.linear_rows(X.double(), W.double()), "float64"),
     (lambda: blocks.linear_rows(X, W, torch.zeros(8)), "bias has shape"),
@@ -79,6 +80,8 @@ def test_c_entry_points_refuse_before_touching_a_device():
     refused(L.papr_linear_fwd(D(0, 0, 0, 0, -1, 6, 8), p, 8, p, 8, None, None, 0, p, None, None, None), "M -1")
     refused(L.papr_linear_fwd(D(0, 0, 0, 0, 4, 6, 0), p, 8, p, 8, None, None, 0, p, None, None, None), "K 0")
     refused(L.papr_linear_fwd(D(0, 0, 0, 0, 4, 6, 8), None, 8, p, 8, None, None, 0, p, None, None, None), "missing")
+    refused(L.papr_linear_fwd(D(0, 0, 0, 0, 4, 6, 8), p, 7, p, 8, None, None, 0, p, None, None, None), "row strides")
+    refused(L.papr_linear_fwd(D(0, 0, 0, 0, 4, 6, 8), p, (1 << 22) + 1, p, 8, None, None, 0, p, None, None, None), "row strides")
     assert L.papr_linear_fwd(D(0, 0, 0, 0, 0, 6, 8), None, 8, p, 8, None, None, 0, None, None, None, None) == 0        # no rows: nothing to do
     bwd = lambda d, dy=p, z=p, x=p, e=None, w=p, dx=p, dw=p, db=p, ws=p: L.papr_linear_bwd(d, dy, 6, z, x, 8, e, w, 8, dx, dw, db, ws, None)
     refused(bwd(D(0, 0, 0, 0, 0, 6, 8)), "no rows")
@@ -88,11 +91,15 @@ def test_c_entry_points_refuse_before_touching_a_device():
     refused(bwd(D(0, 0, 0, 0, 4, 6, 8), w=None), "weight")
     refused(bwd(D(0, 0, 0, 0, 4, 6, 8), x=None), "rows")
     refused(bwd(D(0, 0, 1, 0, 4, 6, 8)), "rows")         # kept rows without their exponents
+    refused(bwd(D(0, 0, 1, 0, 4, 6, 8), e=p), "32 codes")    # ... whose rows are not whole blocks
+    refused(bwd(D(0, 0, 0, 0, 4, 6, 8), ws=C.c_void_p(4100)), "16 bytes")
+    refused(bwd(D(0, 0, 0, 0, 4, 7, 8)), "row strides")      # d_y's rows overlap
     assert L.papr_linear_bwd_workspace_bytes(D(0, 0, 0, 0, 0, 6, 8)) == 0
     refused(L.papr_rows8_pack(0, 0, p, 8, 4, 8, p, p, None), "format")
     refused(L.papr_rows8_pack(4, 1, p, 8, 4, 8, p, p, None), "type")
     refused(L.papr_rows8_pack(0, 1, p, 8, 4, 0, p, p, None), "width")
     refused(L.papr_rows8_pack(0, 1, p, 8, 4, 8, p, None, None), "missing")
+    refused(L.papr_rows8_pack(0, 1, p, 8, 4, 8, C.c_void_p(4100), p, None), "8 bytes")
     refused(L.papr_rows8_unpack(0, 1, None, p, 4, 8, p, None), "missing")
     assert L.papr_rows8_pack(0, 1, None, 8, 0, 8, None, None, None) == 0
     N = hip.BlockNorm

@@ -145,6 +145,64 @@ def test_linear_rows_strides_and_shapes(dt):
     assert torch.equal(ws.grad, w2.grad) and torch.equal(rs.grad, torch.full_like(r, 36.0))
 
 
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("M, N, K, act, keep", [(8191, 1001, 1003, "silu", None), (8192, 1000, 701, "none", None), (6000, 501, 1408, "gelu", None), (9000, 701, 800, "silu", "int8"),
+                                                (3001, 1104, 1009, "none", None)])
+def test_linear_rows_of_odd_16_bit_rows_that_are_copied_into_whole_vectors(dt, M, N, K, act, keep):
+    """Long products of odd rows stream from padded copies (x, W, d_y, each where its own width is odd; d_z leaves its kernel padded)."""
+    check_linear(*linear_data(M, N, K, dt, seed=M % 97), act=act, keep=keep)
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=ids)
+@pytest.mark.parametrize("M, N, K", [(2048, 2048, 512), (4100, 1040, 264), (700, 3000, 1000)])
+def test_linear_rows_large_tiles(dt, M, N, K):
+    check_linear(*linear_data(M, N, K, dt, seed=M % 89), act="gelu")
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=ids)
+def test_small_products_lose_nothing_to_a_rounded_d_z(dt):
+    """Up to 2^28 terms d_z stays in float32: what is left beside the final rounding (rms u / sqrt 3 of uniform errors, e_out) is z's own, at most 0.8 u |z| rms through the
+    slope's derivative -- under half of e_out: together below 1.15 e_out (with d_z rounded too it was 1.45)."""
+    x, w, b, r, d_y = linear_data(400, 512, 512, dt, seed=12)
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    got = torch.autograd.grad(blocks.linear_rows(x, w, b, r, act="silu"), leaves, d_y)
+    x6, w6 = (t.detach().double() for t in (x, w))
+    d_z = d_y.double() * act64(x6 @ w6.t() + b.double(), "silu")[1]
+    for g, ref in zip(got, (d_z @ w6, d_z.t() @ x6)):
+        floor = (ref.to(dt).double() - ref).norm()
+        assert (g.double() - ref).norm() <= 1.15 * floor
+
+
+def test_linear_rows_far_rows_and_single_rows():
+    """Rows five million elements apart (their tile's offsets pass 32 bits: a copy), a vector instead of rows, a bias and weight that are views."""
+    store = torch.zeros((5_000_000 * 39 + 40,), device="cuda", dtype=torch.float16)
+    far = store.as_strided((40, 32), (5_000_000, 1))
+    far.copy_(torch.randn((40, 32), generator=gen(3), device="cuda"))
+    w, b = torch.randn((2, 64, 50), generator=gen(4), device="cuda").half()[1, :, 3:35], torch.randn((64, 2), generator=gen(5), device="cuda").half()[:, 1]
+    assert torch.equal(blocks.linear_rows(far, w, b), blocks.linear_rows(far.contiguous(), w.contiguous(), b.contiguous()))
+    assert torch.equal(blocks.norm_rows(far, blocks.Norm("rmsnorm")), blocks.norm_rows(far.contiguous(), blocks.Norm("rmsnorm")))
+    one = blocks.linear_rows(far[0], w, b, residual=b, act="silu")
+    assert one.shape == (64,) and torch.equal(one, blocks.linear_rows(far[:1], w, b, residual=b[None], act="silu")[0])
+    assert blocks.pack_rows(far[0]).rows().shape == (32,)
+
+
+def test_operands_written_to_and_graphs_run_twice_are_refused():
+    x, w = torch.randn((8, 16), device="cuda"), torch.randn((16, 16), device="cuda", requires_grad=True)
+    y = blocks.linear_rows(x, w, act="silu")
+    x.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    gain = torch.ones(16, device="cuda", requires_grad=True)
+    y = blocks.join_rows(x, x * 2, post=blocks.Norm("rmsnorm", gain))
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    y = blocks.join_rows(x, x * 2, post=blocks.Norm("rmsnorm", gain))
+    x.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+
+
 def test_linear_rows_of_nothing():
     for dt in DTYPES:
         x, w, b = torch.zeros((0, 24), device="cuda", dtype=dt, requires_grad=True), torch.ones((8, 24), device="cuda", dtype=dt, requires_grad=True), torch.ones((8,), device="cuda", dtype=dt, requires_grad=True)
@@ -595,8 +653,32 @@ def test_captured_steps_replay_with_new_inputs():
             assert all(torch.equal(a, b) for a, b in zip(out, want)) and all(torch.equal(a, b) for a, b in zip(grads, want_g))
 
 
+def test_a_step_accumulates_into_leaves_and_tracks_only_what_is_asked():
+    """backward() into .grad twice is twice the gradient; without grad mode nothing is tracked; the residual alone passes its gradient through."""
+    p = {n: t.requires_grad_(True) for n, t in block_params(torch.bfloat16, 64, 128, 1).items()}
+    x = torch.randn((33, 64), generator=gen(2), device="cuda").bfloat16()
+    for _ in range(2):
+        y, h = block(p, x, "e4m3")
+        (y.float().sum() + h.float().square().sum()).backward()
+    twice = {n: t.grad.clone() for n, t in p.items()}
+    for t in p.values():
+        t.grad = None
+    y, h = block(p, x, "e4m3")
+    (y.float().sum() + h.float().square().sum()).backward()
+    assert all(torch.equal(twice[n], p[n].grad * 2) for n in p)
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in block(p, x, None))
+    r = torch.randn((33, 128), device="cuda").bfloat16().requires_grad_(True)
+    blocks.linear_rows(x, p["w1"].detach(), None, r, act="gelu").sum().backward()
+    assert torch.equal(r.grad, torch.ones_like(r))
+
+
 def test_second_derivatives_are_refused():
     x, w = torch.randn((4, 8), device="cuda", requires_grad=True), torch.randn((6, 8), device="cuda", requires_grad=True)
     g, = torch.autograd.grad(blocks.linear_rows(x, w, act="silu").sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+    y, h = blocks.join_rows(x, x, pre=blocks.Norm("rmsnorm"))
+    g, = torch.autograd.grad((y * h).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        (g.sum() + x.sum()).backward()
