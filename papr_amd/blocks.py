@@ -12,6 +12,7 @@ several streams and in several captured graphs do not share any.  Second derivat
 """
 import collections
 import ctypes as C
+import math
 
 import torch
 
@@ -85,7 +86,28 @@ class PackedRows:
 
     def rows(self):
         """The values they stand for, in the type and shape that was packed."""
-        return _done("papr_rows8_unpack", (_native or _load()).unpack(self.codes, self.exps, KEEPS[self.fmt], TYPES[self.dtype], self.shape))
+        try:
+            x = (_native or _load()).unpack(self.codes, self.exps, KEEPS.get(self.fmt, 0), TYPES.get(self.dtype, -1), self.shape)
+        except TypeError:
+            x = None
+        if x is None:
+            self._explain()
+        return _done("papr_rows8_unpack", x)
+
+    def _explain(self):
+        who, shape = "PackedRows.rows", tuple(self.shape)
+        if self.fmt not in KEEPS:
+            _fail(who, "unknown format %r (%s)" % (self.fmt, ", ".join(KEEPS)))
+        if self.dtype not in TYPES:
+            _fail(who, "type %s (float32, float16, bfloat16)" % (self.dtype,))
+        if not shape or shape[-1] < 1:
+            _fail(who, "shape %s: rows of at least one column" % (shape,))
+        rows, blocks = math.prod(shape[:-1]), (shape[-1] + BLOCK - 1) // BLOCK
+        for name, t, want in (("codes", self.codes, (rows, blocks * BLOCK)), ("exps", self.exps, (rows, blocks))):
+            if not torch.is_tensor(t) or t.dtype != torch.uint8 or tuple(t.shape) != want:
+                _fail(who, "%s of rows %s are uint8 %s" % (name, shape, want))
+        _check_device(who, self.codes, self.exps)
+        _fail(who, "arguments that do not fit")
 
 
 def pack_rows(x, fmt="e4m3"):

@@ -89,11 +89,38 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
 Tensor fresh(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().requires_grad(false)); }
 Tensor bytes_like(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kByte).requires_grad(false)); }
-SavedVariable keep(const Tensor& t) { return t.defined() ? SavedVariable(t, false) : SavedVariable(); }
-SavedVariable keep(const Maybe& t) { return keep(t ? *t : Tensor()); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const Maybe& t) { return t && t->requires_grad(); }
 Tensor or_none(const Maybe& t) { return t ? *t : Tensor(); }
+
+// A tensor kept for the backward pass.  Hooks of saved tensors (moved to host memory and back, recomputed) may bring back another tensor: it has to be of the same
+// sizes, type and device, and its strides are seen to again.
+class Kept {
+    SavedVariable saved;
+    at::DimVector sizes;
+    at::ScalarType type = at::kByte;
+    at::Device device = at::kCPU;
+
+    Tensor checked() const {
+        Tensor t = saved.unpack();
+        TORCH_CHECK(!t.defined() || (t.sizes() == at::IntArrayRef(sizes) && t.scalar_type() == type && t.device() == device), "papr_amd: a saved tensor came back as ",
+                    t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", was ", type, " ", at::IntArrayRef(sizes), " on ", device);
+        return t.defined() ? untracked(t) : t;
+    }
+
+   public:
+    void hold(const Tensor& t) {
+        if (!t.defined()) return;
+        saved = SavedVariable(t, false);
+        sizes.assign(t.sizes().begin(), t.sizes().end());
+        type = t.scalar_type();
+        device = t.device();
+    }
+    void hold(const Maybe& t) { if (t) hold(*t); }
+    void release() { saved.reset_data(); }
+    Tensor rows() const { Tensor t = checked(); return t.defined() ? rows_of(t, sizes.back()) : t; }
+    Tensor dense() const { Tensor t = checked(); return t.defined() ? t.contiguous() : t; }
+};
 
 // gradients of which no derivative exists: using one in a graph raises there
 variable_list last_of_their_kind(variable_list grads, const char* who) {
@@ -122,26 +149,34 @@ py::object pack(const Tensor& x, int fmt) {
     return py::make_tuple(p.first, p.second);
 }
 
-Tensor unpack(const Tensor& codes, const Tensor& exps, int fmt, int type, std::vector<int64_t> shape) {
+py::object unpack(const Tensor& codes, const Tensor& exps, int fmt, int type, std::vector<int64_t> shape) {
     const at::ScalarType types[3] = {at::kFloat, at::kHalf, at::kBFloat16};
-    Tensor out = at::empty(shape, codes.options().dtype(types[type]));
+    if (fmt < 1 || type < 0 || type > 2 || shape.empty() || shape.back() < 1 || shape.back() > INT32_MAX) return py::none();
+    int64_t n = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
+    const int64_t blocks = (shape.back() + 31) / 32;
+    if (!codes.is_cuda() || exps.device() != codes.device() || codes.scalar_type() != at::kByte || exps.scalar_type() != at::kByte) return py::none();
+    if (codes.sizes() != at::IntArrayRef({n, blocks * 32}) || exps.sizes() != at::IntArrayRef({n, blocks})) return py::none();
+    Tensor c = codes.contiguous(), e = exps.contiguous();
+    if ((uintptr_t)ptr(c) & 7) c = c.clone();
+    Tensor out = at::empty(shape, c.options().dtype(types[type]));
     On on(out);
-    check(papr_rows8_unpack_(type, fmt, ptr(codes), ptr(exps), codes.size(0), (int32_t)shape.back(), ptr(out), on.stream), "papr_rows8_unpack");
-    return out;
+    check(papr_rows8_unpack_(type, fmt, ptr(c), ptr(e), n, (int32_t)shape.back(), ptr(out), on.stream), "papr_rows8_unpack");
+    return py::cast(out);
 }
 
 // ------------------------------------------------------------------------------------------ linear layers
 struct LinearBackward : Node {
     papr_linear_desc d{};
-    SavedVariable held, exps, weight, z;
+    Kept held, exps, weight, z;
     std::vector<int64_t> x_shape;
 
     std::string name() const override { return "PaprLinearBackward"; }
     void release_variables() override {
-        held.reset_data();
-        exps.reset_data();
-        weight.reset_data();
-        z.reset_data();
+        held.release();
+        exps.release();
+        weight.release();
+        z.release();
     }
     variable_list apply(variable_list&& grads) override {
         const Tensor& d_y = grads[0];
@@ -150,7 +185,8 @@ struct LinearBackward : Node {
         const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1), need_b = task_should_compute_output(2);
         if (task_should_compute_output(3)) out[3] = d_y;
         if (need_x || need_w || need_b) {
-            Tensor h = held.unpack(), e = exps.unpack(), w = weight.unpack(), zz = z.unpack(), g = rows_of(d_y, d.N);
+            Tensor h = d.keep ? held.dense() : held.rows(), e = exps.dense(), w = weight.rows(), zz = z.dense(), g = rows_of(d_y, d.N);
+            On on(g);
             if (need_x) out[0] = fresh(g, x_shape);
             if (need_w) out[1] = fresh(g, {d.N, d.K});
             if (need_b) out[2] = fresh(g, {d.N});
@@ -159,7 +195,6 @@ struct LinearBackward : Node {
                     if (out[i].defined()) out[i].zero_();
             } else {
                 Tensor ws = bytes_like(g, {(int64_t)papr_linear_bwd_workspace_bytes_(&d) + 16});
-                On on(g);
                 check(papr_linear_bwd_(&d, ptr(g), ld_of(g), ptr(zz), need_w ? ptr(h) : nullptr, h.defined() ? ld_of(h) : 0, ptr(e), need_x ? ptr(w) : nullptr,
                                        w.defined() ? ld_of(w) : 0, ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(ws), on.stream), "papr_linear_bwd");
             }
@@ -194,10 +229,10 @@ py::object linear(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe&
     auto shape = x.sizes().vec();                  // (outputs in their final shape: contiguous, so the same rows)
     shape.back() = N;
     Tensor y = fresh(rows, shape), z = slopes ? fresh(rows, {d.M, N}) : Tensor();
-    const size_t aside = papr_linear_fwd_workspace_bytes_(&d);
-    Tensor ws = aside ? bytes_like(rows, {(int64_t)aside}) : Tensor();
     {
-        On on(rows);
+        On on(rows);                               // (the workspace's size is the device's)
+        const size_t aside = papr_linear_fwd_workspace_bytes_(&d);
+        Tensor ws = aside ? bytes_like(rows, {(int64_t)aside}) : Tensor();
         check(papr_linear_fwd_(&d, ptr(rows), ld_of(rows), ptr(w2), ld_of(w2), ptr(b1), ptr(r2), ld_of(r2), ptr(y), ptr(z), ptr(ws), on.stream), "papr_linear_fwd");
     }
     if (tracked) {
@@ -206,13 +241,13 @@ py::object linear(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe&
         if (wants_grad(w)) {
             if (keep_fmt) {
                 auto p = pack_of(rows, keep_fmt);
-                node->held = keep(p.first);
-                node->exps = keep(p.second);
+                node->held.hold(p.first);
+                node->exps.hold(p.second);
                 d.keep = keep_fmt;
-            } else node->held = keep(rows);
+            } else node->held.hold(rows);
         }
-        if (wants_grad(x)) node->weight = keep(w2);
-        node->z = keep(z);
+        if (wants_grad(x)) node->weight.hold(w2);
+        node->z.hold(z);
         node->d = d;
         node->x_shape = x.sizes().vec();
         torch::autograd::set_history(y, node);
@@ -252,26 +287,27 @@ struct Joint {                                     // operands as the library ta
 struct JoinBackward : Node {
     papr_join_desc d{};                            // numbers only: the pointers are set when the saved tensors are back
     bool has_h = false;
-    SavedVariable x, f, gate, stats, params[5];
+    Kept x, f, gate, stats, params[5];
     std::vector<int64_t> shape, gate_shape;
 
     std::string name() const override { return "PaprJoinBackward"; }
     void release_variables() override {
-        x.reset_data();
-        f.reset_data();
-        gate.reset_data();
-        stats.reset_data();
-        for (auto& p : params) p.reset_data();
+        x.release();
+        f.release();
+        gate.release();
+        stats.release();
+        for (auto& p : params) p.release();
     }
     variable_list apply(variable_list&& grads) override {
         variable_list out(8);
         Joint j;
-        auto back = [](const SavedVariable& s) { Tensor t = s.unpack(); return t.defined() ? Maybe(t) : Maybe(); };
-        j.x = x.unpack();
-        j.f = back(f);
-        j.gate = back(gate);
-        for (int i = 0; i < 5; ++i) j.params[i] = back(params[i]);
-        Tensor st = stats.unpack();
+        auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
+        j.x = x.rows();
+        j.f = maybe(f.rows());
+        j.gate = maybe(gate.rows());
+        for (int i = 0; i < 5; ++i) j.params[i] = maybe(params[i].dense());
+        Tensor st = stats.dense();
+        On on(j.x);
         j.d = d;
         j.describe();
         const int64_t rows = j.d.rows, width = j.d.width;
@@ -291,10 +327,7 @@ struct JoinBackward : Node {
             }
         papr_join_grads g = {ptr(out[6]), ptr(out[7]), ptr(out[4]), ptr(out[5]), ptr(out[3])};
         Tensor ws = sums ? bytes_like(j.x, {(int64_t)papr_join_bwd_workspace_bytes_(rows, (int32_t)width) + 16}) : Tensor();
-        {
-            On on(j.x);
-            check(papr_join_bwd_(&j.d, (const float*)ptr(st), ptr(d_y), ptr(d_h), ptr(out[0]), ptr(out[1]), ptr(out[2]), &g, ptr(ws), on.stream), "papr_join_bwd");
-        }
+        check(papr_join_bwd_(&j.d, (const float*)ptr(st), ptr(d_y), ptr(d_h), ptr(out[0]), ptr(out[1]), ptr(out[2]), &g, ptr(ws), on.stream), "papr_join_bwd");
         return last_of_their_kind(std::move(out), "join_rows");
     }
 };
@@ -347,11 +380,11 @@ py::object join(const Tensor& x, const Maybe& f, const Maybe& gate, double scale
                                                                  or_none(pre_shift)));
         node->d = j.d;
         node->has_h = pre_kind >= 0;
-        node->x = keep(j.x);
-        node->f = keep(j.f);
-        node->gate = keep(j.gate);
-        node->stats = keep(stats);
-        for (int i = 0; i < 5; ++i) node->params[i] = keep(j.params[i]);
+        node->x.hold(j.x);
+        node->f.hold(j.f);
+        node->gate.hold(j.gate);
+        node->stats.hold(stats);
+        for (int i = 0; i < 5; ++i) node->params[i].hold(j.params[i]);
         node->shape = x.sizes().vec();
         if (gate) node->gate_shape = gate->sizes().vec();
         if (y.defined()) torch::autograd::set_history(y, node);

@@ -115,7 +115,7 @@ extern "C" int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t
     bool vec = papr_rows_aligned(x, ldx, d->K, b) && papr_rows_aligned(w, ldw, d->K, b);
     Operand A = {x, ldx, d->M, nullptr}, B = {w, ldw, d->N, nullptr};
     if (pads_forward(d)) {
-        PAPR_REQUIRE(workspace, "papr_linear_fwd: the workspace is missing");
+        PAPR_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0, "papr_linear_fwd: the workspace is missing or does not start on 16 bytes");
         const int64_t ld = up8(d->K);
         char* wide_w = (char*)workspace + (size_t)d->M * ld * 2;
         const Rows rows = {(const uint16_t*)x, ldx, d->M, (uint16_t*)workspace}, weight = {(const uint16_t*)w, ldw, d->N, (uint16_t*)wide_w};

@@ -132,3 +132,36 @@ def test_workspaces_grow_with_the_call():
     assert ws(0, 512000) > ws(0, 1000)
     assert L.papr_join_bwd_workspace_bytes(0, 256) == 0
     assert L.papr_join_bwd_workspace_bytes(1, 256) == 5 * 256 * 4
+
+
+def packed(rows=(4, 40), codes=(4, 64), exps=(4, 2), fmt="e4m3", dtype=torch.float32, byte=torch.uint8):
+    return blocks.PackedRows(torch.zeros(codes, dtype=byte), torch.zeros(exps, dtype=byte), fmt, rows, dtype)
+
+
+@pytest.mark.parametrize("p, word", [
+    (packed(codes=(4, 40)), "codes of rows"),
+    (packed(codes=(3, 64)), "codes of rows"),
+    (packed(exps=(4, 1)), "exps of rows"),
+    (packed(byte=torch.int8), "codes of rows"),
+    (packed(rows=(4, 65)), "codes of rows"),
+    (packed(rows=(2, 4, 40)), "codes of rows"),
+    (packed(rows=()), "at least one column"),
+    (packed(fmt="fp8"), "unknown format"),
+    (packed(dtype=torch.float64), "float64"),
+])
+def test_packed_rows_that_do_not_fit_their_shape_are_refused(p, word):
+    with pytest.raises(ValueError, match=word):
+        p.rows()
+
+
+def test_packed_rows_held_on_the_host_are_refused():
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        packed().rows()
+
+
+def test_a_forward_workspace_starts_on_16_bytes():
+    L, p = hip.lib(), C.c_void_p(4096)
+    d = hip.LinearDesc(2, 0, 0, 0, 8192, 1000, 701)       # (its rows are copied into whole vectors)
+    assert L.papr_linear_fwd_workspace_bytes(d) == (8192 + 1000) * 704 * 2
+    for ws in (None, C.c_void_p(4104)):
+        refused(L.papr_linear_fwd(d, p, 701, p, 701, None, None, 0, p, None, ws, None), "16 bytes")

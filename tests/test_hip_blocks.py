@@ -682,3 +682,46 @@ def test_second_derivatives_are_refused():
     g, = torch.autograd.grad((y * h).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         (g.sum() + x.sum()).backward()
+
+
+def test_packed_rows_in_other_strides_and_places():
+    """Codes that moved to host memory and back, lie with gaps between rows, or start on an odd byte stand for the same values."""
+    x = torch.randn((33, 100), generator=gen(1), device="cuda").bfloat16()
+    p = blocks.pack_rows(x, "int8")
+    want, codes, exps = p.rows(), p.codes, p.exps
+    wide = torch.zeros((33, 200), dtype=torch.uint8, device="cuda")
+    wide[:, 3:131] = codes
+    odd = torch.empty(codes.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view_as(codes).copy_(codes)
+    for c, e in ((codes.cpu().cuda(), exps.cpu().cuda()), (wide[:, 3:131], exps.t().contiguous().t()), (odd, exps)):
+        p.codes, p.exps = c, e
+        assert torch.equal(p.rows(), want)
+    p.codes = codes.cpu()
+    with pytest.raises((ValueError, RuntimeError)):
+        p.rows()
+
+
+@pytest.mark.parametrize("keep", [None, "e4m3"])
+def test_saved_tensors_may_leave_the_device_or_be_recomputed(keep):
+    """Hooks of saved tensors and checkpoints bring back what was kept: the same gradients, to the bit, strided and padded rows among them."""
+    from torch.utils.checkpoint import checkpoint
+    p = {n: t.requires_grad_(True) for n, t in block_params(torch.bfloat16, 142, 256, 1).items()}
+    x = torch.randn((37, 160), generator=gen(2), device="cuda").bfloat16()[:, 3:145].requires_grad_(True)
+    cot = [torch.randn((37, 142), generator=gen(3 + i), device="cuda").bfloat16() for i in range(2)]
+    grads = lambda out: torch.autograd.grad(out, [x] + list(p.values()), cot)
+    want = grads(block(p, x, keep))
+    with torch.autograd.graph.save_on_cpu():
+        out = block(p, x, keep)
+    away = grads(out)
+    again = grads(checkpoint(lambda t: block(p, t, keep), x, use_reentrant=False))
+    for other in (away, again):
+        assert all(torch.equal(a, b) for a, b in zip(want, other))
+
+
+@pytest.mark.parametrize("back", [lambda t: t.cpu(), lambda t: t[:-1], lambda t: t.double()], ids=["host", "shorter", "wider type"])
+def test_saved_tensors_that_come_back_as_something_else_are_refused(back):
+    x, w = torch.randn((8, 16), device="cuda"), torch.randn((16, 16), device="cuda", requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+        y, j = blocks.linear_rows(x, w, act="silu"), blocks.join_rows(x, x * w[0])
+    for out in (y, j):
+        with pytest.raises(RuntimeError, match="came back"):
+            out.sum().backward()
