@@ -23,6 +23,26 @@ static inline bool papr_rows_aligned(const void* p, int64_t ld, int64_t width, i
     return ((uintptr_t)p & 15) == 0 && (ld * bytes) % 16 == 0 && (width * bytes) % 16 == 0;
 }
 
+// N elements of a row of which `left` are there (the others zero, or not written).  LOOSE: rows that start anywhere and end inside a vector -- the hardware takes 16 bytes
+// at any address, and the one lane with the row's end takes its elements one by one; otherwise left >= N and the address is the vector's own.
+template <bool LOOSE, typename T, int N>
+__device__ __forceinline__ void papr_get(papr_pack<T, N>& t, const T* p, int left) {
+    if (!LOOSE) t = *reinterpret_cast<const papr_pack<T, N>*>(p);
+    else if (left >= N) __builtin_memcpy(&t, __builtin_assume_aligned(p, sizeof(T)), sizeof(t));
+    else
+#pragma unroll
+        for (int i = 0; i < N; ++i) t.v[i] = i < left ? p[i] : (T)0.f;
+}
+template <bool LOOSE, typename T, int N>
+__device__ __forceinline__ void papr_put(T* p, const papr_pack<T, N>& t, int left) {
+    if (!LOOSE) *reinterpret_cast<papr_pack<T, N>*>(p) = t;
+    else if (left >= N) __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &t, sizeof(t));
+    else
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < left) p[i] = t.v[i];
+}
+
 // 1 / (1 + exp(-z)), hardware exp2 and reciprocal.  EXACT (float32 rows): the exponent's product with log2(e) in two parts, a relative error of a few ulp for every z.
 // Otherwise one product: |z| 2^-24 relative, far below a 16-bit type's rounding, and half the instructions (they are what an epilogue of short sums waits for).
 template <bool EXACT>

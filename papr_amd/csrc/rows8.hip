@@ -26,19 +26,14 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ x,
         const int b = (int)(blk - row * blocks), col = b * 32 + (int)(u & 3) * 8;
         const T* src = x + row * ldx + col;
         float v[8];
-        if (VEC) {
-            constexpr int V = 16 / sizeof(T);
+        constexpr int V = 16 / sizeof(T);
 #pragma unroll
-            for (int c = 0; c < 8 / V; ++c) {
-                papr_pack<T, V> t;
-                const bool in = col + c * V < width;
-                if (in) t = *reinterpret_cast<const papr_pack<T, V>*>(src + c * V);
+        for (int c = 0; c < 8 / V; ++c) {
+            papr_pack<T, V> t;
+            const int left = width - (col + c * V);
+            if (left > 0) papr_get<!VEC>(t, src + c * V, left);
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[c * V + i] = in ? (float)t.v[i] : 0.f;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = col + i < width ? (float)src[i] : 0.f;
+            for (int i = 0; i < V; ++i) v[c * V + i] = left > 0 ? (float)t.v[i] : 0.f;
         }
         float peak = 0.f;
         unsigned bad = 0;
@@ -96,19 +91,14 @@ __global__ __launch_bounds__(256) void unpack_rows_kernel(const uint8_t* __restr
         papr_codes_to_float<FMT>(w.x, scale, v);
         papr_codes_to_float<FMT>(w.y, scale, v + 4);
         T* dst = x + row * width + col;
-        if (VEC) {
-            constexpr int V = 16 / sizeof(T);
+        constexpr int V = 16 / sizeof(T);
 #pragma unroll
-            for (int c = 0; c < 8 / V; ++c) {
-                papr_pack<T, V> t;
+        for (int c = 0; c < 8 / V; ++c) {
+            papr_pack<T, V> t;
+            const int left = width - (col + c * V);
 #pragma unroll
-                for (int i = 0; i < V; ++i) t.v[i] = (T)v[c * V + i];
-                if (col + c * V < width) *reinterpret_cast<papr_pack<T, V>*>(dst + c * V) = t;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (col + i < width) dst[i] = (T)v[i];
+            for (int i = 0; i < V; ++i) t.v[i] = (T)v[c * V + i];
+            if (left > 0) papr_put<!VEC>(dst + c * V, t, left);
         }
     }
 }

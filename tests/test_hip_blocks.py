@@ -474,6 +474,15 @@ def test_join_rows_many_rows_and_leading_dimensions():
 
 
 @pytest.mark.parametrize("dt", DTYPES, ids=ids)
+@pytest.mark.parametrize("width", [4104, 4602, 4601])
+@pytest.mark.parametrize("post, pre, gate, use", [("layernorm", "rmsnorm", "row", (True, True)), (None, "layernorm", "full", (False, True)), ("rmsnorm", "none", "none", (True, True)),
+                                                  ("rmsnorm", "layernorm", "full", (True, False)), ("none", None, "row", (True, True))])
+def test_join_rows_widest_rows_several_a_workgroup(dt, width, post, pre, gate, use):
+    """Rows above 4096 columns (whole vectors, pairs and single values), more of them than workgroups."""
+    check_join(521, width, dt, post, pre, gate, "columns", seed=width, use=use)
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=ids)
 @pytest.mark.parametrize("kind", ["layernorm", "rmsnorm", "none"])
 def test_norm_rows(dt, kind):
     g = gen(3)
