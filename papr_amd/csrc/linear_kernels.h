@@ -392,6 +392,9 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[S::IM][S::IN], sh
     }
 }
 
+// Operands through registers: what the streaming kernel cannot take -- float32 (512,000 x 256 -> 256 forward 545 us, d_x 410, d_W 382: 123 - 176 TFLOP/s for the card's 154 of a
+// float32 library product; 8192 x 4096 x 1024 200), 8-bit rows (d_W of 65,536 x 1024 -> 1024 200 us, 690 TFLOP/s), a wide d_z and short odd rows.  Bound by one stage of
+// loads being on its way and, in float32, by cutting the values apart.
 template <typename T, int LA, int LB, int FA, int FMT, bool VEC, int OUT, typename S>
 __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Operand B, int64_t K, int64_t k_per_part, unsigned tiles_m, unsigned tiles_n, Epilogue ep) {
     typedef Plan<T, LA, LB, FA, FMT, VEC, S> P;
@@ -485,6 +488,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Opera
 // Rows past the operand's end: some row of it (never stored); terms past the part's end: a block of zeros.
 // The fragments of a 16-term step are read under the matrix instructions of the step before, and the stage's one barrier stands between its two steps: in front of
 // it a wave has read all of its stage (whose buffer the requests behind the barrier overwrite), behind it the next stage, requested three stages earlier, is there.
+// What bounds it: the matrix pipe and, for short sums, filling the pipeline and writing the results.  8192^3 in bf16 0.88 - 0.98 ms (1120 - 1250 TFLOP/s; the card's library
+// product 1281), 65,536 x 1024 -> 1024 backward 135 us (1020).
 __device__ const uint4 zero_block[4] = {};
 
 __device__ __forceinline__ void request16(const void* src, unsigned lds) {         // 64 lanes x 16 bytes -> LDS [lds, +1 KB) in lane order
@@ -739,7 +744,7 @@ int launch_few_rows(const Operand& A, const Operand& B, int64_t K, bool vec, con
 }
 
 // The slabs of a sum in parts, V results a lane.  SPREAD: the four waves of a workgroup take a quarter of the parts each (many parts: their loads are a chain), quarters
-// added in order; otherwise a lane adds all parts of its results.
+// added in order; otherwise a lane adds all parts of its results.  Bound by reading the slabs, which mostly still lie in the caches: 8192 x 4096 -> 1024 12 us with its launch.
 template <typename T, int V, bool SPREAD>
 __global__ __launch_bounds__(256) void join_slabs_kernel(const float* __restrict__ slab, int64_t n, int parts, T* __restrict__ out) {
     __shared__ float lds[SPREAD ? 4 : 1][SPREAD ? 64 * V : 1];
@@ -790,7 +795,8 @@ int join_slabs(const float* slab, int64_t n, int parts, T* out, hipStream_t s) {
     return 0;
 }
 
-// d_z = d_y act'(z) in the rows' type (none: d_y as it is, nothing is written) and the column sums of it in float32, one partial row per workgroup.
+// d_z = d_y act'(z) in the rows' type (none: d_y as it is, nothing is written) and the column sums of it in float32, one partial row per workgroup.  Bound by HBM:
+// 512,000 x 256 float32 320 us (4.9 TB/s), 8192 x 4096 bf16 45 (4.5).
 // D: the rows' type, or float32 for a product of few terms (keeps_wide).  A thread holds whole vectors of columns; the threads of a workgroup beyond one row's take further rows.
 template <typename T, typename D, bool VEC>
 __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, int64_t ld, const T* __restrict__ z, int64_t M, int N, int act, int lanes, D* __restrict__ d_z, int64_t ldz,
