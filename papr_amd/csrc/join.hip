@@ -139,6 +139,7 @@ __device__ __forceinline__ void standardise(float (&v)[E], int kind, float eps, 
     for (int i = 0; i < E; ++i) v[i] *= stats[1];
 }
 
+// (four waves a SIMD, the four workgroups a compute unit that join_blocks counts on: with registers for three the last quarter ran alone, 79,282 x 712 float32 315 us for 175)
 template <typename T, int V, int G>
 __global__ __launch_bounds__(G > 256 ? G : 256, 4) void join_fwd_kernel(papr_join_desc d, T* __restrict__ y_out, T* __restrict__ h_out, float* __restrict__ stats_out) {
     typedef Row<T, V, G> R;
