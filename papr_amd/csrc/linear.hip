@@ -33,12 +33,8 @@ SlopeGrid slope_grid(int64_t M, int N, int piece) {
 
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
-// d_z of 16-bit rows is rounded to their type in front of its two products, an error of the gradients' own rounding's size (together 1.4 times it).  Where the products
-// are over in a few microseconds whatever they multiply (2^28 terms: 5 us at a fifth of the matrix pipe's rate) that is not paid for: d_z stays in float32 and the
-// products take it as the sum of two 16-bit values.  (none and relu: d_z is d_y or zero and needs no rounding.)
-bool keeps_wide(const papr_linear_desc* d) {
-    return d->type != PAPR_TYPE_F32 && d->act != PAPR_ACT_NONE && d->act != PAPR_ACT_RELU && (double)d->M * (double)d->N * (double)d->K <= 268435456.0;
-}
+// d_z of 16-bit rows is two values of their type (linear_kernels.h says why), but for none and relu, whose d_z is d_y or zero: exact in one.
+bool is_pair(const papr_linear_desc* d) { return d->type != PAPR_TYPE_F32 && d->act != PAPR_ACT_NONE && d->act != PAPR_ACT_RELU; }
 
 // Rows of 16-bit values whose width is no multiple of eight start anywhere, and the streaming kernels want them on 16 bytes: where a product is long enough, its operands
 // are copied into rows of whole vectors first (zeros behind the end).  20,000 x 701 -> 500 forward: 94 us through registers, 39 streaming, the copies 14.
@@ -50,14 +46,14 @@ bool pads_forward(const papr_linear_desc* d) {
 }
 // the backward pass's two products: what each gains by it, its own copies counted (d_z leaves the slope kernel padded; where there is none, d_y is copied)
 bool pads_rows(const papr_linear_desc* d) {
-    if (d->type == PAPR_TYPE_F32 || keeps_wide(d) || (d->K % 8 == 0 && d->N % 8 == 0)) return false;
+    if (d->type == PAPR_TYPE_F32 || (d->K % 8 == 0 && d->N % 8 == 0)) return false;
     const double copies = (d->K % 8 ? copy_us(d->N, d->K) : 0) + (d->act == PAPR_ACT_NONE && d->N % 8 ? copy_us(d->M, d->N) : 0);
-    return choose(d->M, d->K, d->N, PATH_STREAM, true).us + copies < choose(d->M, d->K, d->N, PATH_REGISTERS, true).us;
+    return choose(d->M, d->K, d->N, path_of(d->type, true, 0, is_pair(d)), true).us + copies < choose(d->M, d->K, d->N, path_of(d->type, false, 0, is_pair(d)), true).us;
 }
 bool pads_weight(const papr_linear_desc* d) {
-    if (d->type == PAPR_TYPE_F32 || keeps_wide(d) || d->keep || (d->K % 8 == 0 && d->N % 8 == 0)) return false;
+    if (d->type == PAPR_TYPE_F32 || d->keep || (d->K % 8 == 0 && d->N % 8 == 0)) return false;
     const double copies = (d->K % 8 ? copy_us(d->M, d->K) : 0) + (d->act == PAPR_ACT_NONE && d->N % 8 ? copy_us(d->M, d->N) : 0);
-    return choose(d->N, d->K, d->M, PATH_STREAM, true).us + copies < choose(d->N, d->K, d->M, PATH_REGISTERS, true).us;
+    return choose(d->N, d->K, d->M, path_of(d->type, true, 0, is_pair(d)), true).us + copies < choose(d->N, d->K, d->M, path_of(d->type, false, 0, is_pair(d)), true).us;
 }
 
 // rows of `width` 16-bit values to rows of up8(width): eight a lane, one or two sets of rows of one width in a launch
@@ -132,12 +128,13 @@ extern "C" int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t
 namespace {
 
 // what the backward pass keeps in its workspace, in this order
-struct Layout { size_t d_z, part, d_y, x, w, slab, total; int64_t ldz; };
+struct Layout { size_t d_z, part, d_y, x, w, slab, total; int64_t ldz, low; };
 Layout layout_of(const papr_linear_desc* d) {
     Layout l = {};
     const bool slope = d->act != PAPR_ACT_NONE, rows = pads_rows(d), weight = pads_weight(d);
     l.ldz = rows || weight ? up8(d->N) : d->N;
-    l.d_z = slope ? up16((size_t)d->M * l.ldz * (keeps_wide(d) ? 4 : papr_type_bytes(d->type))) : 0;
+    l.d_z = slope ? up16((size_t)d->M * l.ldz * papr_type_bytes(d->type)) : 0;
+    if (is_pair(d)) { l.low = (int64_t)l.d_z; l.d_z *= 2; }
     for (int piece = 1; piece <= 8; piece *= 2) {
         const size_t p = up16((size_t)slope_grid(d->M, (int)up8(d->N), piece).blocks * d->N * sizeof(float));
         l.part = p > l.part ? p : l.part;
@@ -172,7 +169,7 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
     PAPR_REQUIRE(!d_w || !d->keep || (ldx == (K + 31) / 32 * 32 && ((uintptr_t)x & 7) == 0), "papr_linear_bwd: kept rows are whole blocks of 32 codes on 8 bytes");
     PAPR_REQUIRE(((uintptr_t)workspace & 15) == 0, "papr_linear_bwd: the workspace starts on 16 bytes");
     const int b = papr_type_bytes(d->type);
-    const bool slope = d->act != PAPR_ACT_NONE, wide = keeps_wide(d);
+    const bool slope = d->act != PAPR_ACT_NONE;
     const Layout l = layout_of(d);
     char* at = reinterpret_cast<char*>(workspace);
     auto take = [&](size_t bytes) { char* p = at; at += bytes; return (void*)p; };
@@ -184,7 +181,7 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
     if (slope || d_b) {
         const bool vec = papr_rows_aligned(d_y, ld_dy, N, b) && ((uintptr_t)z & 15) == 0;
         const SlopeGrid g = slope_grid(M, (int)(vec ? N : up8(N)), vec ? 16 / b : 1);
-        PAPR_TYPE_SWITCH(d->type, rc = slopes<T>(wide, vec, g, d_y, ld_dy, z, M, (int)N, d->act, slope ? dz : nullptr, l.ldz, d_b ? part : nullptr, s));
+        PAPR_TYPE_SWITCH(d->type, rc = slopes<T>(vec, g, d_y, ld_dy, z, M, (int)N, d->act, slope ? dz : nullptr, l.low, l.ldz, d_b ? part : nullptr, s));
         if (rc) return rc;
         if (d_b) {
             papr_colsum_out out = {};
@@ -194,7 +191,7 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
         }
     }
     // d_z as the products take it: from the slope kernel, or d_y itself, copied where its rows have to start on 16 bytes
-    Operand G = {slope ? dz : d_y, slope ? l.ldz : ld_dy, 0, nullptr};
+    Operand G = {slope ? dz : d_y, slope ? l.ldz : ld_dy, 0, nullptr, l.low};
     if (l.d_y && (d_x || d_w)) {
         if ((rc = pad_rows({(const uint16_t*)d_y, ld_dy, M, (uint16_t*)y8}, nullptr, N, s))) return rc;
         G = {y8, l.ldz, 0, nullptr};
@@ -204,7 +201,7 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
     const bool copy_w = d_x && l.w, copy_x = d_w && l.x;
     if (copy_w || copy_x)
         if ((rc = pad_rows(copy_x ? rows : weight, copy_x && copy_w ? &weight : nullptr, K, s))) return rc;
-    const bool vg = papr_rows_aligned(G.p, G.ld, G.ld == l.ldz ? l.ldz : N, wide ? 4 : b);
+    const bool vg = papr_rows_aligned(G.p, G.ld, G.ld == l.ldz ? l.ldz : N, b);
     if (d_x) {
         Operand A = G, B = {w, ldw, K, nullptr};
         A.rows = M;
@@ -213,7 +210,7 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
             B = {w8, up8(K), K, nullptr};
             vec = vg;
         }
-        PAPR_TYPE_SWITCH(d->type, rc = grad_rows<T>(wide, vec, A, B, N, d_x, slab, s));
+        PAPR_TYPE_SWITCH(d->type, rc = grad_rows<T>(vec, A, B, N, d_x, slab, s));
         if (rc) return rc;
     }
     if (d_w) {
@@ -224,7 +221,7 @@ extern "C" int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64
             B = {x8, up8(K), K, nullptr};
             vec = vg;
         }
-        PAPR_TYPE_SWITCH(d->type, rc = grad_weight<T>(wide, d->keep, vec, A, B, M, d_w, slab, s));
+        PAPR_TYPE_SWITCH(d->type, rc = grad_weight<T>(d->keep, vec, A, B, M, d_w, slab, s));
         if (rc) return rc;
     }
     return 0;

@@ -6,8 +6,11 @@
 //   * float32: every value is cut into three bfloat16 parts (8 + 8 + 8 bits, rounded to nearest: exact for every normal number) on its way into LDS, and the six
 //     products of weight 2^-18 and more are summed -- what is left out is below 2^-26 of a term, less than float32's own rounding.  2.5 PFLOP/s / 6 = 416 TFLOP/s
 //     against 157 of the float32 matrix instructions.  Infinities and NaN give NaN (inf - inf), magnitudes above 2^128 (1 - 2^-9) count as infinite.
-//   * d_z is an operand of two products and is kept in the rows' type (rounded once, to nearest; small products of 16-bit rows: in float32, see keeps_wide).  d_b sums it
-//     in float32 before that rounding.
+//   * d_z is an operand of two products.  For 16-bit rows with an activation that bends it (leakyrelu, gelu, silu) it is kept as the sum of two values of the rows' type, high
+//     and low (16 significant bits or more), and both products take both: rounded to one such value it would be an error of the gradients' own rounding's size in each
+//     of them (measured 1.45 times that rounding together, 1.06 so), and a slope up to 1.13 can take it past float16's largest number.  Twice the matrix instructions: 8192 x 1024
+//     -> 4096 in bfloat16, forward and backward, 448 us; with d_z rounded once it was 332.
+//     d_b sums it in float32.
 #pragma once
 #include "linear.h"
 #include <atomic>
@@ -100,17 +103,15 @@ __device__ __forceinline__ s16x4 read_tr4(unsigned a) { return __builtin_amdgcn_
 //   K_RUNS:   image [R][BK] halfs, 16-byte pieces exchanged by the row number so that 16 rows' reads of one piece cover all 64 banks.
 //   ROWS_RUN: image [BK][R + pad] halfs as it lies in memory; the transposing LDS read hands a lane 8 consecutive k of its row.  The row stride is
 //             64 bytes modulo 256: the four k a 16-lane group reads lie on different quarters of the banks.
-// FMT: 0 rows of type T; PAPR_KEEP_* 8-bit rows (ROWS_RUN only); WIDE float32 rows that a 16-bit product takes as the sum of two values of type T.
+// FMT: 0 rows of type T; PAPR_KEEP_* 8-bit rows (ROWS_RUN only); PAIR rows that are the sum of two sets of rows of type T, Operand::low bytes apart.
 // A thread's pieces sit at fixed 32-bit offsets from a uniform tile address that advances with k.
-constexpr int WIDE = 3;
+constexpr int PAIR = 3;
 template <typename T, int LAYOUT, int FMT, bool VEC, int R, int BK, int THREADS>
 struct Tile {
-    static constexpr bool PACKED = FMT == PAPR_KEEP_E4M3 || FMT == PAPR_KEEP_INT8, SPLIT = FMT == WIDE || (sizeof(T) == 4 && FMT == 0);
-    typedef typename std::conditional<FMT == WIDE, float, T>::type Source;
-    typedef typename std::conditional<sizeof(T) == 4, bf16, T>::type Part;
-    static constexpr int PLANES = FMT == WIDE ? 2 : SPLIT ? 3 : 1;
+    static constexpr bool PACKED = FMT == PAPR_KEEP_E4M3 || FMT == PAPR_KEEP_INT8, SPLIT = sizeof(T) == 4 && FMT == 0;
+    static constexpr int SOURCES = FMT == PAIR ? 2 : 1, PLANES = SPLIT ? 3 : SOURCES;
     static constexpr int PIECE = SPLIT ? 4 : 8;                                   // elements of one load
-    static constexpr int BYTES = PACKED ? 1 : sizeof(Source);
+    static constexpr int BYTES = PACKED ? 1 : sizeof(T);
     static constexpr int N = R * BK / PIECE / THREADS;
     static constexpr int STRIDE = LAYOUT == K_RUNS ? BK : (R * 2 % 256 == 64 ? R : R + 32);
     static constexpr int PLANE = (LAYOUT == K_RUNS ? R : BK) * STRIDE;            // halfs
@@ -118,7 +119,7 @@ struct Tile {
     static_assert(R * BK % (PIECE * THREADS) == 0, "whole pieces per thread");
     typedef typename Matrix<T>::frag frag;
 
-    struct Held { uint4 reg[N]; uint8_t ex[PACKED ? N : 1]; };                    // a tile on its way
+    struct Held { uint4 reg[SOURCES][N]; uint8_t ex[PACKED ? N : 1]; };           // a tile on its way
     unsigned off[N];                                                              // bytes from the tile's address
     unsigned exo[PACKED ? N : 1];
     const char* base;                                                             // (uniform) rows r0, the next k
@@ -156,40 +157,44 @@ struct Tile {
     __device__ __forceinline__ void load(Held& h, const Operand& o, int64_t r0, int64_t k0, int64_t K) {
         bool inside = k0 + BK <= K;
         if (LAYOUT == ROWS_RUN && !VEC && !PACKED) inside = k0 + BK < K && o.rows >= PIECE;
-        if (inside) {
 #pragma unroll
-            for (int q = 0; q < N; ++q) {
-                const char* src = base + off[q];
-                if (PACKED) {
-                    const uint2 c = *reinterpret_cast<const uint2*>(src);
-                    h.reg[q].x = c.x; h.reg[q].y = c.y;
-                    h.ex[q] = exb[exo[q]];
-                } else if (VEC) h.reg[q] = *reinterpret_cast<const uint4*>(src);
-                else __builtin_memcpy(&h.reg[q], __builtin_assume_aligned(src, sizeof(Source)), 16);
-            }
-        } else {
+        for (int n = 0; n < SOURCES; ++n) {
+            const char* const at = base + (n ? o.low : 0);
+            if (inside) {
 #pragma unroll
-            for (int q = 0; q < N; ++q) {
-                int r, k;
-                where(q, r, k);
-                const bool in = k0 + k < K;
-                const char* src = in ? base + off[q] : base;                      // (base: rows r0, the tile's first k < K)
-                if (PACKED) {
-                    const uint2 c = *reinterpret_cast<const uint2*>(src);
-                    h.reg[q].x = in ? c.x : 0u; h.reg[q].y = in ? c.y : 0u;
-                    h.ex[q] = exb[in ? exo[q] : 0u];
-                } else if (VEC) {
-                    const uint4 t = *reinterpret_cast<const uint4*>(src);
-                    h.reg[q].x = in ? t.x : 0u; h.reg[q].y = in ? t.y : 0u; h.reg[q].z = in ? t.z : 0u; h.reg[q].w = in ? t.w : 0u;
-                } else {
-                    papr_pack<Source, PIECE> t;
-                    if (LAYOUT == ROWS_RUN && r0 + r >= o.rows) r = 0;
+                for (int q = 0; q < N; ++q) {
+                    const char* src = at + off[q];
+                    if (PACKED) {
+                        const uint2 c = *reinterpret_cast<const uint2*>(src);
+                        h.reg[n][q].x = c.x; h.reg[n][q].y = c.y;
+                        h.ex[q] = exb[exo[q]];
+                    } else if (VEC) h.reg[n][q] = *reinterpret_cast<const uint4*>(src);
+                    else __builtin_memcpy(&h.reg[n][q], __builtin_assume_aligned(src, sizeof(T)), 16);
+                }
+            } else {
 #pragma unroll
-                    for (int i = 0; i < PIECE; ++i) {
-                        const bool ok = LAYOUT == K_RUNS ? k0 + k + i < K : in && r0 + r + i < o.rows;
-                        t.v[i] = ok ? reinterpret_cast<const Source*>(src)[i] : (Source)0.f;
+                for (int q = 0; q < N; ++q) {
+                    int r, k;
+                    where(q, r, k);
+                    const bool in = k0 + k < K;
+                    const char* src = in ? at + off[q] : at;                      // (at: rows r0, the tile's first k < K)
+                    if (PACKED) {
+                        const uint2 c = *reinterpret_cast<const uint2*>(src);
+                        h.reg[n][q].x = in ? c.x : 0u; h.reg[n][q].y = in ? c.y : 0u;
+                        h.ex[q] = exb[in ? exo[q] : 0u];
+                    } else if (VEC) {
+                        const uint4 t = *reinterpret_cast<const uint4*>(src);
+                        h.reg[n][q].x = in ? t.x : 0u; h.reg[n][q].y = in ? t.y : 0u; h.reg[n][q].z = in ? t.z : 0u; h.reg[n][q].w = in ? t.w : 0u;
+                    } else {
+                        papr_pack<T, PIECE> t;
+                        if (LAYOUT == ROWS_RUN && r0 + r >= o.rows) r = 0;
+#pragma unroll
+                        for (int i = 0; i < PIECE; ++i) {
+                            const bool ok = LAYOUT == K_RUNS ? k0 + k + i < K : in && r0 + r + i < o.rows;
+                            t.v[i] = ok ? reinterpret_cast<const T*>(src)[i] : (T)0.f;
+                        }
+                        __builtin_memcpy(&h.reg[n][q], &t, 16);
                     }
-                    __builtin_memcpy(&h.reg[q], &t, 16);
                 }
             }
         }
@@ -206,27 +211,31 @@ struct Tile {
             if constexpr (PACKED) {
                 float v[4], w[4];
                 const float scale = __uint_as_float((unsigned)h.ex[q] << 23);
-                papr_codes_to_float<FMT>(h.reg[q].x, scale, v);
-                papr_codes_to_float<FMT>(h.reg[q].y, scale, w);
+                papr_codes_to_float<FMT>(h.reg[0][q].x, scale, v);
+                papr_codes_to_float<FMT>(h.reg[0][q].y, scale, w);
                 frag to;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) { to[i] = v[i]; to[4 + i] = w[i]; }     // (exact: at most 8 significant bits)
                 *reinterpret_cast<frag*>(lds + at) = to;
             } else if (SPLIT) {
-                const float f[4] = {__uint_as_float(h.reg[q].x), __uint_as_float(h.reg[q].y), __uint_as_float(h.reg[q].z), __uint_as_float(h.reg[q].w)};
-                papr_pack<Part, 4> p[PLANES];
+                const uint4 t = h.reg[0][q];
+                const float f[4] = {__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z), __uint_as_float(t.w)};
+                papr_pack<bf16, 4> p[PLANES];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float rest = f[i];
 #pragma unroll
                     for (int n = 0; n < PLANES; ++n) {
-                        p[n].v[i] = (Part)rest;
+                        p[n].v[i] = (bf16)rest;
                         rest -= (float)p[n].v[i];
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<Part, 4>*>(lds + n * PLANE + at) = p[n];
-            } else *reinterpret_cast<uint4*>(lds + at) = h.reg[q];
+                for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<bf16, 4>*>(lds + n * PLANE + at) = p[n];
+            } else {
+#pragma unroll
+                for (int n = 0; n < SOURCES; ++n) *reinterpret_cast<uint4*>(lds + n * PLANE + at) = h.reg[n][q];
+            }
         }
     }
 
@@ -271,7 +280,7 @@ struct Shape {
 
 template <typename T, int LA, int LB, int FA, int FMT, bool VEC, typename S>
 struct Plan {
-    static constexpr int BK = sizeof(T) == 2 ? 64 : 32, BUFFERS = sizeof(T) == 4 && S::TM > 64 ? 1 : 2;
+    static constexpr int BK = sizeof(T) == 2 ? 64 : 32, BUFFERS = (sizeof(T) == 4 || FA == PAIR) && S::TM > 64 ? 1 : 2;
     typedef Tile<T, LA, FA, VEC, S::TM, BK, S::THREADS> TA;
     typedef Tile<T, LB, FMT, VEC, S::TN, BK, S::THREADS> TB;
     static constexpr int BUF = TA::HALFS + TB::HALFS;
@@ -528,13 +537,13 @@ struct Stage {
         }
         step = (LAYOUT == K_RUNS ? (int64_t)BK : BK * o.ld) * 2;
     }
-    // requests of the next stage; `left`: terms from its first on
-    __device__ __forceinline__ void request(unsigned lds, int64_t left, int wave) {
+    // requests of the next stage; `left`: terms from its first on; `low`: bytes to the rows that are asked for; `last`: the stage behind it takes the next terms
+    __device__ __forceinline__ void request(unsigned lds, int64_t left, int wave, int64_t low, bool last) {
 #pragma unroll
         for (int q = 0; q < N; ++q) {
-            const void* p = k[q] < left ? (const void*)src[q] : (const void*)zero_block;
+            const void* p = k[q] < left ? (const void*)(src[q] + low) : (const void*)zero_block;
             request16(p, lds + (unsigned)(wave * N + q) * LINE);
-            src[q] += step;
+            if (last) src[q] += step;
         }
     }
     // this lane's corner of the fragments (bytes): rows `row` .. + 31, step 0
@@ -568,7 +577,7 @@ struct Stream {
     static constexpr size_t LOOP = (size_t)DEPTH * BYTES, LDS = S::EPI > LOOP ? S::EPI : LOOP;
 };
 
-template <typename T, int LA, int LB, int OUT, typename S>
+template <typename T, int LA, int LB, int FA, int OUT, typename S>
 __global__ __launch_bounds__(S::THREADS, 2) void stream_kernel(Operand A, Operand B, int64_t K, int64_t k_per_part, unsigned tiles_m, unsigned tiles_n, Epilogue ep) {
     typedef Stream<T, LA, LB, S> P;
     typedef typename P::SA SA;
@@ -579,7 +588,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void stream_kernel(Operand A, Operan
     const Place at = place_of(blockIdx.x, gridDim.x, tiles_m, tiles_n);
     const int64_t m0 = (int64_t)at.m * S::TM, n0 = (int64_t)at.n * S::TN;
     const int64_t kb = at.part * k_per_part, ke = kb + k_per_part < K ? kb + k_per_part : K;
-    const int stages = (int)((ke - kb + 31) / 32);
+    constexpr int SETS = FA == PAIR ? 2 : 1;        // (a pair's high and low rows: two stages with the same terms of B)
+    const int stages = (int)((ke - kb + 31) / 32) * SETS;
     const unsigned lds = (unsigned)(size_t)smem;
     f32x16 acc[IM][IN];
 #pragma unroll
@@ -595,9 +605,10 @@ __global__ __launch_bounds__(S::THREADS, 2) void stream_kernel(Operand A, Operan
     int64_t left = ke - kb;
     auto request = [&](int st) {
         const unsigned to = lds + (unsigned)(st % P::DEPTH) * P::BYTES;
-        a.request(to, left, wave);
-        b.request(to + SA::BYTES, left, wave);
-        left -= 32;
+        const int set = SETS == 2 ? st & 1 : 0;
+        a.request(to, left, wave, set ? A.low : 0, set == SETS - 1);
+        b.request(to + SA::BYTES, left, wave, 0, set == SETS - 1);
+        if (set == SETS - 1) left -= 32;
     };
     unsigned ca[IM], cb[IN];
 #pragma unroll
@@ -795,22 +806,27 @@ int join_slabs(const float* slab, int64_t n, int parts, T* out, hipStream_t s) {
     return 0;
 }
 
-// d_z = d_y act'(z) in the rows' type (none: d_y as it is, nothing is written) and the column sums of it in float32, one partial row per workgroup.  Bound by HBM:
-// 512,000 x 256 float32 320 us (4.9 TB/s), 8192 x 4096 bf16 45 (4.5).
-// D: the rows' type, or float32 for a product of few terms (keeps_wide).  A thread holds whole vectors of columns; the threads of a workgroup beyond one row's take further rows.
-template <typename T, typename D, bool VEC>
-__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, int64_t ld, const T* __restrict__ z, int64_t M, int N, int act, int lanes, D* __restrict__ d_z, int64_t ldz,
-                                                    float* __restrict__ part, int64_t rows_per_block) {
+// d_z = d_y act'(z) (none: d_y as it is, nothing is written) and the column sums of it in float32, one partial row per workgroup.  In the rows' type where that is exact
+// (float32; relu: d_y or zero), else SPLIT in two values of it: high = d_z rounded and kept finite, low = what is left, rounded (so an infinity stays one in their sum).  Bound by
+// HBM: 512,000 x 256 float32 320 us (4.9 TB/s), 8192 x 4096 bfloat16 in two values 55 (4.9).
+// A thread holds whole vectors of columns; the threads of a workgroup beyond one row's take further rows.
+template <typename T, bool SPLIT, bool VEC>
+__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, int64_t ld, const T* __restrict__ z, int64_t M, int N, int act, int lanes, T* __restrict__ d_z,
+                                                    T* __restrict__ low, int64_t ldz, float* __restrict__ part, int64_t rows_per_block) {
     constexpr int V = VEC ? 16 / sizeof(T) : 1;
     __shared__ float fold[256 * V];
     const int per = 256 / lanes, cg = threadIdx.x % lanes, rl = threadIdx.x / lanes;
     const int c = (blockIdx.y * lanes + cg) * V;
     const int64_t beg = (int64_t)blockIdx.x * rows_per_block, end = beg + rows_per_block < M ? beg + rows_per_block : M;
+    constexpr float MOST = __is_same(T, f16) ? 65504.f : 3.38953139e38f;
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
     if (d_z && !VEC && c >= N && c < ldz)           // (zeros up to whole vectors)
-        for (int64_t m = beg + rl; m < end; m += per) d_z[m * ldz + c] = (D)0.f;
+        for (int64_t m = beg + rl; m < end; m += per) {
+            d_z[m * ldz + c] = (T)0.f;
+            if (SPLIT) low[m * ldz + c] = (T)0.f;
+        }
     if (c < N)
 #pragma unroll 4
         for (int64_t m = beg + rl; m < end; m += per) {
@@ -821,14 +837,15 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
 #pragma unroll
                 for (int i = 0; i < V; ++i) { v[i] = (float)g.v[i]; zv[i] = (float)t.v[i]; }
                 act_slopes<sizeof(T) == 4>(v, zv, act);
-                struct alignas(16) { D v[V]; } to;
+                papr_pack<T, V> to, rest;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     sum[i] += v[i];
-                    to.v[i] = (D)v[i];
+                    to.v[i] = (T)(SPLIT ? __builtin_amdgcn_fmed3f(v[i], -MOST, MOST) : v[i]);
+                    if (SPLIT) rest.v[i] = (T)(v[i] - (float)to.v[i]);
                 }
-                if constexpr (VEC) *reinterpret_cast<decltype(to)*>(d_z + m * ldz + c) = to;
-                else d_z[m * ldz + c] = to.v[0];
+                *reinterpret_cast<papr_pack<T, V>*>(d_z + m * ldz + c) = to;
+                if (SPLIT) *reinterpret_cast<papr_pack<T, V>*>(low + m * ldz + c) = rest;
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[i] += (float)g.v[i];
@@ -872,18 +889,17 @@ int launch_kernel(const Operand& A, const Operand& B, int64_t K, const Choice& c
 
 template <typename T, int LA, int LB, int FA, int FMT, bool VEC, int OUT, typename S>
 int launch_shape(const Operand& A, const Operand& B, int64_t K, const Choice& c, const Epilogue& ep, hipStream_t s) {
-    if constexpr (sizeof(T) == 2 && FA == 0 && FMT == 0 && VEC && S::TM >= 128)
-        return launch_kernel<stream_kernel<T, LA, LB, OUT, S>, Stream<T, LA, LB, S>::LDS, S>(A, B, K, c, ep, s);
+    if constexpr (sizeof(T) == 2 && FMT == 0 && VEC && S::TM >= 128)
+        return launch_kernel<stream_kernel<T, LA, LB, FA, OUT, S>, Stream<T, LA, LB, S>::LDS, S>(A, B, K, c, ep, s);
     else
         return launch_kernel<product_kernel<T, LA, LB, FA, FMT, VEC, OUT, S>, Plan<T, LA, LB, FA, FMT, VEC, S>::LDS, S>(A, B, K, c, ep, s);
 }
 
 template <typename T, int LA, int LB, int FA, int FMT, bool VEC, int OUT>
 int launch_choice(const Choice& c, const Operand& A, const Operand& B, int64_t K, const Epilogue& ep, hipStream_t s) {
-    if constexpr (FA == 0 && FMT == 0 && VEC)
+    if constexpr (FMT == 0 && VEC)
         if (c.shape == 0) return launch_shape<T, LA, LB, FA, FMT, VEC, OUT, Large>(A, B, K, c, ep, s);
-    if constexpr (FA == 0)
-        if (c.shape <= 1) return launch_shape<T, LA, LB, FA, FMT, VEC, OUT, Middle>(A, B, K, c, ep, s);
+    if (c.shape <= 1) return launch_shape<T, LA, LB, FA, FMT, VEC, OUT, Middle>(A, B, K, c, ep, s);
     return launch_shape<T, LA, LB, FA, FMT, VEC, OUT, Small>(A, B, K, c, ep, s);
 }
 template <typename T, int LA, int LB, int FA, int FMT, int OUT>
@@ -894,7 +910,7 @@ int launch_product(const Choice& c, bool vec, const Operand& A, const Operand& B
 // C = A B^T into contiguous rows of type T, the sum in parts where the tiles alone do not fill the chip
 template <typename T, int LA, int LB, int FA, int FMT>
 int rows_product(bool vec, const Operand& A, const Operand& B, int64_t K, void* out, float* slab, hipStream_t s) {
-    const Choice c = choose(A.rows, B.rows, K, path_of(sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, vec, FMT, FA == WIDE), true);
+    const Choice c = choose(A.rows, B.rows, K, path_of(sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, vec, FMT, FA == PAIR), true);
     Epilogue ep = {};
     if (c.parts == 1) {
         ep.out = out;
@@ -921,28 +937,29 @@ int forward(const Operand& x, const Operand& w, int64_t K, bool vec, const Epilo
 }
 
 template <typename T>
-int grad_rows(bool wide, bool vec, const Operand& d_z, const Operand& w, int64_t N, void* d_x, float* slab, hipStream_t s) {
+int grad_rows(bool vec, const Operand& d_z, const Operand& w, int64_t N, void* d_x, float* slab, hipStream_t s) {
     if constexpr (sizeof(T) == 2)
-        if (wide) return rows_product<T, K_RUNS, ROWS_RUN, WIDE, 0>(vec, d_z, w, N, d_x, slab, s);
+        if (d_z.low) return rows_product<T, K_RUNS, ROWS_RUN, PAIR, 0>(vec, d_z, w, N, d_x, slab, s);
     return rows_product<T, K_RUNS, ROWS_RUN, 0, 0>(vec, d_z, w, N, d_x, slab, s);
 }
 
 template <typename T>
-int grad_weight(bool wide, int keep, bool vec, const Operand& d_z, const Operand& x, int64_t M, void* d_w, float* slab, hipStream_t s) {
+int grad_weight(int keep, bool vec, const Operand& d_z, const Operand& x, int64_t M, void* d_w, float* slab, hipStream_t s) {
     if constexpr (sizeof(T) == 2)
-        if (wide) return weight_product<T, WIDE>(keep, vec, d_z, x, M, d_w, slab, s);
+        if (d_z.low) return weight_product<T, PAIR>(keep, vec, d_z, x, M, d_w, slab, s);
     return weight_product<T, 0>(keep, vec, d_z, x, M, d_w, slab, s);
 }
 
 template <typename T>
-int slopes(bool wide, bool vec, const SlopeGrid& g, const void* d_y, int64_t ld, const void* z, int64_t M, int N, int act, void* d_z, int64_t ldz, float* part, hipStream_t s) {
+int slopes(bool vec, const SlopeGrid& g, const void* d_y, int64_t ld, const void* z, int64_t M, int N, int act, void* d_z, int64_t low, int64_t ldz, float* part, hipStream_t s) {
     const dim3 grid((unsigned)g.blocks, g.cols);
-    if (wide) {
-        if (vec) slope_kernel<T, float, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (float*)d_z, ldz, part, g.rows_per_block);
-        else slope_kernel<T, float, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (float*)d_z, ldz, part, g.rows_per_block);
+    T *high = (T*)d_z, *rest = low ? (T*)((char*)d_z + low) : nullptr;
+    if (low) {
+        if (vec) slope_kernel<T, sizeof(T) == 2, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
+        else slope_kernel<T, sizeof(T) == 2, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
     } else {
-        if (vec) slope_kernel<T, T, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (T*)d_z, ldz, part, g.rows_per_block);
-        else slope_kernel<T, T, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, (T*)d_z, ldz, part, g.rows_per_block);
+        if (vec) slope_kernel<T, false, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
+        else slope_kernel<T, false, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
     }
     PAPR_CHECK_LAUNCH("papr_linear_bwd");
     return 0;
@@ -954,7 +971,7 @@ int slopes(bool wide, bool vec, const SlopeGrid& g, const void* d_y, int64_t ld,
 #define PAPR_LINEAR_INSTANCES(T)                                                                                                                                    \
     namespace papr_linear {                                                                                                                                         \
     template int forward<T>(const Operand&, const Operand&, int64_t, bool, const Epilogue&, hipStream_t);                                                           \
-    template int grad_rows<T>(bool, bool, const Operand&, const Operand&, int64_t, void*, float*, hipStream_t);                                                     \
-    template int grad_weight<T>(bool, int, bool, const Operand&, const Operand&, int64_t, void*, float*, hipStream_t);                                              \
-    template int slopes<T>(bool, bool, const SlopeGrid&, const void*, int64_t, const void*, int64_t, int, int, void*, int64_t, float*, hipStream_t);                \
+    template int grad_rows<T>(bool, const Operand&, const Operand&, int64_t, void*, float*, hipStream_t);                                                           \
+    template int grad_weight<T>(int, bool, const Operand&, const Operand&, int64_t, void*, float*, hipStream_t);                                                    \
+    template int slopes<T>(bool, const SlopeGrid&, const void*, int64_t, const void*, int64_t, int, int, void*, int64_t, int64_t, float*, hipStream_t);              \
     }
