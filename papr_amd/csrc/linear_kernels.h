@@ -24,6 +24,8 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 namespace papr_linear {
 
+template <typename T> __device__ __forceinline__ float largest() { return __is_same(T, f16) ? 65504.f : 3.38953139e38f; }      // of the 16-bit types
+
 // Phi(z) and phi(z) of the erf form of gelu.  float32 rows: the library's erf and exp.  16-bit rows: erfc(x) = t (a1 + ... + a5 t^4) exp(-x^2), t = 1 / (1 + p x)
 // (Abramowitz and Stegun 7.1.26, 1.5e-7 absolute), a sixteenth of the rows' own rounding and a third of erf's instructions: erf in the epilogue of an
 // 8192 x 1024 -> 4096 layer took longer than its matrix instructions.
@@ -293,6 +295,14 @@ __device__ __forceinline__ void put(T* to, const papr_pack<T, E>& t) {
     if (LOOSE) __builtin_memcpy(to, &t, sizeof(t));
     else *reinterpret_cast<papr_pack<T, E>*>(to) = t;
 }
+// z as 16-bit rows hold it: beyond their largest number that number (the slopes there are the activations' limits, 0 and 1, where those of an infinity are 0 times
+// infinity); NaN stays
+template <typename T>
+__device__ __forceinline__ float kept_finite(float z) {
+    if (sizeof(T) == 4) return z;
+    const float most = largest<T>();
+    return z == z ? __builtin_amdgcn_fmed3f(z, -most, most) : z;
+}
 template <typename T, int OUT, int E, bool LOOSE>
 __device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int64_t N, const float (&bias)[E], const papr_pack<T, E>& res, const Epilogue& ep) {
     if (OUT == OUT_FORWARD) {
@@ -301,7 +311,7 @@ __device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int6
         if (ep.z) {
             papr_pack<T, E> t;
 #pragma unroll
-            for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
+            for (int i = 0; i < E; ++i) t.v[i] = (T)kept_finite<T>(v[i]);
             put<T, E, LOOSE>(reinterpret_cast<T*>(ep.z) + m * N + n, t);
         }
         act_values<sizeof(T) == 4>(v, ep.act);
@@ -818,7 +828,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
     const int per = 256 / lanes, cg = threadIdx.x % lanes, rl = threadIdx.x / lanes;
     const int c = (blockIdx.y * lanes + cg) * V;
     const int64_t beg = (int64_t)blockIdx.x * rows_per_block, end = beg + rows_per_block < M ? beg + rows_per_block : M;
-    constexpr float MOST = __is_same(T, f16) ? 65504.f : 3.38953139e38f;
+    const float most = largest<T>();
     float sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
@@ -841,7 +851,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     sum[i] += v[i];
-                    to.v[i] = (T)(SPLIT ? __builtin_amdgcn_fmed3f(v[i], -MOST, MOST) : v[i]);
+                    to.v[i] = (T)(SPLIT ? __builtin_amdgcn_fmed3f(v[i], -most, most) : v[i]);
                     if (SPLIT) rest.v[i] = (T)(v[i] - (float)to.v[i]);
                 }
                 *reinterpret_cast<papr_pack<T, V>*>(d_z + m * ldz + c) = to;

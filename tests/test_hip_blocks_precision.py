@@ -114,3 +114,43 @@ def test_gradients_that_are_not_finite_stay_in_their_row_and_column(dt, M, N, K)
             v = x.detach().double() @ w.detach().double().t() + b.double()
             slope = act64(v, "silu")[1][7, 5]
             assert torch.equal(d_x[7].double(), (bad * slope) * w.detach()[5].double()) and torch.equal(d_w[5].double(), (bad * slope) * x.detach()[7].double())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "leakyrelu", "relu"])
+@pytest.mark.parametrize("M, N, K", [(1, 64, 64), (20, 40, 33), (50, 37, 16), (300, 128, 64), (4096, 512, 256), (3001, 519, 261)])
+def test_an_activation_s_argument_beyond_float16_has_the_slope_of_its_limit(act, M, N, K):
+    """A third of the columns of z are at 76,800, a third at -76,800 (float16 ends at 65,504): y is 76,800 -> infinite or zero, the slopes are 1 and 0 (leakyrelu: 1 and 0.2), and
+    the gradients finite.  The other third: silu's and gelu's slopes move by 0.8 u |z|."""
+    dt, u = torch.float16, unit(torch.float16)
+    x, w, b, _, d_y = linear_data(M, N, K, dt, seed=M % 71, res=False)
+    x[:, 0] = 256.0
+    w[:, 0] = torch.tensor([300.0, -300.0, 0.0], device="cuda").repeat((N + 2) // 3)[:N]
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = blocks.linear_rows(x, w, b, act=act)
+    d_x, d_w, d_b = torch.autograd.grad(y, leaves, d_y)
+    x6, w6, g6 = (t.detach().double() for t in (x, w, d_y))
+    z = x6 @ w6.t() + b.detach().double()
+    v, slope = act64(z, act)
+    S = x6.abs() @ w6.abs().t() + b.detach().double().abs()
+    assert torch.isposinf(y[:, ::3]).all() and not torch.isnan(y).any()
+    near = z.abs() < 100                         # (elsewhere the slope is constant to 2^-50)
+    keeps = (z.abs() > (K + 16) * E32 * S + u * z.abs() + 2.0 ** -24) if act in ("relu", "leakyrelu") else torch.ones_like(near)      # (where z's rounding moves no step of the slope)
+    d_z = g6 * slope
+    err_f = torch.where(near, (0.8 if act in ("silu", "gelu") else 0.0) * (u * z.abs() + (K + 16) * E32 * S), 0.0) * g6.abs() + 16 * E32 * (d_z.abs() + g6.abs()) + (~keeps) * g6.abs()
+    err_d = err_f + u * u * d_z.abs() + tiny(dt)
+    ref = d_z @ w6
+    close(d_x, ref, u * ref.abs() + err_d @ w6.abs() + (2 * N + 16) * E32 * (d_z.abs() @ w6.abs()) + tiny(dt), "d_x")
+    ref = d_z.t() @ x6
+    close(d_w, ref, u * ref.abs() + err_d.t() @ x6.abs() + (2 * M + 16) * E32 * (d_z.abs().t() @ x6.abs()) + tiny(dt), "d_w")
+    ref = d_z.sum(0)
+    close(d_b, ref, u * ref.abs() + err_f.sum(0) + (M + 16) * E32 * d_z.abs().sum(0) + tiny(dt), "d_b")
+
+
+def test_an_activation_s_argument_that_is_nan_stays_one():
+    x, w, b, _, d_y = linear_data(40, 24, 16, torch.float16, seed=1, res=False)
+    x[3, 2] = math.nan
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = blocks.linear_rows(x, w, b, act="silu")
+    d_x, _, d_b = torch.autograd.grad(y, leaves, d_y)
+    at = torch.arange(40, device="cuda") != 3
+    assert torch.isnan(y[3]).all() and torch.isnan(d_x[3]).all() and torch.isnan(d_b).all() and torch.isfinite(d_x[at]).all() and torch.isfinite(y[at]).all()
