@@ -154,3 +154,22 @@ def test_an_activation_s_argument_that_is_nan_stays_one():
     d_x, _, d_b = torch.autograd.grad(y, leaves, d_y)
     at = torch.arange(40, device="cuda") != 3
     assert torch.isnan(y[3]).all() and torch.isnan(d_x[3]).all() and torch.isnan(d_b).all() and torch.isfinite(d_x[at]).all() and torch.isfinite(y[at]).all()
+
+
+@pytest.mark.parametrize("dt", HALVES, ids=ids)
+@pytest.mark.parametrize("M", [20, 700])
+def test_gelu_s_tail_is_as_exact_as_its_middle(dt, M):
+    """z exact (one term, a weight of one), no bias, no residual: y is gelu(z) rounded once.  Beside that: the erfc form's 6.4e-7 and its float32 steps (48 e together), and the
+    exponent z^2 / 2, five roundings, each e of it."""
+    x = torch.linspace(-9.0 if dt == torch.float16 else -13.0, 6.0, M, device="cuda", dtype=torch.float64).to(dt)[:, None]
+    w = torch.ones((24, 1), device="cuda", dtype=dt)
+    x.requires_grad_(True)
+    y = blocks.linear_rows(x, w, act="gelu")
+    d_x, = torch.autograd.grad(y[:, :1], x, torch.ones_like(x))
+    z = x.detach().double()
+    cdf, pdf = 0.5 * torch.erfc(-z / math.sqrt(2)), torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    rel = (2.5 * z * z + 48) * E32
+    ref = z * cdf
+    close(y, ref.expand(M, 24), (unit(dt) * ref.abs() + rel * ref.abs() + tiny(dt)).expand(M, 24), "y")
+    ref = cdf + z * pdf
+    close(d_x, ref, unit(dt) * ref.abs() + rel * (cdf + z.abs() * pdf) + tiny(dt), "d_x")
