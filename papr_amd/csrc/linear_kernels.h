@@ -3,9 +3,11 @@
 // x (M, K), W (N, K) in float32, float16 or bfloat16; sums in float32.  One kernel, C(m, n) = sum_k A(m, k) B(n, k), serves the three products; an operand
 // lies with k contiguous (x and W forward, d_z in d_x) or with its rows contiguous (W in d_x, both in d_W), or it is a set of 8-bit rows (rows8.hip: d_W).
 //   * float16 / bfloat16: the values themselves are the matrix operands.
-//   * float32: every value is cut into three bfloat16 parts (8 + 8 + 8 bits, rounded to nearest: exact for every normal number) on its way into LDS, and the six
-//     products of weight 2^-18 and more are summed -- what is left out is below 2^-26 of a term, less than float32's own rounding.  2.5 PFLOP/s / 6 = 416 TFLOP/s
-//     against 157 of the float32 matrix instructions.  Infinities and NaN give NaN (inf - inf), magnitudes above 2^128 (1 - 2^-9) count as infinite.
+//   * float32: every value is cut into three bfloat16 parts (8 + 8 + 8 bits, rounded to nearest, the first kept finite: exact for every magnitude of 2^-109 and more, below that
+//     off by 2^-134 at most, bfloat16's smallest half step) on its way into LDS, and six of the nine products are summed.  The parts are at most 1, 2^-8 and 2^-17 of a value, so
+//     what is left out (second times third, twice, and third times third) is at most 2^-24 of a term: float32's own rounding.  Summed from the small products up, so that
+//     a value near the largest number is itself again before anything is added to its first part (2^128 - 2^120 here, 2^128 with the second).
+//     2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the float32 matrix instructions.  Infinities and NaN give NaN (inf - inf).
 //   * d_z is an operand of two products.  For 16-bit rows with an activation that bends it (leakyrelu, gelu, silu) it is kept as the sum of two values of the rows' type, high
 //     and low (16 significant bits or more), and both products take both: rounded to one such value it would be an error of the gradients' own rounding's size in each
 //     of them (measured 1.45 times that rounding together, 1.06 so), and a slope up to 1.13 can take it past float16's largest number.  Twice the matrix instructions: 8192 x 1024
@@ -91,6 +93,16 @@ __device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], i
             g[i] *= p * __builtin_fmaf(z[i], 1.f - p, 1.f);
         }
     }
+}
+
+// a float32 value in three bfloat16 parts
+__device__ __forceinline__ void cut_float(float v, bf16 (&part)[3]) {
+    const float most = largest<bf16>();
+    part[0] = (bf16)__builtin_amdgcn_fmed3f(v, -most, most);
+    v -= (float)part[0];
+    part[1] = (bf16)v;
+    v -= (float)part[1];
+    part[2] = (bf16)v;
 }
 
 enum { K_RUNS = 0, ROWS_RUN = 1 };                // which index of an operand is contiguous in memory
@@ -230,12 +242,10 @@ struct Tile {
                 papr_pack<bf16, 4> p[PLANES];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float rest = f[i];
+                    bf16 cut[3];
+                    cut_float(f[i], cut);
 #pragma unroll
-                    for (int n = 0; n < PLANES; ++n) {
-                        p[n].v[i] = (bf16)rest;
-                        rest -= (float)p[n].v[i];
-                    }
+                    for (int n = 0; n < PLANES; ++n) p[n].v[i] = cut[n];
                 }
 #pragma unroll
                 for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<bf16, 4>*>(lds + n * PLANE + at) = p[n];
@@ -470,14 +480,16 @@ __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Opera
 #pragma unroll
                 for (int j = 0; j < IN; ++j) fb[p][j] = TB::read(lb, p, (wn * IN + j) * 32, ks);
 #pragma unroll
-            for (int p = 0; p < TA::PLANES; ++p)
+            for (int w = 2; w >= 0; --w)          // (the parts' products in order of weight, smallest first; those of weight 2^-25 are left out)
 #pragma unroll
-                for (int q = 0; q < TB::PLANES; ++q)
-                    if (p + q < 3)                // (the parts' products below 2^-26 are left out)
+                for (int p = 0; p < TA::PLANES; ++p)
 #pragma unroll
-                        for (int i = 0; i < IM; ++i)
+                    for (int q = 0; q < TB::PLANES; ++q)
+                        if (p + q == w)
 #pragma unroll
-                            for (int j = 0; j < IN; ++j) acc[i][j] = mfma(fa[p][i], fb[q][j], acc[i][j]);
+                            for (int i = 0; i < IM; ++i)
+#pragma unroll
+                                for (int j = 0; j < IN; ++j) acc[i][j] = mfma(fa[p][i], fb[q][j], acc[i][j]);
         }
     };
     load(kb);
@@ -693,10 +705,9 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand
         for (int i = 0; i < 8; ++i) {
             if constexpr (PARTS == 1) f[0][i] = v.t.v[i];
             else {
-                f[0][i] = (bf16)v.t.v[i];
-                const float rest = v.t.v[i] - (float)f[0][i];
-                f[1][i] = (bf16)rest;
-                f[2][i] = (bf16)(rest - (float)f[1][i]);
+                bf16 cut[3];
+                cut_float(v.t.v[i], cut);
+                f[0][i] = cut[0]; f[1][i] = cut[1]; f[2][i] = cut[2];
             }
         }
     };
@@ -722,13 +733,15 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand
                 frag xf[PARTS];
                 parts(xf, xv[a][t]);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
+                for (int w = 2; w >= 0; --w)
 #pragma unroll
-                    for (int q = 0; q < PARTS; ++q)
-                        if (p + q < 3) {
+                    for (int p = 0; p < PARTS; ++p) {
+                        const int q = w - p;
+                        if (q >= 0 && q < PARTS) {
                             if constexpr (__is_same(T, f16)) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[p], wf[q], acc[t], 0, 0, 0);
                             else acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[p], wf[q], acc[t], 0, 0, 0);
                         }
+                    }
             }
         }
     }
