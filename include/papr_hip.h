@@ -576,7 +576,7 @@ enum { PAPR_TYPE_F32 = 0, PAPR_TYPE_F16 = 1, PAPR_TYPE_BF16 = 2 };
  * Backward: with d_z = d_y act'(z):  d_x = d_z W (M, K),  d_w = d_z^T x (N, K),  d_b = column sums of d_z (N); each optional (NULL).  d_z of 16-bit rows is held as the sum
  * of two values of their type (none, relu: exact in one).  keep != 0: x is rows kept in 8 bits (papr_rows8_pack; ldx in codes, exps its exponents) and d_w = d_z^T of the
  * values they stand for.  M = 0: the forward call does nothing, the backward call is an error (the gradients are zero: the caller's).
- * float32 rows: infinities give NaN.  workspace: papr_linear_fwd_workspace_bytes(desc) (mostly none: NULL) and
+ * workspace: papr_linear_fwd_workspace_bytes(desc) (mostly none: NULL) and
  * papr_linear_bwd_workspace_bytes(desc) bytes, 16-byte aligned. */
 enum { PAPR_KEEP_ROWS = 0, PAPR_KEEP_E4M3 = 1, PAPR_KEEP_INT8 = 2 };
 #define PAPR_LINEAR_MAX_STRIDE (1 << 22)      /* elements between rows of x, W and d_y; M < 2^31, N and K <= 2^20 */

@@ -7,7 +7,7 @@
 //     off by 2^-134 at most, bfloat16's smallest half step) on its way into LDS, and six of the nine products are summed.  The parts are at most 1, 2^-8 and 2^-17 of a value, so
 //     what is left out (second times third, twice, and third times third) is at most 2^-24 of a term: float32's own rounding.  Summed from the small products up, so that
 //     a value near the largest number is itself again before anything is added to its first part (2^128 - 2^120 here, 2^128 with the second).
-//     2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the float32 matrix instructions.  Infinities and NaN give NaN (inf - inf).
+//     2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the float32 matrix instructions.  An infinity's third part is it.
 //   * d_z is an operand of two products.  For 16-bit rows with an activation that bends it (leakyrelu, gelu, silu) it is kept as the sum of two values of the rows' type, high
 //     and low (16 significant bits or more), and both products take both: rounded to one such value it would be an error of the gradients' own rounding's size in each
 //     of them (measured 1.45 times that rounding together, 1.06 so), and a slope up to 1.13 can take it past float16's largest number.  Twice the matrix instructions: 8192 x 1024
@@ -95,14 +95,30 @@ __device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], i
     }
 }
 
-// a float32 value in three bfloat16 parts
-__device__ __forceinline__ void cut_float(float v, bf16 (&part)[3]) {
+// N float32 values in three bfloat16 parts each.  An infinity is (+-1, 0, +-infinity): its third part meets the other value's first alone, so the result has the sign of their
+// product (and is NaN beside a zero).
+template <int N>
+__device__ __forceinline__ void cut_floats(const float (&f)[N], bf16 (&part)[3][N]) {
     const float most = largest<bf16>();
-    part[0] = (bf16)__builtin_amdgcn_fmed3f(v, -most, most);
-    v -= (float)part[0];
-    part[1] = (bf16)v;
-    v -= (float)part[1];
-    part[2] = (bf16)v;
+    float peak = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float v = f[i];
+        part[0][i] = (bf16)__builtin_amdgcn_fmed3f(v, -most, most);
+        v -= (float)part[0][i];
+        part[1][i] = (bf16)v;
+        v -= (float)part[1][i];
+        part[2][i] = (bf16)v;
+        peak = fmaxf(peak, fabsf(f[i]));
+    }
+    if (__builtin_expect(peak == __builtin_inff(), 0))
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (fabsf(f[i]) == __builtin_inff()) {
+                part[0][i] = (bf16)__builtin_copysignf(1.f, f[i]);
+                part[1][i] = (bf16)0.f;
+                part[2][i] = (bf16)f[i];
+            }
 }
 
 enum { K_RUNS = 0, ROWS_RUN = 1 };                // which index of an operand is contiguous in memory
@@ -239,16 +255,10 @@ struct Tile {
             } else if (SPLIT) {
                 const uint4 t = h.reg[0][q];
                 const float f[4] = {__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z), __uint_as_float(t.w)};
-                papr_pack<bf16, 4> p[PLANES];
+                bf16 cut[3][4];
+                cut_floats(f, cut);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    bf16 cut[3];
-                    cut_float(f[i], cut);
-#pragma unroll
-                    for (int n = 0; n < PLANES; ++n) p[n].v[i] = cut[n];
-                }
-#pragma unroll
-                for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<bf16, 4>*>(lds + n * PLANE + at) = p[n];
+                for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<bf16, 4>*>(lds + n * PLANE + at) = {{cut[n][0], cut[n][1], cut[n][2], cut[n][3]}};
             } else {
 #pragma unroll
                 for (int n = 0; n < SOURCES; ++n) *reinterpret_cast<uint4*>(lds + n * PLANE + at) = h.reg[n][q];
@@ -701,14 +711,14 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand
         }
     };
     auto parts = [&](frag (&f)[PARTS], const Eight& v) __attribute__((always_inline)) {
+        if constexpr (PARTS == 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (PARTS == 1) f[0][i] = v.t.v[i];
-            else {
-                bf16 cut[3];
-                cut_float(v.t.v[i], cut);
-                f[0][i] = cut[0]; f[1][i] = cut[1]; f[2][i] = cut[2];
-            }
+            for (int i = 0; i < 8; ++i) f[0][i] = v.t.v[i];
+        } else {
+            bf16 cut[3][8];
+            cut_floats(v.t.v, cut);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { f[0][i] = cut[0][i]; f[1][i] = cut[1][i]; f[2][i] = cut[2][i]; }
         }
     };
     f32x4 acc[MT];

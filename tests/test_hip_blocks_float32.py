@@ -83,3 +83,31 @@ def test_what_the_six_products_leave_out_is_2_to_the_24th_of_a_term(M, N):
         x, w = torch.full((M, K), v, device="cuda"), torch.full((N, K), v, device="cuda")
         y, ref = blocks.linear_rows(x, w), torch.full((M, N), K * v * v, device="cuda", dtype=torch.float64)
         close(y, ref, (1 + 2.0 ** -9) * 2.0 ** -24 * ref + unit(torch.float32) * ref + (6 * K + 16) * E32 * ref * (0 if K == 1 else 1))
+
+
+def as_defined(got, ref, S, n):
+    """The infinities and NaN of the definition, and finite values within the bound of a sum of n terms."""
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got[torch.isinf(ref)].double(), ref[torch.isinf(ref)])
+    close(got[fine], ref[fine], unit(torch.float32) * ref[fine].abs() + (6 * n + 16) * E32 * S[fine])
+
+
+@pytest.mark.parametrize("M, N, K", SHAPES)
+def test_infinities_are_those_of_the_definition(M, N, K):
+    """Infinite x, W and d_y here and there, some of them meeting (inf inf, inf - inf, inf 0): the sign of every infinite result, and NaN only where the definition has it."""
+    x, w, _, _, d_y = linear_data(M, N, K, torch.float32, seed=6)
+    x[0, 1], x[M // 2, K - 1], x[M - 1, 0] = math.inf, -math.inf, math.inf
+    x[M - 1, K - 2] = -math.inf
+    w[1] *= 1000
+    w[3, 1], w[5, K - 1], w[2, 1] = 0.0, math.inf, -math.inf
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    y = blocks.linear_rows(x, w)
+    x6, w6 = x.detach().double(), w.detach().double()
+    fin = lambda t: t.abs().nan_to_num(0.0, posinf=0.0)
+    as_defined(y, x6 @ w6.t(), fin(x6) @ fin(w6).t(), K)
+    d_y[M // 3, N - 1], d_y[M - 1, 2] = math.inf, -math.inf
+    d_x, d_w = torch.autograd.grad(y, leaves, d_y)
+    g6 = d_y.double()
+    as_defined(d_x, g6 @ w6, fin(g6) @ fin(w6), N)
+    as_defined(d_w, g6.t() @ x6, fin(g6).t() @ fin(x6), M)
+    assert torch.isinf(y).any() and torch.isnan(y).any()
