@@ -3,6 +3,7 @@
 // kernels (25,600 x 117 float32 rows through a joint and back: 190 us of host time around 47 us of device time).  The library's entry points arrive as addresses
 // (bind), so that there is one loaded library in the process.  Arguments that do not fit are answered with None; papr_amd/blocks.py says what is wrong with them.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
@@ -73,6 +74,15 @@ struct On {
     void* stream;
     explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
+
+// These calls work on the operands' memory, once, and know the backward pass alone.  What goes another way would get the wrong answer without a word: a tangent lost.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level*/ 0).defined(); }
+bool has_tangent(const Maybe& t) { return t && has_tangent(*t); }
+template <typename... Operands>
+void refuse_tangents(const char* who, const Operands&... operands) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !(has_tangent(operands) || ...), "papr_amd: ", who,
+                                " has no forward-mode derivative (an operand carries a tangent)");
+}
 
 Tensor untracked(const Tensor& t) { return t.requires_grad() ? t.detach() : t; }
 
@@ -182,6 +192,7 @@ struct LinearBackward : Node {
         const Tensor& d_y = grads[0];
         variable_list out(4);
         if (!d_y.defined()) return out;
+        refuse_tangents("linear_rows", d_y);
         const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1), need_b = task_should_compute_output(2);
         if (task_should_compute_output(3)) out[3] = d_y;
         if (need_x || need_w || need_b) {
@@ -214,6 +225,7 @@ bool linear_fits(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& 
 }
 
 py::object linear(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int act, int keep_fmt) {
+    refuse_tangents("linear_rows", x, w, b, r);
     if (!linear_fits(x, w, b, r, act, keep_fmt)) return py::none();
     const int64_t K = w.size(1), N = w.size(0);
     const bool tracked = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(r));
@@ -313,6 +325,7 @@ struct JoinBackward : Node {
         const int64_t rows = j.d.rows, width = j.d.width;
         Tensor d_y = j.f ? grads[0] : Tensor(), d_h = has_h ? grads.back() : Tensor();
         if (!d_y.defined() && !d_h.defined()) return out;
+        refuse_tangents("join_rows", d_y, d_h);
         auto full = [&](const Tensor& t) { return t.defined() ? untracked(t).reshape({rows, width}).contiguous() : t; };
         d_y = full(d_y);
         d_h = full(d_h);
@@ -337,6 +350,7 @@ bool param_fits(const Maybe& p, const Tensor& x) { return !p || (type_of(*p) >= 
 // pre_kind < 0: no next norm
 py::object join(const Tensor& x, const Maybe& f, const Maybe& gate, double scale, const Maybe& scale_cols, int post_kind, double post_eps, const Maybe& post_gain,
                 const Maybe& post_shift, int pre_kind, double pre_eps, const Maybe& pre_gain, const Maybe& pre_shift, int gate_act) {
+    refuse_tangents(f ? "join_rows" : "norm_rows", x, f, gate, scale_cols, post_gain, post_shift, pre_gain, pre_shift);
     if (!x.is_cuda() || type_of(x) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > PAPR_JOIN_MAX_WIDTH || post_kind < 0 || gate_act < 0 || pre_kind < -1) return py::none();
     const int64_t width = x.size(-1);
     if (width < 2 && (post_kind == PAPR_NORM_LAYER || pre_kind == PAPR_NORM_LAYER)) return py::none();
