@@ -8,7 +8,8 @@
 They are what `FeedForward.forward` of the reference does around its MLP (models/attn.py:111-117: innorm, mlp, outnorm, the residual branch), for rows that are not
 the render path's own: `papr_amd.ops` runs the embedding MLPs as whole chains instead.  All work goes through libpapr_hip.so (include/papr_hip.h: papr_linear_*,
 papr_join_*, papr_rows8_*) on the current stream of the rows' device; there is no CPU form.  The calls and their autograd nodes are native (csrc/blocks_glue.cpp).  Workspaces come from torch's allocator call by call, so calls on
-several streams and in several captured graphs do not share any.  Second derivatives and forward-mode derivatives are not defined and refused.
+several streams and in several captured graphs do not share any.  Second derivatives and forward-mode derivatives are not defined and refused,
+and so are traces (torch.jit.trace, make_fx) and torch.func transforms: the calls are not torch operators.
 """
 import collections
 import ctypes as C

@@ -5,6 +5,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/function.h>
@@ -12,6 +13,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -75,9 +77,28 @@ struct On {
     explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
-// These calls work on the operands' memory, once, and know the backward pass alone.  What goes another way would get the wrong answer without a word: a tangent lost.
+// These calls work on the operands' memory, once, and know the backward pass alone.  What goes another way would get the wrong answer without a word: a tangent lost, a
+// recorded program without the call in it, an operand without memory taken for one that is not there.
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level*/ 0).defined(); }
 bool has_tangent(const Maybe& t) { return t && has_tangent(*t); }
+bool stands_for(const Tensor& t) {                  // another tensor, or none: subclasses with a dispatch of their own (fake, distributed), operands of torch.func transforms
+    return t.defined() && t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                                                   c10::DispatchKey::Functionalize}));
+}
+bool stands_for(const Maybe& t) { return t && stands_for(*t); }
+bool recording() {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    if (torch::jit::tracer::isTracing()) return true;
+    if (!Modes::any_modes_set()) return false;
+    for (auto key : {c10::impl::TorchDispatchModeKey::PROXY, c10::impl::TorchDispatchModeKey::FAKE, c10::impl::TorchDispatchModeKey::FUNCTIONAL})
+        if (Modes::get_mode(key)) return true;
+    return false;
+}
+template <typename... Operands>
+void refuse_recording(const char* who, const Operands&... operands) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!recording(), "papr_amd: ", who, " cannot be traced (torch.jit.trace, make_fx, torch.export): its call is not a torch operator");
+    TORCH_CHECK_NOT_IMPLEMENTED(!(stands_for(operands) || ...), "papr_amd: ", who, " takes plain tensors, not a torch.func transform's or a subclass with a dispatch of its own");
+}
 template <typename... Operands>
 void refuse_tangents(const char* who, const Operands&... operands) {
     TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !(has_tangent(operands) || ...), "papr_amd: ", who,
@@ -154,12 +175,14 @@ std::pair<Tensor, Tensor> pack_of(const Tensor& rows, int fmt) {
 }
 
 py::object pack(const Tensor& x, int fmt) {
+    refuse_recording("pack_rows", x);
     if (!x.is_cuda() || type_of(x) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > INT32_MAX) return py::none();
     auto p = pack_of(rows_of(x, x.size(-1)), fmt);
     return py::make_tuple(p.first, p.second);
 }
 
 py::object unpack(const Tensor& codes, const Tensor& exps, int fmt, int type, std::vector<int64_t> shape) {
+    refuse_recording("PackedRows.rows", codes, exps);
     const at::ScalarType types[3] = {at::kFloat, at::kHalf, at::kBFloat16};
     if (fmt < 1 || type < 0 || type > 2 || shape.empty() || shape.back() < 1 || shape.back() > INT32_MAX) return py::none();
     int64_t n = 1;
@@ -192,6 +215,7 @@ struct LinearBackward : Node {
         const Tensor& d_y = grads[0];
         variable_list out(4);
         if (!d_y.defined()) return out;
+        refuse_recording("linear_rows", d_y);
         refuse_tangents("linear_rows", d_y);
         const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1), need_b = task_should_compute_output(2);
         if (task_should_compute_output(3)) out[3] = d_y;
@@ -225,6 +249,7 @@ bool linear_fits(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& 
 }
 
 py::object linear(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int act, int keep_fmt) {
+    refuse_recording("linear_rows", x, w, b, r);
     refuse_tangents("linear_rows", x, w, b, r);
     if (!linear_fits(x, w, b, r, act, keep_fmt)) return py::none();
     const int64_t K = w.size(1), N = w.size(0);
@@ -325,6 +350,7 @@ struct JoinBackward : Node {
         const int64_t rows = j.d.rows, width = j.d.width;
         Tensor d_y = j.f ? grads[0] : Tensor(), d_h = has_h ? grads.back() : Tensor();
         if (!d_y.defined() && !d_h.defined()) return out;
+        refuse_recording("join_rows", d_y, d_h);
         refuse_tangents("join_rows", d_y, d_h);
         auto full = [&](const Tensor& t) { return t.defined() ? untracked(t).reshape({rows, width}).contiguous() : t; };
         d_y = full(d_y);
@@ -350,7 +376,9 @@ bool param_fits(const Maybe& p, const Tensor& x) { return !p || (type_of(*p) >= 
 // pre_kind < 0: no next norm
 py::object join(const Tensor& x, const Maybe& f, const Maybe& gate, double scale, const Maybe& scale_cols, int post_kind, double post_eps, const Maybe& post_gain,
                 const Maybe& post_shift, int pre_kind, double pre_eps, const Maybe& pre_gain, const Maybe& pre_shift, int gate_act) {
-    refuse_tangents(f ? "join_rows" : "norm_rows", x, f, gate, scale_cols, post_gain, post_shift, pre_gain, pre_shift);
+    const char* who = f ? "join_rows" : "norm_rows";
+    refuse_recording(who, x, f, gate, scale_cols, post_gain, post_shift, pre_gain, pre_shift);
+    refuse_tangents(who, x, f, gate, scale_cols, post_gain, post_shift, pre_gain, pre_shift);
     if (!x.is_cuda() || type_of(x) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > PAPR_JOIN_MAX_WIDTH || post_kind < 0 || gate_act < 0 || pre_kind < -1) return py::none();
     const int64_t width = x.size(-1);
     if (width < 2 && (post_kind == PAPR_NORM_LAYER || pre_kind == PAPR_NORM_LAYER)) return py::none();

@@ -25,3 +25,33 @@ def test_a_tangent_on_an_operand_or_a_gradient_is_refused():
                 torch.autograd.grad(out, [p["w1"]], fwad.make_dual(torch.ones_like(out), torch.ones_like(out)), retain_graph=True)
         assert torch.autograd.grad(h, [p["w1"]], torch.ones_like(h), retain_graph=True)[0].abs().sum() > 0
     torch.autograd.grad([y, h], list(p.values()), [torch.ones_like(y), torch.ones_like(h)])
+
+
+def test_traces_and_transforms_are_refused_and_modes_that_watch_are_not():
+    """(A trace recorded the output's allocation alone: the traced function returned memory as it was.)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    p = block_params(torch.bfloat16, 64, 128, 1)
+    x = torch.randn((8, 64), generator=gen(1), device="cuda").bfloat16()
+    want = block(p, x, None)
+    calls = [lambda t: blocks.linear_rows(t, p["w1"]), lambda t: blocks.norm_rows(t, blocks.Norm("rmsnorm")), lambda t: blocks.join_rows(t, t), lambda t: blocks.pack_rows(t).codes,
+             lambda t: blocks.PackedRows(blocks.pack_rows(x).codes, t, "e4m3", (8, 64), torch.bfloat16).rows()]
+    for i, call in enumerate(calls):
+        t = x if i < 4 else blocks.pack_rows(x).exps
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            torch.jit.trace(call, t)
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            make_fx(call)(t)
+        with pytest.raises(NotImplementedError, match="plain tensors"):
+            torch.func.vmap(call)(t[None].expand(3, *t.shape))
+    with pytest.raises(NotImplementedError, match="plain tensors"):
+        torch.func.grad(lambda t: blocks.linear_rows(t, p["w1"]).float().sum())(x)
+    out = blocks.linear_rows(x.clone().requires_grad_(True), p["w1"])
+    with pytest.raises(NotImplementedError, match="cannot be traced"):
+        make_fx(lambda g: torch.autograd.grad(out, [out.grad_fn.next_functions[0][0].variable], g, retain_graph=True))(torch.ones_like(out))
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    with Watch():
+        assert all(torch.equal(a, b) for a, b in zip(block(p, x, None), want))
