@@ -105,7 +105,8 @@ void refuse_tangents(const char* who, const Operands&... operands) {
                                 " has no forward-mode derivative (an operand carries a tangent)");
 }
 
-Tensor untracked(const Tensor& t) { return t.requires_grad() ? t.detach() : t; }
+// the values in memory (a view that torch negates lazily -- the imaginary part of a conjugate -- holds them with the other sign), outside the graph
+Tensor untracked(const Tensor& t) { return (t.requires_grad() ? t.detach() : t).resolve_neg(); }
 
 // t as (rows, width) with unit column stride and rows that do not overlap; a copy only where its strides ask for one
 Tensor rows_of(const Tensor& given, int64_t width) {

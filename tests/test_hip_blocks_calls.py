@@ -55,3 +55,34 @@ def test_traces_and_transforms_are_refused_and_modes_that_watch_are_not():
             return func(*args, **(kwargs or {}))
     with Watch():
         assert all(torch.equal(a, b) for a, b in zip(block(p, x, None), want))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16], ids=lambda t: str(t)[6:])
+def test_operands_that_torch_negates_lazily(dt):
+    """Imaginary parts of a conjugate are views whose memory holds the values with the other sign: as rows, parameters, codes' source and incoming gradients."""
+    def lazy(t):
+        if dt != torch.float32:
+            return torch._neg_view(-t)
+        v = torch.complex(t, -t).conj().imag
+        assert v.is_neg() and torch.equal(v, t)
+        return v
+    g = gen(3)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dt)
+    x, w, b, q, f, gate, gain, shift, c = r(40, 48), r(64, 48), r(64), r(40, 64), r(40, 48), r(40, 1), r(48), r(48), r(40, 64)
+    names = [x, w, b, q, f, gate, gain, shift]
+
+    def run(flip):
+        leaves = [t.clone().requires_grad_(True) for t in names]
+        X, Wt, Bi, Q, F, G, A, S = [torch._neg_view(-t) for t in leaves] if flip else leaves
+        assert X.is_neg() == flip and A.is_neg() == flip
+        norm = blocks.Norm("rmsnorm", A, S)
+        y = blocks.linear_rows(X, Wt, Bi, Q, act="silu", keep="int8")
+        j, h = blocks.join_rows(X, F, gate=G, scale=A, post=norm, pre=norm)
+        cots = [c, x, f]
+        cots = [lazy(t) for t in cots] if flip else cots
+        grads = torch.autograd.grad([y, j, h], leaves, cots)
+        return [y, j, h, blocks.norm_rows(X, norm), blocks.pack_rows(X).rows()] + list(grads)
+    with torch.no_grad():
+        assert torch.equal(blocks.linear_rows(lazy(x), w), blocks.linear_rows(x, w))
+    for got, want in zip(run(True), run(False)):
+        assert torch.equal(got, want)
