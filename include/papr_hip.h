@@ -565,7 +565,8 @@ int papr_profile_collect(papr_profile_record* out, int cap);
 /* ------------------------------------------------------------------------------------
  * Row blocks (ABI 28): the parts of a residual feed-forward block -- FeedForward.forward of the reference, models/attn.py:111-117, with its
  * `residual_ff` branch, and Linear layers of 16-bit rows -- as calls of their own.  Rows are float32, float16 or bfloat16 (PAPR_TYPE_*), arithmetic and
- * sums float32, every output rounded once.  Row strides are in elements; rows need not be 16-byte aligned (odd widths and strides run on kernels with
+ * sums float32, every output rounded once.  Row strides are in elements and cover the
+ * rows (of more than one); rows need not be 16-byte aligned (odd widths and strides run on kernels with
  * narrower loads).  Sums run in a fixed order: the same bits on every run.  Workspaces are the caller's, their contents irrelevant on entry; two calls
  * that may run at the same time (other streams, captured graphs) need workspaces of their own. */
 enum { PAPR_TYPE_F32 = 0, PAPR_TYPE_F16 = 1, PAPR_TYPE_BF16 = 2 };
@@ -600,7 +601,7 @@ int papr_rows8_unpack(int32_t type, int32_t fmt, const void* codes, const void* 
  * gate: (rows, width), one per row (rows, 1), or absent; a = identity, sigmoid, silu.  y, h (rows, width) contiguous, either may be NULL.
  * stats (rows, 6) floats or NULL: what papr_join_bwd reads.  Backward: d_y, d_h (rows, width) contiguous, one may be NULL; d_x, d_f (rows, width), d_g (like the
  * gate, contiguous) and the parameters' gradients (in the parameters' types; g and each of its members optional).
- * workspace: papr_join_bwd_workspace_bytes(rows, width) bytes where a parameter's gradient is asked for.  width <= PAPR_JOIN_MAX_WIDTH. */
+ * workspace: papr_join_bwd_workspace_bytes(rows, width) bytes, 16-byte aligned, where a parameter's gradient is asked for.  width <= PAPR_JOIN_MAX_WIDTH. */
 enum { PAPR_NORM_NONE = 0, PAPR_NORM_LAYER = 1, PAPR_NORM_RMS = 2 };
 enum { PAPR_GATE_NONE = 0, PAPR_GATE_SIGMOID = 1, PAPR_GATE_SILU = 2 };                       /* gate_act */
 enum { PAPR_GATE_ABSENT = 0, PAPR_GATE_ROW = 1, PAPR_GATE_FULL = 2 };                         /* gate_form */

@@ -616,6 +616,8 @@ int join_check(const papr_join_desc* d, const char* who) {
     PAPR_REQUIRE(d->rows == 0 || d->x, "%s: x is missing", who);
     PAPR_REQUIRE(d->rows == 0 || (d->gate_form != PAPR_GATE_ABSENT) == (d->gate != nullptr), "%s: gate and gate_form disagree", who);
     PAPR_REQUIRE(d->gate_form == PAPR_GATE_ABSENT || d->f || d->rows == 0, "%s: a gate without the block's output f", who);
+    PAPR_REQUIRE(d->rows <= 1 || (d->ldx >= d->width && (!d->f || d->ldf >= d->width) && (!d->gate || d->ldg >= (d->gate_form == PAPR_GATE_FULL ? d->width : 1))),
+                 "%s: row strides %lld, %lld, %lld do not cover the rows", who, (long long)d->ldx, (long long)d->ldf, (long long)d->ldg);
     const papr_block_norm* norms[2] = {&d->post, &d->pre};
     for (const papr_block_norm* n : norms) {
         PAPR_REQUIRE(n->kind >= PAPR_NORM_NONE && n->kind <= PAPR_NORM_RMS, "%s: unknown norm %d", who, n->kind);
@@ -662,6 +664,7 @@ extern "C" int papr_join_fwd(const papr_join_desc* d, void* y, void* h, float* s
     if (d->rows == 0) return 0;
     PAPR_REQUIRE(y || h, "papr_join_fwd: neither y nor h is asked for");
     PAPR_REQUIRE(!y || d->f, "papr_join_fwd: y without the block's output f (it would be x)");
+    PAPR_REQUIRE(((uintptr_t)stats & 3) == 0, "papr_join_fwd: the stats start on 4 bytes");
     const void* rows_out[2] = {y, h};
     const int vec = join_vector(*d, rows_out, 2);
     const int G = lanes_for(d->width);
@@ -693,7 +696,8 @@ extern "C" int papr_join_bwd(const papr_join_desc* d, const float* stats, const 
     }
     PAPR_REQUIRE(!sums || d->rows == 0 || workspace, "papr_join_bwd: parameter gradients need the workspace");
     if (d->rows == 0) return sums ? papr_colsum_reduce(nullptr, 0, d->width, 5, out, as_stream(stream)) : 0;
-    PAPR_REQUIRE(stats, "papr_join_bwd: the forward call's stats are missing");
+    PAPR_REQUIRE(stats && ((uintptr_t)stats & 3) == 0, "papr_join_bwd: the forward call's stats are missing or do not start on 4 bytes");
+    PAPR_REQUIRE(!sums || ((uintptr_t)workspace & 15) == 0, "papr_join_bwd: the workspace starts on 16 bytes");
     PAPR_REQUIRE(d_y || d_h, "papr_join_bwd: neither d_y nor d_h is given");
     PAPR_REQUIRE(d->f || (!d_f && !d_g), "papr_join_bwd: gradients of f or its gate without f");
     const void* rows_out[5] = {d_y, d_h, d_x, d_f, d->gate_form == PAPR_GATE_FULL ? d_g : nullptr};

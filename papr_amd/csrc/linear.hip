@@ -107,6 +107,7 @@ extern "C" int papr_linear_fwd(const papr_linear_desc* d, const void* x, int64_t
     PAPR_REQUIRE(x && w && y, "papr_linear_fwd: a pointer is missing");
     PAPR_REQUIRE(stride_ok(ldx, d->K) && stride_ok(ldw, d->K), "papr_linear_fwd: row strides %lld, %lld (%lld .. %d)", (long long)ldx, (long long)ldw, (long long)d->K,
                  PAPR_LINEAR_MAX_STRIDE);
+    PAPR_REQUIRE(!res || d->M == 1 || ld_res >= d->N, "papr_linear_fwd: the residual's row stride %lld does not cover %lld columns", (long long)ld_res, (long long)d->N);
     const int b = papr_type_bytes(d->type);
     bool vec = papr_rows_aligned(x, ldx, d->K, b) && papr_rows_aligned(w, ldw, d->K, b);
     Operand A = {x, ldx, d->M, nullptr}, B = {w, ldw, d->N, nullptr};

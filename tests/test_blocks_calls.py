@@ -64,3 +64,22 @@ def test_tensors_that_stand_for_others_are_refused(call):
         call(lambda t: mode.from_tensor(t))
     with pytest.raises((NotImplementedError, RuntimeError, ValueError)):
         call(lambda t: t.to("meta"))
+
+
+def test_c_entry_points_refuse_strides_and_workspaces_that_do_not_fit():
+    import ctypes as C
+    from papr_amd import hip
+    L, p = hip.lib(), C.c_void_p(4096)                   # (never read: the checks come first)
+    refused = lambda code, word: (code != 0 and word in L.papr_last_error().decode()) or pytest.fail("%d %r" % (code, L.papr_last_error()))
+    none, rms = hip.BlockNorm(0, 0, 0.0, 0, None, None), hip.BlockNorm(2, 0, 1e-6, 0, None, None)
+    J = lambda ldx=8, ldf=8, ldg=8, form=2, rows=4, f=4096, gate=4096: hip.JoinDesc(rows, 8, 0, 4096, ldx, f, ldf, gate, ldg, form, 1, None, 0, 1.0, none, rms)
+    grads = hip.JoinGrads(4096, None, None, None, None)
+    for bad in (J(ldx=7), J(ldf=7), J(ldg=7), J(ldx=-8), J(ldg=0, form=1), J(ldx=0, f=None, gate=None, form=0)):
+        refused(L.papr_join_fwd(bad, None, p, None, None), "row strides")
+        refused(L.papr_join_bwd(bad, p, None, p, p, None, None, None, None, None), "row strides")
+    refused(L.papr_join_fwd(J(), None, p, C.c_void_p(4098), None), "4 bytes")
+    refused(L.papr_join_bwd(J(), C.c_void_p(4098), p, p, p, p, None, None, None, None), "4 bytes")
+    refused(L.papr_join_bwd(J(), p, p, p, p, p, None, grads, C.c_void_p(4104), None), "16 bytes")
+    refused(L.papr_rows8_pack(0, 1, p, 7, 4, 8, p, p, None), "row stride")
+    refused(L.papr_rows8_pack(0, 1, p, -8, 4, 8, p, p, None), "row stride")
+    refused(L.papr_linear_fwd(hip.LinearDesc(0, 0, 0, 0, 4, 6, 8), p, 8, p, 8, None, p, 5, p, None, None, None), "residual")
