@@ -592,6 +592,7 @@ int papr_linear_bwd(const papr_linear_desc* d, const void* d_y, int64_t ld_dy, c
 /* Rows kept in 8 bits: 32 columns of a row share a scale 2^e, the smallest (e >= -120) with max|x| <= top 2^e, and hold x / 2^e rounded to nearest even as
  * e4m3 (top 448) or int8 (top 127).  codes (rows, 32 ceil(width / 32)) bytes, padding zero; exps (rows, ceil(width / 32)) bytes = e + 127.  Magnitudes above
  * 1.875 (e4m3) / 1.984375 (int8) times 2^15 (float16) / 2^127 (float32, bfloat16) are kept as that; NaN and infinities come back as NaN. */
+#define PAPR_ROWS8_MAX_WIDTH (1 << 30)        /* columns */
 int papr_rows8_pack(int32_t type, int32_t fmt, const void* x, int64_t ldx, int64_t rows, int32_t width, void* codes, void* exps, papr_stream_t stream);
 int papr_rows8_unpack(int32_t type, int32_t fmt, const void* codes, const void* exps, int64_t rows, int32_t width, void* x, papr_stream_t stream);
 

@@ -103,6 +103,8 @@ class PackedRows:
             _fail(who, "type %s (float32, float16, bfloat16)" % (self.dtype,))
         if not shape or shape[-1] < 1:
             _fail(who, "shape %s: rows of at least one column" % (shape,))
+        if shape[-1] > hip.ROWS8_MAX_WIDTH:
+            _fail(who, "rows of %d columns (at most %d)" % (shape[-1], hip.ROWS8_MAX_WIDTH))
         rows, blocks = math.prod(shape[:-1]), (shape[-1] + BLOCK - 1) // BLOCK
         for name, t, want in (("codes", self.codes, (rows, blocks * BLOCK)), ("exps", self.exps, (rows, blocks))):
             if not torch.is_tensor(t) or t.dtype != torch.uint8 or tuple(t.shape) != want:
@@ -120,6 +122,8 @@ def pack_rows(x, fmt="e4m3"):
         _check_rows("pack_rows", "x", x)
         if fmt not in KEEPS:
             _fail("pack_rows", "unknown format %r (%s)" % (fmt, ", ".join(KEEPS)))
+        if x.shape[-1] > hip.ROWS8_MAX_WIDTH:
+            _fail("pack_rows", "rows of %d columns (at most %d)" % (x.shape[-1], hip.ROWS8_MAX_WIDTH))
         _check_device("pack_rows", x)
     return _done("papr_rows8_pack", PackedRows(packed[0], packed[1], fmt, x.shape, x.dtype))
 

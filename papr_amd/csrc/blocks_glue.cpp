@@ -177,7 +177,7 @@ std::pair<Tensor, Tensor> pack_of(const Tensor& rows, int fmt) {
 
 py::object pack(const Tensor& x, int fmt) {
     refuse_recording("pack_rows", x);
-    if (!x.is_cuda() || type_of(x) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > INT32_MAX) return py::none();
+    if (!x.is_cuda() || type_of(x) < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > PAPR_ROWS8_MAX_WIDTH) return py::none();
     auto p = pack_of(rows_of(x, x.size(-1)), fmt);
     return py::make_tuple(p.first, p.second);
 }
@@ -185,7 +185,7 @@ py::object pack(const Tensor& x, int fmt) {
 py::object unpack(const Tensor& codes, const Tensor& exps, int fmt, int type, std::vector<int64_t> shape) {
     refuse_recording("PackedRows.rows", codes, exps);
     const at::ScalarType types[3] = {at::kFloat, at::kHalf, at::kBFloat16};
-    if (fmt < 1 || type < 0 || type > 2 || shape.empty() || shape.back() < 1 || shape.back() > INT32_MAX) return py::none();
+    if (fmt < 1 || type < 0 || type > 2 || shape.empty() || shape.back() < 1 || shape.back() > PAPR_ROWS8_MAX_WIDTH) return py::none();
     int64_t n = 1;
     for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
     const int64_t blocks = (shape.back() + 31) / 32;

@@ -113,7 +113,7 @@ unsigned rows8_grid(int64_t rows, int blocks) {
 
 extern "C" int papr_rows8_pack(int32_t type, int32_t fmt, const void* x, int64_t ldx, int64_t rows, int32_t width, void* codes, void* exps, papr_stream_t stream) {
     PAPR_REQUIRE(papr_type_ok(type) && (fmt == PAPR_KEEP_E4M3 || fmt == PAPR_KEEP_INT8), "papr_rows8_pack: unknown type %d or format %d", type, fmt);
-    PAPR_REQUIRE(rows >= 0 && width >= 1, "papr_rows8_pack: rows %lld, width %d", (long long)rows, width);
+    PAPR_REQUIRE(rows >= 0 && width >= 1 && width <= PAPR_ROWS8_MAX_WIDTH, "papr_rows8_pack: rows %lld, width %d (1 .. %d)", (long long)rows, width, PAPR_ROWS8_MAX_WIDTH);
     PAPR_REQUIRE(rows <= 1 || ldx >= width, "papr_rows8_pack: row stride %lld does not cover %d columns", (long long)ldx, width);
     if (rows == 0) return 0;
     PAPR_REQUIRE(x && codes && exps, "papr_rows8_pack: a pointer is missing");
@@ -137,7 +137,7 @@ extern "C" int papr_rows8_pack(int32_t type, int32_t fmt, const void* x, int64_t
 
 extern "C" int papr_rows8_unpack(int32_t type, int32_t fmt, const void* codes, const void* exps, int64_t rows, int32_t width, void* x, papr_stream_t stream) {
     PAPR_REQUIRE(papr_type_ok(type) && (fmt == PAPR_KEEP_E4M3 || fmt == PAPR_KEEP_INT8), "papr_rows8_unpack: unknown type %d or format %d", type, fmt);
-    PAPR_REQUIRE(rows >= 0 && width >= 1, "papr_rows8_unpack: rows %lld, width %d", (long long)rows, width);
+    PAPR_REQUIRE(rows >= 0 && width >= 1 && width <= PAPR_ROWS8_MAX_WIDTH, "papr_rows8_unpack: rows %lld, width %d (1 .. %d)", (long long)rows, width, PAPR_ROWS8_MAX_WIDTH);
     if (rows == 0) return 0;
     PAPR_REQUIRE(x && codes && exps, "papr_rows8_unpack: a pointer is missing");
     PAPR_REQUIRE(((uintptr_t)codes & 7) == 0, "papr_rows8_unpack: the codes start on 8 bytes");

@@ -106,6 +106,7 @@ class JoinGrads(C.Structure):            # papr_join_grads
 
 
 JOIN_MAX_WIDTH = 8192
+ROWS8_MAX_WIDTH = 1 << 30
 _lib = None
 
 

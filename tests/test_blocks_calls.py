@@ -83,3 +83,17 @@ def test_c_entry_points_refuse_strides_and_workspaces_that_do_not_fit():
     refused(L.papr_rows8_pack(0, 1, p, 7, 4, 8, p, p, None), "row stride")
     refused(L.papr_rows8_pack(0, 1, p, -8, 4, 8, p, p, None), "row stride")
     refused(L.papr_linear_fwd(hip.LinearDesc(0, 0, 0, 0, 4, 6, 8), p, 8, p, 8, None, p, 5, p, None, None, None), "residual")
+
+
+def test_packed_rows_too_wide_for_32_bit_columns_are_refused():
+    """(The number of blocks of a row of 2^31 - 1 columns overflowed: nothing was packed, and no error.)"""
+    import ctypes as C
+    from papr_amd import hip
+    L, p = hip.lib(), C.c_void_p(4096)
+    for width in (hip.ROWS8_MAX_WIDTH + 1, 2 ** 31 - 40, 2 ** 31 - 1):
+        for code in (L.papr_rows8_pack(1, 1, p, width, 1, width, p, p, None), L.papr_rows8_unpack(1, 1, p, p, 1, width, p, None)):
+            assert code == 1 and "width %d" % width in L.papr_last_error().decode()
+        with pytest.raises(ValueError, match="at most"):
+            blocks.pack_rows(torch.zeros(1).expand(1, width))
+        with pytest.raises(ValueError, match="at most"):
+            blocks.PackedRows(PACKED.codes, PACKED.exps, "e4m3", (1, width), torch.float16).rows()
