@@ -63,15 +63,9 @@ def _load():
         from . import _blocks as m
     except ImportError as e:
         raise RuntimeError("papr_amd: papr_amd/_blocks.so is missing or does not load (%s) -- run `python -c 'import __graft_entry__ as g; g.build()'`" % e)
-    m.bind({name: C.cast(getattr(L, name), C.c_void_p).value for name in hip.EXPORTS if name.startswith(("papr_linear_", "papr_join_", "papr_rows8_", "papr_last_error"))})
+    m.bind({name: C.cast(getattr(L, name), C.c_void_p).value for name in hip.EXPORTS if name.startswith(("papr_linear_", "papr_join_", "papr_rows8_", "papr_last_error"))}, hip)
     _native = m
     return m
-
-
-def _done(what, result):
-    if hip.DEBUG_SYNC:
-        hip.check(0, what)
-    return result
 
 
 # ---------------------------------------------------------------------------------------------- rows in 8 bits
@@ -93,7 +87,7 @@ class PackedRows:
             x = None
         if x is None:
             self._explain()
-        return _done("papr_rows8_unpack", x)
+        return x
 
     def _explain(self):
         who, shape = "PackedRows.rows", tuple(self.shape)
@@ -125,7 +119,7 @@ def pack_rows(x, fmt="e4m3"):
         if x.shape[-1] > hip.ROWS8_MAX_WIDTH:
             _fail("pack_rows", "rows of %d columns (at most %d)" % (x.shape[-1], hip.ROWS8_MAX_WIDTH))
         _check_device("pack_rows", x)
-    return _done("papr_rows8_pack", PackedRows(packed[0], packed[1], fmt, x.shape, x.dtype))
+    return PackedRows(packed[0], packed[1], fmt, x.shape, x.dtype)
 
 
 # ---------------------------------------------------------------------------------------------- linear layers
@@ -142,7 +136,7 @@ def linear_rows(x, weight, bias=None, residual=None, act="none", keep=None):
         y = None
     if y is None:
         _explain_linear(x, weight, bias, residual, act, keep)
-    return _done("papr_linear_fwd", y)
+    return y
 
 
 def _explain_linear(x, weight, bias, residual, act, keep):
@@ -217,7 +211,7 @@ def norm_rows(x, norm):
         _check_norm("norm_rows", "norm", norm, x)
         _check_device("norm_rows", x, norm.gain, norm.shift)
         _fail("norm_rows", "arguments that do not fit")
-    return _done("papr_join_fwd", h)
+    return h
 
 
 def join_rows(x, f, gate=None, scale=1.0, post=None, pre=None, gate_act="sigmoid"):
@@ -232,7 +226,7 @@ def join_rows(x, f, gate=None, scale=1.0, post=None, pre=None, gate_act="sigmoid
     out = _join(x, f, gate, 1.0 if cols else scale, scale if cols else None, _PLAIN if post is None else post, pre, gate_act) if f is not None else None
     if out is None:
         _explain_join(x, f, gate, scale, post, pre, gate_act)
-    return _done("papr_join_fwd", out)
+    return out
 
 
 def _explain_join(x, f, gate, scale, post, pre, gate_act):

@@ -43,7 +43,13 @@ PAPR_ENTRY(papr_join_bwd);
 PAPR_ENTRY(papr_join_bwd_workspace_bytes);
 #undef PAPR_ENTRY
 
-void bind(const py::dict& at) {
+PyObject *hip_names = nullptr, *debug_name = nullptr;      // papr_amd.hip's namespace (never released: autograd threads may outlive the interpreter's modules)
+
+void bind(const py::dict& at, const py::object& hip) {
+    if (!hip_names) {
+        hip_names = py::object(hip.attr("__dict__")).release().ptr();
+        debug_name = PyUnicode_InternFromString("DEBUG_SYNC");
+    }
     auto take = [&](auto& fn, const char* name) { fn = reinterpret_cast<std::decay_t<decltype(fn)>>(at[name].cast<uintptr_t>()); };
     take(papr_last_error_, "papr_last_error");
     take(papr_linear_fwd_, "papr_linear_fwd");
@@ -59,6 +65,10 @@ void bind(const py::dict& at) {
 
 void check(int code, const char* what) {
     if (code) throw std::runtime_error(std::string(what) + " failed (" + std::to_string(code) + "): " + papr_last_error_());
+    // hip.DEBUG_SYNC: every library call named and waited for, those of the backward pass's threads too
+    struct Held { PyGILState_STATE state = PyGILState_Ensure(); ~Held() { PyGILState_Release(state); } } held;
+    PyObject* debug = PyDict_GetItem(hip_names, debug_name);
+    if (debug && debug != Py_False && PyObject_IsTrue(debug)) py::reinterpret_borrow<py::dict>(hip_names)["check"](0, what);
 }
 
 int type_of(const Tensor& t) {

@@ -86,3 +86,23 @@ def test_operands_that_torch_negates_lazily(dt):
         assert torch.equal(blocks.linear_rows(lazy(x), w), blocks.linear_rows(x, w))
     for got, want in zip(run(True), run(False)):
         assert torch.equal(got, want)
+
+
+def test_debug_sync_names_every_library_call_and_waits(capfd, monkeypatch):
+    from papr_amd import hip
+    p = {n: t.requires_grad_(True) for n, t in block_params(torch.float16, 64, 128, 1).items()}
+    x = torch.randn((8, 64), generator=gen(1), device="cuda").half()
+    block(p, x, "int8")
+    assert capfd.readouterr().err == ""
+    waits = []
+    wait = torch.cuda.synchronize
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: (waits.append(1), wait()))
+    monkeypatch.setattr(hip, "DEBUG_SYNC", True)
+    y, h = block(p, x, "int8")
+    blocks.pack_rows(x).rows()
+    forward = capfd.readouterr().err.splitlines()
+    torch.autograd.grad([y, h], list(p.values()), [torch.ones_like(y), torch.ones_like(h)])
+    backward = capfd.readouterr().err.splitlines()
+    call = lambda *names: ["papr call: papr_" + n for n in names]
+    assert forward == call("join_fwd", "linear_fwd", "rows8_pack", "linear_fwd", "rows8_pack", "linear_fwd", "join_fwd", "rows8_pack", "rows8_unpack")
+    assert sorted(backward) == call("join_bwd", "join_bwd", "linear_bwd", "linear_bwd", "linear_bwd") and len(waits) == 14
