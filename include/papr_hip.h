@@ -514,6 +514,8 @@ int papr_adam_step_scaled(const papr_adam_tensor* tensors, int32_t n_tensors, co
  *             8 gemm_tn_h3 (split-f16 weight gradient)
  *             9 mlp_chain forward run   10 mlp_chain data-gradient run   (several layers in one launch; N = number of
  *               layers, K = input width; bytes / flops below carry the algorithmic totals of the launch)
+ *            11 3x3 convolution   12 its weight gradient
+ *            13 papr_linear_fwd's product   14 papr_linear_bwd's d_x   15 its d_w   (M, N, K of the layer)
  */
 typedef struct {
     int32_t kernel;
@@ -521,7 +523,7 @@ typedef struct {
     int64_t M;      /* rows (rays for kernel 5, with N = points, K = k) */
     float ms;       /* hipEventElapsedTime between the events bracketing the launch */
     int64_t bytes;  /* kernels 9, 10: algorithmic HBM bytes of the launch (input rows + stored rows + masks read + weights); else 0 */
-    int64_t flops;  /* kernels 9, 10: fp32-equivalent 2 M N K summed over the layers (each product costs three f16 MFMA products); else 0 */
+    int64_t flops;  /* kernels 9, 10: fp32-equivalent 2 M N K summed over the layers (each product costs three f16 MFMA products); 13 .. 15: 2 M N K; else 0 */
 } papr_profile_record;
 
 int papr_profile_enable(int on);

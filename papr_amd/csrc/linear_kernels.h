@@ -773,6 +773,16 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand
     }
 }
 
+// papr_profile_collect: one record a product (its slabs' joining included)
+struct Timed {
+    hipStream_t s;
+    bool on;
+    Timed(int kernel, int64_t M, int64_t N, int64_t K, hipStream_t stream) : s(stream), on(papr_prof_on()) {
+        if (on) papr_prof_begin2(kernel, (long)M, (int)N, (int)K, 0, 2LL * M * N * K, s);
+    }
+    ~Timed() { if (on) papr_prof_end(s); }
+};
+
 // Up to here the few-rows kernel is the faster one: 1 x 1024 -> 4096 bf16 3.8 us against 10.1 of 64 x 64 tiles, 32 x 4096 -> 1024 26.8 against 29.6, 64 x 4096 -> 1024 48 against 30.
 constexpr int FEW_ROWS = 32;
 
@@ -969,6 +979,7 @@ int weight_product(int keep, bool vec, const Operand& A, const Operand& B, int64
 
 template <typename T>
 int forward(const Operand& x, const Operand& w, int64_t K, bool vec, const Epilogue& ep, hipStream_t s) {
+    Timed timed(13, x.rows, w.rows, K, s);
     if (x.rows <= FEW_ROWS) return launch_few_rows<T>(x, w, K, vec, ep, s);
     const Choice c = choose(x.rows, w.rows, K, path_of(sizeof(T) == 4 ? PAPR_TYPE_F32 : PAPR_TYPE_F16, vec, 0, false), false, aside_of(ep.res, ep.z, sizeof(T)));
     return ep.wide ? launch_product<T, K_RUNS, K_RUNS, 0, 0, OUT_FORWARD>(c, vec, x, w, K, ep, s) : launch_product<T, K_RUNS, K_RUNS, 0, 0, OUT_FORWARD_LOOSE>(c, vec, x, w, K, ep, s);
@@ -976,6 +987,7 @@ int forward(const Operand& x, const Operand& w, int64_t K, bool vec, const Epilo
 
 template <typename T>
 int grad_rows(bool vec, const Operand& d_z, const Operand& w, int64_t N, void* d_x, float* slab, hipStream_t s) {
+    Timed timed(14, d_z.rows, N, w.rows, s);
     if constexpr (sizeof(T) == 2)
         if (d_z.low) return rows_product<T, K_RUNS, ROWS_RUN, PAIR, 0>(vec, d_z, w, N, d_x, slab, s);
     return rows_product<T, K_RUNS, ROWS_RUN, 0, 0>(vec, d_z, w, N, d_x, slab, s);
@@ -983,6 +995,7 @@ int grad_rows(bool vec, const Operand& d_z, const Operand& w, int64_t N, void* d
 
 template <typename T>
 int grad_weight(int keep, bool vec, const Operand& d_z, const Operand& x, int64_t M, void* d_w, float* slab, hipStream_t s) {
+    Timed timed(15, M, d_z.rows, x.rows, s);
     if constexpr (sizeof(T) == 2)
         if (d_z.low) return weight_product<T, PAIR>(keep, vec, d_z, x, M, d_w, slab, s);
     return weight_product<T, 0>(keep, vec, d_z, x, M, d_w, slab, s);

@@ -106,3 +106,22 @@ def test_debug_sync_names_every_library_call_and_waits(capfd, monkeypatch):
     call = lambda *names: ["papr call: papr_" + n for n in names]
     assert forward == call("join_fwd", "linear_fwd", "rows8_pack", "linear_fwd", "rows8_pack", "linear_fwd", "join_fwd", "rows8_pack", "rows8_unpack")
     assert sorted(backward) == call("join_bwd", "join_bwd", "linear_bwd", "linear_bwd", "linear_bwd") and len(waits) == 14
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=lambda t: str(t)[6:])
+def test_linear_products_appear_in_the_profile(dt):
+    from papr_amd import hip
+    x = torch.randn((300, 48), generator=gen(1), device="cuda").to(dt).requires_grad_(True)
+    w = torch.randn((64, 48), generator=gen(2), device="cuda").to(dt).requires_grad_(True)
+    hip.profile_collect()
+    hip.profile_enable(True)
+    try:
+        y = blocks.linear_rows(x, w, act="silu")
+        torch.autograd.grad(y, [x, w], torch.ones_like(y))
+        blocks.linear_rows(x[:3].detach(), w.detach())
+    finally:
+        hip.profile_enable(False)
+    records = hip.profile_collect()
+    flops = 2 * 300 * 64 * 48
+    assert [r[:4] + r[5:] for r in records] == [(13, 300, 64, 48, 0, flops), (14, 300, 64, 48, 0, flops), (15, 300, 64, 48, 0, flops), (13, 3, 64, 48, 0, flops // 100)]
+    assert all(0 < r[4] < 100 for r in records)
