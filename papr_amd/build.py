@@ -91,11 +91,23 @@ def _register_metadata_ok(asm, kernel_substr="mlp_chain4_kernel"):
 ROW_BLOCKS = ["join.hip", "rows8.hip", "linear.hip", "linear_f32.hip", "linear_f16.hip", "linear_bf16.hip"]      # (headers of their own)
 
 
-def _stale(target, deps):
+def _stale(target, deps, made_by):
+    """Missing, older than a dependency, or made by another command than `made_by` (flags, the torch it was built against): the command is kept beside the target."""
     if not os.path.exists(target):
+        return True
+    try:
+        with open(target + ".cmd") as f:
+            if f.read() != made_by:
+                return True
+    except OSError:
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _made(target, made_by):
+    with open(target + ".cmd", "w") as f:
+        f.write(made_by)
 
 
 def build_library(force=False, verbose=True):
@@ -108,15 +120,15 @@ def build_library(force=False, verbose=True):
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src.replace(".hip", ".o"))
         objs.append(o)
-        if force or _stale(o, [s] + headers + ([os.path.join(CSRC, h) for h in ("block_types.h", "linear.h", "linear_kernels.h")] if src in ROW_BLOCKS else [])):
-            cmd = [hipcc] + FLAGS + EXTRA_FLAGS.get(src, []) + ["-c", s, "-o", o]
+        cmd = [hipcc] + FLAGS + EXTRA_FLAGS.get(src, []) + ["-c", s, "-o", o]
+        if force or _stale(o, [s] + headers + ([os.path.join(CSRC, h) for h in ("block_types.h", "linear.h", "linear_kernels.h")] if src in ROW_BLOCKS else []), " ".join(cmd)):
             if verbose:
                 print(" ".join(cmd), flush=True)
-            procs.append((src, subprocess.Popen(cmd)))
-    for src, p in procs:
+            procs.append((src, o, " ".join(cmd), subprocess.Popen(cmd)))
+    for src, _, _, p in procs:
         if p.wait() != 0:
             raise RuntimeError("hipcc failed on %s" % src)
-    for src, _ in procs:
+    for src, _, _, _ in procs:
         if src in NO_ACCVGPR:
             asm = subprocess.run([hipcc] + [f for f in FLAGS if f != "-fPIC"] + EXTRA_FLAGS.get(src, []) + ["-w", "-S", "--cuda-device-only", os.path.join(CSRC, src), "-o", "-"],
                                  check=True, capture_output=True, text=True).stdout
@@ -133,11 +145,14 @@ def build_library(force=False, verbose=True):
                 os.remove(os.path.join(objdir, src.replace(".hip", ".o")))
                 raise RuntimeError("%s: the compiler uses AGPRs itself (%d instructions outside the inline asm name an AGPR): register pressure too high for the by-name "
                                    "weight fragments, see the comment in the source" % (src, n))
-    if force or procs or _stale(LIB, objs):
-        cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + ["-Wl,-rpath,/opt/rocm/lib", "-Wl,--no-undefined"]
+    for _, o, made_by, _ in procs:
+        _made(o, made_by)
+    cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + ["-Wl,-rpath,/opt/rocm/lib", "-Wl,--no-undefined"]
+    if force or procs or _stale(LIB, objs, " ".join(cmd)):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+        _made(LIB, " ".join(cmd))
     return LIB
 
 
@@ -149,16 +164,17 @@ def build_glue(force=False, verbose=True):
     import sysconfig
     import torch
     src = os.path.join(CSRC, "blocks_glue.cpp")
-    if not (force or _stale(GLUE, [src, os.path.join(os.path.dirname(PKG), "include", "papr_hip.h")])):
-        return GLUE
     root = os.path.dirname(torch.__file__)
     inc = os.path.join(root, "include")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-D__HIP_PLATFORM_AMD__=1",
            "-DUSE_ROCM=1", "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], "-I/opt/rocm/include", src, "-o", GLUE,
            "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.check_call(cmd)
+    made_by = " ".join(cmd) + " # torch " + torch.__version__
+    if force or _stale(GLUE, [src, os.path.join(os.path.dirname(PKG), "include", "papr_hip.h")], made_by):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+        _made(GLUE, made_by)
     return GLUE
 
 
