@@ -7,7 +7,8 @@
 //     off by 2^-134 at most, bfloat16's smallest half step) on its way into LDS, and six of the nine products are summed.  The parts are at most 1, 2^-8 and 2^-17 of a value, so
 //     what is left out (second times third, twice, and third times third) is at most 2^-24 of a term: float32's own rounding.  Summed from the small products up, so that
 //     a value near the largest number is itself again before anything is added to its first part (2^128 - 2^120 here, 2^128 with the second).
-//     2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the float32 matrix instructions.  An infinity's third part is it.
+//     2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the float32 matrix instructions.  The parts of an infinity are no
+//     number, and their products NaN: a result that is NaN is summed again from the values themselves (sum_again).
 //   * d_z is an operand of two products.  For 16-bit rows with an activation that bends it (leakyrelu, gelu, silu) it is kept as the sum of two values of the rows' type, high
 //     and low (16 significant bits or more), and both products take both: rounded to one such value it would be an error of the gradients' own rounding's size in each
 //     of them (measured 1.45 times that rounding together, 1.06 so), and a slope up to 1.13 can take it past float16's largest number.  Twice the matrix instructions: 8192 x 1024
@@ -95,30 +96,14 @@ __device__ __forceinline__ void act_slopes(float (&g)[N], const float (&z)[N], i
     }
 }
 
-// N float32 values in three bfloat16 parts each.  An infinity is (+-1, 0, +-infinity): its third part meets the other value's first alone, so the result has the sign of their
-// product (and is NaN beside a zero).
-template <int N>
-__device__ __forceinline__ void cut_floats(const float (&f)[N], bf16 (&part)[3][N]) {
+// a float32 value in three bfloat16 parts (of an infinity the third is NaN)
+__device__ __forceinline__ void cut_float(float v, bf16 (&part)[3]) {
     const float most = largest<bf16>();
-    float peak = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        float v = f[i];
-        part[0][i] = (bf16)__builtin_amdgcn_fmed3f(v, -most, most);
-        v -= (float)part[0][i];
-        part[1][i] = (bf16)v;
-        v -= (float)part[1][i];
-        part[2][i] = (bf16)v;
-        peak = fmaxf(peak, fabsf(f[i]));
-    }
-    if (__builtin_expect(peak == __builtin_inff(), 0))
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (fabsf(f[i]) == __builtin_inff()) {
-                part[0][i] = (bf16)__builtin_copysignf(1.f, f[i]);
-                part[1][i] = (bf16)0.f;
-                part[2][i] = (bf16)f[i];
-            }
+    part[0] = (bf16)__builtin_amdgcn_fmed3f(v, -most, most);
+    v -= (float)part[0];
+    part[1] = (bf16)v;
+    v -= (float)part[1];
+    part[2] = (bf16)v;
 }
 
 enum { K_RUNS = 0, ROWS_RUN = 1 };                // which index of an operand is contiguous in memory
@@ -255,10 +240,16 @@ struct Tile {
             } else if (SPLIT) {
                 const uint4 t = h.reg[0][q];
                 const float f[4] = {__uint_as_float(t.x), __uint_as_float(t.y), __uint_as_float(t.z), __uint_as_float(t.w)};
-                bf16 cut[3][4];
-                cut_floats(f, cut);
+                papr_pack<bf16, 4> p[PLANES];
 #pragma unroll
-                for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<bf16, 4>*>(lds + n * PLANE + at) = {{cut[n][0], cut[n][1], cut[n][2], cut[n][3]}};
+                for (int i = 0; i < 4; ++i) {
+                    bf16 cut[3];
+                    cut_float(f[i], cut);
+#pragma unroll
+                    for (int n = 0; n < PLANES; ++n) p[n].v[i] = cut[n];
+                }
+#pragma unroll
+                for (int n = 0; n < PLANES; ++n) *reinterpret_cast<papr_pack<bf16, 4>*>(lds + n * PLANE + at) = p[n];
             } else {
 #pragma unroll
                 for (int n = 0; n < SOURCES; ++n) *reinterpret_cast<uint4*>(lds + n * PLANE + at) = h.reg[n][q];
@@ -349,6 +340,13 @@ __device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int6
     for (int i = 0; i < E; ++i) t.v[i] = (T)v[i];
     put<T, E, LOOSE>(reinterpret_cast<T*>(ep.out) + m * N + n, t);
 }
+template <typename T>
+__device__ __forceinline__ void finish_one(float value, int64_t m, int64_t n, int64_t N, const Epilogue& ep) {
+    float v[1] = {value}, bias[1] = {ep.bias ? (float)reinterpret_cast<const T*>(ep.bias)[n] : 0.f};
+    papr_pack<T, 1> res;
+    if (ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
+    finish<T, OUT_FORWARD, 1, false>(v, m, n, N, bias, res, ep);
+}
 // 32 rows of a wave's part, from its LDS: 16 bytes of a row a lane
 template <typename T, int OUT, typename S, bool LOOSE>
 __device__ __forceinline__ void write_block(const float* epi, int64_t mw, int64_t n, int64_t M, int64_t N, const float (&bias)[16 / sizeof(T)], const Epilogue& ep) {
@@ -384,10 +382,8 @@ __device__ __forceinline__ void write_block(const float* epi, int64_t mw, int64_
             const float* at = epi + (r * RPP + lane / LPR) * S::EPI_STRIDE + lane % LPR * E;
 #pragma unroll 1
             for (int i = 0; m < M && n + i < N; ++i) {
-                float v1[1] = {at[i]}, b1[1] = {OUT == OUT_FORWARD && ep.bias ? (float)reinterpret_cast<const T*>(ep.bias)[n + i] : 0.f};
-                papr_pack<T, 1> r1;
-                if (with_res) r1.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n + i];
-                finish<T, OUT, 1, false>(v1, m, n + i, N, b1, r1, ep);
+                if (OUT == OUT_FORWARD) finish_one<T>(at[i], m, n + i, N, ep);
+                else reinterpret_cast<T*>(ep.out)[m * N + n + i] = (T)at[i];
             }
         }
 }
@@ -436,6 +432,22 @@ __device__ __forceinline__ void write_tile(const f32x16 (&acc)[S::IM][S::IN], sh
     }
 }
 
+// A float32 result that is NaN because an operand is (then it is found at once) or is infinite: the sum of its terms as the definition has them.
+template <typename T, int LAYOUT, int FMT>
+__device__ __forceinline__ float term(const Operand& o, int64_t r, int64_t k) {
+    const int64_t at = LAYOUT == K_RUNS ? r * o.ld + k : k * o.ld + r;
+    if (FMT == 0) return (float)reinterpret_cast<const T*>(o.p)[at];
+    float v[4];
+    papr_codes_to_float<FMT>((unsigned)reinterpret_cast<const uint8_t*>(o.p)[at], __uint_as_float((unsigned)o.exps[at >> 5] << 23), v);
+    return v[0];
+}
+template <typename T, int LA, int LB, int FMT>
+__device__ __forceinline__ float sum_again(const Operand& A, const Operand& B, int64_t m, int64_t n, int64_t kb, int64_t ke) {
+    float s = 0.f;
+    for (int64_t k = kb; k < ke && s == s; ++k) s = __builtin_fmaf(term<T, LA, 0>(A, m, k), term<T, LB, FMT>(B, n, k), s);
+    return s;
+}
+
 // Operands through registers: what the streaming kernel cannot take -- float32 (512,000 x 256 -> 256 forward 545 us, d_x 410, d_W 382: 123 - 176 TFLOP/s for the card's 154 of a
 // float32 library product; 8192 x 4096 x 1024 200), 8-bit rows (d_W of 65,536 x 1024 -> 1024 200 us, 690 TFLOP/s), a wide d_z and short odd rows.  Bound by one stage of
 // loads being on its way and, in float32, by cutting the values apart.
@@ -446,7 +458,10 @@ __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Opera
     typedef typename P::TB TB;
     constexpr int IM = S::IM, IN = S::IN, BK = P::BK;
     extern __shared__ __attribute__((aligned(16))) short smem[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
+    __shared__ int nan_seen;                       // (float32 only)
+    constexpr bool SPLIT = TA::SPLIT || TB::SPLIT;
+    if (SPLIT && threadIdx.x == 0) nan_seen = 0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / S::WN, wn = wave % S::WN;
     const Place at = place_of(blockIdx.x, gridDim.x, tiles_m, tiles_n);
     const int64_t m0 = (int64_t)at.m * S::TM, n0 = (int64_t)at.n * S::TN;
     const int64_t kb = at.part * k_per_part, ke = kb + k_per_part < K ? kb + k_per_part : K;
@@ -522,7 +537,34 @@ __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Opera
             __syncthreads();
         }
     }
+    bool again = false;
+    if constexpr (SPLIT) {                         // (looking at every value on its way into LDS instead cost 4 to 8 % of a product)
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < IM; ++i)
+#pragma unroll
+            for (int j = 0; j < IN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) nan |= __builtin_isunordered(acc[i][j][e], acc[i][j][e + 1]);
+        if (nan) nan_seen = 1;
+        __syncthreads();
+        again = nan_seen != 0;
+    }
     write_tile<T, OUT, S>(acc, smem, m0, n0, A.rows, B.rows, at.part, ep);
+    if constexpr (SPLIT) {
+        if (!again) return;
+        __syncthreads();
+        float* out = reinterpret_cast<float*>(ep.out) + (OUT == OUT_SLAB ? at.part * A.rows * B.rows : 0);
+        for (int i = threadIdx.x; i < S::TM * S::TN; i += S::THREADS) {
+            const int64_t m = m0 + i / S::TN, n = n0 + i % S::TN;
+            if (m >= A.rows || n >= B.rows) continue;
+            float& to = out[m * B.rows + n];
+            if (to == to) continue;
+            float v[1] = {sum_again<T, LA, LB, FMT>(A, B, m, n, kb, ke)};
+            if constexpr (OUT == OUT_SLAB || OUT == OUT_ROWS) to = v[0];
+            else finish_one<T>(v[0], m, n, B.rows, ep);
+        }
+    }
 }
 
 // The same product for 16-bit rows that start on 16 bytes: operands go straight from memory into LDS (global_load_lds, 16 bytes a lane), DEPTH stages of 32 terms, three
@@ -715,10 +757,12 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[0][i] = v.t.v[i];
         } else {
-            bf16 cut[3][8];
-            cut_floats(v.t.v, cut);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { f[0][i] = cut[0][i]; f[1][i] = cut[1][i]; f[2][i] = cut[2][i]; }
+            for (int i = 0; i < 8; ++i) {
+                bf16 cut[3];
+                cut_float(v.t.v[i], cut);
+                f[0][i] = cut[0]; f[1][i] = cut[1]; f[2][i] = cut[2];
+            }
         }
     };
     f32x4 acc[MT];
@@ -763,13 +807,12 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(Operand A, Operand
     for (int i = threadIdx.x; i < MT * 256; i += 64 * WAVES) {
         const int64_t m = i >> 4, n = n0 + (i & 15);
         if (m >= M || n >= N) continue;
-        float v[1] = {0.f}, bias[1] = {0.f};
+        float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) v[0] += lds[w][m][i & 15];
-        if (ep.bias) bias[0] = (float)reinterpret_cast<const T*>(ep.bias)[n];
-        papr_pack<T, 1> res;
-        if (ep.res) res.v[0] = reinterpret_cast<const T*>(ep.res)[m * ep.ld_res + n];
-        finish<T, OUT_FORWARD, 1, false>(v, m, n, N, bias, res, ep);
+        for (int w = 0; w < WAVES; ++w) v += lds[w][m][i & 15];
+        if constexpr (sizeof(T) == 4)
+            if (v != v) v = sum_again<T, K_RUNS, K_RUNS, 0>(A, B, m, n, 0, K);
+        finish_one<T>(v, m, n, N, ep);
     }
 }
 
