@@ -111,3 +111,22 @@ def test_infinities_are_those_of_the_definition(M, N, K):
     as_defined(d_x, g6 @ w6, fin(g6) @ fin(w6), N)
     as_defined(d_w, g6.t() @ x6, fin(g6).t() @ fin(x6), M)
     assert torch.isinf(y).any() and torch.isnan(y).any()
+
+
+@pytest.mark.parametrize("M, N, K", SHAPES)
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+def test_infinities_pass_the_epilogue_and_its_slopes(M, N, K, act):
+    """+inf in rows of x, through the bias, the activation and the residual: y is infinite or act(-inf), with the other rows as they were, to the bit; kept rows hold NaN for it."""
+    x, w, b, r, d_y = linear_data(M, N, K, torch.float32, seed=8)
+    clean = blocks.linear_rows(x, w, b, r, act=act)
+    x[M // 2, K // 2] = math.inf
+    y = blocks.linear_rows(x, w, b, r, act=act)
+    others = torch.arange(M, device="cuda") != M // 2
+    assert torch.equal(y[others], clean[others])
+    up = w[:, K // 2] > 0
+    assert torch.isposinf(y[M // 2][up]).all()
+    assert torch.equal(y[M // 2][~up], r[M // 2][~up]) if act == "relu" else torch.isnan(y[M // 2][~up]).all()          # (silu, gelu: -inf times zero)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    d_x, d_w = torch.autograd.grad(blocks.linear_rows(x, w, act="relu", keep="int8"), [x, w], d_y)
+    assert torch.isfinite(d_x).all() and torch.isnan(d_w[:, K // 2]).all() and torch.isfinite(d_w[:, torch.arange(K, device="cuda") != K // 2]).all()
