@@ -4,8 +4,8 @@
 // with N = layernorm (v - mean) / (std_unbiased + eps) * gain + shift -- the framework's own form (models/attn.py:39-42) -- or rmsnorm
 // v / sqrt(mean(v^2) + eps) * gain (+ shift), a = identity, sigmoid or silu, g one gate per element or per row, s a number or one per column.
 // Bound by HBM: forward reads x, f, g and writes y, h; backward reads x, f, g, d_y, d_h and writes d_x, d_f, d_g.  The backward pass reads x and
-// recomputes y in float32 (reading the rounded y instead would move the same bytes).  Measured: 16,384 x 2048 bf16 forward with a full gate 64 us (5.2 TB/s, a large copy's
-// rate); 512,000 x 256 f16 with a row gate 220 us forward (4.8 TB/s) and 367 backward (4.3); 60,000 x 1000 float32 187 and 245 (5.1, 5.9).
+// recomputes y in float32 (reading the rounded y instead would move the same bytes).  Measured: 16,384 x 2048 bf16 forward with a full gate 66 us (5.1 TB/s; a large copy 5.2);
+// 512,000 x 256 f16 with a row gate 202 us forward (5.2 TB/s) and 307 backward (5.1); 60,000 x 1000 float32 without a gate 188 and 242 (5.1, 6.0).
 //
 // A row lies in the registers of G lanes, eight elements each (G = the power of two that covers the width): sums over a row are DPP steps inside a
 // wave, one LDS exchange where a row takes several waves.  Norms in two passes over the registers (mean, then squares): no cancellation.
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void join_bwd_kernel(papr_joi
     int turn = 0;
     const int j = threadIdx.x % G, width = d.width;
     const float rw = 1.f / (float)width;
-    // What a compute unit has on its way is what bounds this kernel (eight waves; with one row's operands each 3.2 TB/s, with two 4.3): two rows ahead of the arithmetic,
+    // What a compute unit has on its way is what bounds this kernel (eight waves; 512,000 x 256 float16 with one row's operands each 352 us, 4.5 TB/s, with two 311, 5.1): two rows ahead of the arithmetic,
     // with the parameters read again from LDS row by row instead of sitting in 32 registers.  float32 rows (twice the bytes) and odd ones: one row ahead.
     constexpr int AHEAD = G == 512 || sizeof(T) == 4 || V == 1 ? 1 : 2;
     // Rows of eight waves: gates and p are computed again behind the next norm's sums instead of being carried over them (32 registers).

@@ -5,14 +5,14 @@
 //   * float16 / bfloat16: the values themselves are the matrix operands.
 //   * float32: every value is cut into three bfloat16 parts (8 + 8 + 8 bits, rounded to nearest, the first kept finite: exact for every magnitude of 2^-109 and more, below that
 //     off by 2^-134 at most, bfloat16's smallest half step) on its way into LDS, and six of the nine products are summed.  The parts are at most 1, 2^-8 and 2^-17 of a value, so
-//     what is left out (second times third, twice, and third times third) is at most 2^-24 of a term: float32's own rounding.  Summed from the small products up, so that
-//     a value near the largest number is itself again before anything is added to its first part (2^128 - 2^120 here, 2^128 with the second).
-//     2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the float32 matrix instructions.  The parts of an infinity are no
-//     number, and their products NaN: a result that is NaN is summed again from the values themselves (sum_again).
+//     what is left out (second times third, twice, and third times third) is at most 2^-24 of a term: float32's own rounding.  Summed from the small products up: the first two
+//     parts of the largest number alone add to 2^128, which is infinite.  2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the float32 matrix instructions.  The third part of an
+//     infinity is NaN, and so are its products: a result that is NaN is summed again from the values themselves (sum_again).
+//   * z is kept for the backward pass in the rows' type: a slope moves by at most 0.8 of z's rounding, for half (float32: none) of the memory that float32 would take.
 //   * d_z is an operand of two products.  For 16-bit rows with an activation that bends it (leakyrelu, gelu, silu) it is kept as the sum of two values of the rows' type, high
 //     and low (16 significant bits or more), and both products take both: rounded to one such value it would be an error of the gradients' own rounding's size in each
 //     of them (measured 1.45 times that rounding together, 1.06 so), and a slope up to 1.13 can take it past float16's largest number.  Twice the matrix instructions: 8192 x 1024
-//     -> 4096 in bfloat16, forward and backward, 448 us; with d_z rounded once it was 332.
+//     -> 4096 in bfloat16, forward and backward, 453 us; with d_z rounded once it was 332.
 //     d_b sums it in float32.
 #pragma once
 #include "linear.h"
@@ -448,9 +448,9 @@ __device__ __forceinline__ float sum_again(const Operand& A, const Operand& B, i
     return s;
 }
 
-// Operands through registers: what the streaming kernel cannot take -- float32 (512,000 x 256 -> 256 forward 545 us, d_x 410, d_W 382: 123 - 176 TFLOP/s for the card's 154 of a
-// float32 library product; 8192 x 4096 x 1024 200), 8-bit rows (d_W of 65,536 x 1024 -> 1024 200 us, 690 TFLOP/s), a wide d_z and short odd rows.  Bound by one stage of
-// loads being on its way and, in float32, by cutting the values apart.
+// Operands through registers: what the streaming kernel cannot take -- float32 (512,000 x 256 -> 256 forward 501 us, d_x 419, d_W 375: 134 - 179 TFLOP/s for the card's 154 of a
+// float32 library product; 8192 x 1024 -> 4096 200), 8-bit rows (d_W of 65,536 x 1024 -> 1024 from a pair and codes 293 us, 940 TFLOP/s of its two products, the matrix pipe 42 %
+// busy) and short odd rows.  Bound by one stage of loads being on its way and, in float32, by cutting the values apart.
 template <typename T, int LA, int LB, int FA, int FMT, bool VEC, int OUT, typename S>
 __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Operand B, int64_t K, int64_t k_per_part, unsigned tiles_m, unsigned tiles_n, Epilogue ep) {
     typedef Plan<T, LA, LB, FA, FMT, VEC, S> P;
@@ -568,16 +568,16 @@ __global__ __launch_bounds__(S::THREADS, 2) void product_kernel(Operand A, Opera
 }
 
 // The same product for 16-bit rows that start on 16 bytes: operands go straight from memory into LDS (global_load_lds, 16 bytes a lane), DEPTH stages of 32 terms, three
-// of them on their way while one is multiplied -- with one stage on its way in registers (product_kernel) half of a wave's time was waiting for it (256 x 256 tiles:
-// the matrix pipe 34 % busy).  An instruction fills 1 KB in lane order, so the images are made by which address a lane asks for:
+// of them on their way while one is multiplied (product_kernel: one, in registers).  In d_x and d_W of 8192 x 1024 -> 4096 waves wait 31 to 38 % of their time and the matrix pipe
+// is half busy, as at 8192^3.  An instruction fills 1 KB in lane order, so the images are made by which address a lane asks for:
 //   K_RUNS:   16 rows of 32 halfs, pieces exchanged by the row number as in Tile;
 //   ROWS_RUN: one "line" = the k rows q, q + LINES, q + 2 LINES, ... of R halfs one behind the other (1 KB), lines 1,088 bytes apart: the four consecutive k that a
 //             16-lane group of a transposing read wants lie on different quarters of the banks.
 // Rows past the operand's end: some row of it (never stored); terms past the part's end: a block of zeros.
 // The fragments of a 16-term step are read under the matrix instructions of the step before, and the stage's one barrier stands between its two steps: in front of
 // it a wave has read all of its stage (whose buffer the requests behind the barrier overwrite), behind it the next stage, requested three stages earlier, is there.
-// What bounds it: the matrix pipe and, for short sums, filling the pipeline and writing the results.  8192^3 in bf16 0.88 - 0.98 ms (1120 - 1250 TFLOP/s; the card's library
-// product 1281), 65,536 x 1024 -> 1024 backward 135 us (1020).
+// What bounds it: the matrix pipe and, for short sums, filling the pipeline and writing the results (the forward product of 65,536 x 1024 -> 1024: 234 us, a quarter busy).  8192^3 in
+// bf16 0.86 - 0.96 ms (1150 - 1280 TFLOP/s; the card's library product 1281), d_x and d_W of 65,536 x 1024 -> 1024 from a pair 258 and 245 us (1060, 1120 of their two products).
 __device__ const uint4 zero_block[4] = {};
 
 __device__ __forceinline__ void request16(const void* src, unsigned lds) {         // 64 lanes x 16 bytes -> LDS [lds, +1 KB) in lane order
