@@ -125,3 +125,40 @@ def test_linear_products_appear_in_the_profile(dt):
     flops = 2 * 300 * 64 * 48
     assert [r[:4] + r[5:] for r in records] == [(13, 300, 64, 48, 0, flops), (14, 300, 64, 48, 0, flops), (15, 300, 64, 48, 0, flops), (13, 3, 64, 48, 0, flops // 100)]
     assert all(0 < r[4] < 100 for r in records)
+
+
+def test_inference_mode_and_its_tensors():
+    """Inside inference mode, and its tensors outside of it, where no gradient is asked for."""
+    p = block_params(torch.float16, 64, 128, 1)
+    x = torch.randn((8, 64), generator=gen(1), device="cuda").half()
+    want = block(p, x, "e4m3")
+    with torch.inference_mode():
+        inner = x.clone()
+        got = block(p, inner, "e4m3")
+        assert not got[0].requires_grad and inner.is_inference()
+    with torch.no_grad():
+        again = block(p, inner, "e4m3")
+    for out in (got, again):
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert torch.equal(blocks.pack_rows(inner).rows(), blocks.pack_rows(x).rows())
+
+
+def test_one_tensor_in_several_places():
+    """The rows as residual and gate, the weight as rows: gradients add up as autograd adds them."""
+    g = gen(2)
+    x = torch.randn((40, 64), generator=g, device="cuda", dtype=torch.float32).requires_grad_(True)
+    w = (torch.randn((64, 64), generator=g, device="cuda") / 8).requires_grad_(True)
+
+    def run(f, sep):
+        xs = [x.detach().clone().requires_grad_(True) for _ in range(4)] if sep else [x] * 4
+        ws = [w.detach().clone().requires_grad_(True) for _ in range(2)] if sep else [w] * 2
+        y = blocks.linear_rows(xs[0], ws[0], residual=xs[1], act="silu", keep="int8")
+        z = blocks.linear_rows(ws[1], ws[0])
+        j = blocks.join_rows(xs[2], y, gate=xs[3], scale=z[0].clone())
+        leaves = xs + ws if sep else [x, w]
+        got = torch.autograd.grad(j, leaves, torch.ones_like(j))
+        return j, (got if not sep else (got[0] + got[1] + got[2] + got[3], got[4] + got[5]))
+    a, b = run(None, False), run(None, True)
+    assert torch.equal(a[0], b[0])
+    for s, t in zip(a[1], b[1]):
+        assert (s - t).abs().max() <= 8 * 2.0 ** -24 * t.abs().max() * 4          # (four float32 additions in another order)
