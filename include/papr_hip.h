@@ -574,8 +574,8 @@ int papr_profile_collect(papr_profile_record* out, int cap);
 enum { PAPR_TYPE_F32 = 0, PAPR_TYPE_F16 = 1, PAPR_TYPE_BF16 = 2 };
 
 /* Linear layer with its epilogue: y = act(x W^T + bias) + res, x (M, K), W (N, K), bias (N) or NULL, res (M, N) or NULL, y (M, N) contiguous.
- * z (M, N) or NULL: receives x W^T + bias in the rows' type, what the backward pass of an activation reads (not needed for PAPR_ACT_NONE); 16-bit
- * rows hold what is beyond their largest number as that number.
+ * z (M, N) or NULL: receives x W^T + bias in the rows' type (ABI 29: gelu and silu of bfloat16 rows in float16, an eighth of the rounding), what the
+ * backward pass of an activation reads (not needed for PAPR_ACT_NONE); what is beyond a 16-bit type's largest number is held as that number.
  * Backward: with d_z = d_y act'(z):  d_x = d_z W (M, K),  d_w = d_z^T x (N, K),  d_b = column sums of d_z (N); each optional (NULL).  d_z of 16-bit rows is held as the sum
  * of two values of their type (none, relu: exact in one).  keep != 0: x is rows kept in 8 bits (papr_rows8_pack; ldx in codes, exps its exponents) and d_w = d_z^T of the
  * values they stand for.  M = 0: the forward call does nothing, the backward call is an error (the gradients are zero: the caller's).

@@ -128,8 +128,8 @@ def linear_rows(x, weight, bias=None, residual=None, act="none", keep=None):
     bfloat16; sums in float32, the result rounded once).  act: none, relu, leakyrelu (slope 0.2), gelu (erf form), silu.
 
     keep = "e4m3" / "int8": in training the rows x are held for the weight's gradient as pack_rows keeps them -- a quarter (float32) or half of the memory -- and that
-    gradient is d_z^T times the values they stand for; y and every other gradient are those of keep=None.  An activation's argument is held in the rows' type for the
-    backward pass; nothing else there is rounded below 32 bits or two values of that type before the gradients themselves are."""
+    gradient is d_z^T times the values they stand for; y and every other gradient are those of keep=None.  An activation's argument is held in 16 bits for the
+    backward pass of 16-bit rows (silu and gelu: float16); nothing else there is rounded below 32 bits or two values of the rows' type before the gradients themselves are."""
     try:
         y = (_native or _load()).linear(x, weight, bias, residual, ACTS.get(act, -1), 0 if keep is None else KEEPS.get(keep, -1))
     except TypeError:

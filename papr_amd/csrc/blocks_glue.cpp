@@ -276,7 +276,8 @@ py::object linear(const Tensor& x, const Tensor& w, const Maybe& b, const Maybe&
     const bool slopes = tracked && act != PAPR_ACT_NONE && (wants_grad(x) || wants_grad(w) || wants_grad(b));
     auto shape = x.sizes().vec();                  // (outputs in their final shape: contiguous, so the same rows)
     shape.back() = N;
-    Tensor y = fresh(rows, shape), z = slopes ? fresh(rows, {d.M, N}) : Tensor();
+    Tensor y = fresh(rows, shape), z;
+    if (slopes) z = at::empty({d.M, N}, rows.options().requires_grad(false).dtype(d.type == PAPR_TYPE_BF16 && (act == PAPR_ACT_GELU || act == PAPR_ACT_SILU) ? at::kHalf : rows.scalar_type()));
     {
         On on(rows);                               // (the workspace's size is the device's)
         const size_t aside = papr_linear_fwd_workspace_bytes_(&d);

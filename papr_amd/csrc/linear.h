@@ -4,6 +4,8 @@
 
 namespace papr_linear {
 
+__host__ __device__ inline bool z_in_f16(int act) { return act == PAPR_ACT_GELU || act == PAPR_ACT_SILU; }       // of bfloat16 rows
+
 struct Operand { const void* p; int64_t ld; int64_t rows; const uint8_t* exps; int64_t low = 0; };       // exps: 8-bit rows only (ld in codes); low: bytes to the second half of a pair
 struct Epilogue {                                  // out and z (M, N) contiguous
     void* out;

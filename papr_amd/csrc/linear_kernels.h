@@ -8,11 +8,13 @@
 //     what is left out (second times third, twice, and third times third) is at most 2^-24 of a term: float32's own rounding.  Summed from the small products up: the first two
 //     parts of the largest number alone add to 2^128, which is infinite.  2.5 PFLOP/s / 6 = 416 TFLOP/s against 157 of the float32 matrix instructions.  The third part of an
 //     infinity is NaN, and so are its products: a result that is NaN is summed again from the values themselves (sum_again).
-//   * z is kept for the backward pass in the rows' type: a slope moves by at most 0.8 of z's rounding, for half (float32: none) of the memory that float32 would take.
+//   * z is kept for the backward pass, which makes a slope of it and nothing else, in the bytes of the rows' type.  A slope moves by at most 0.8 of z's rounding: bfloat16 rows hold gelu's
+//     and silu's z in float16, an eighth of bfloat16's step (its smaller range costs nothing: beyond 65,504 the slopes are their limits, below 2^-14 they move by 2^-25); relu and
+//     leakyrelu look at the sign alone, which float16 loses below 2^-25.
 //   * d_z is an operand of two products.  For 16-bit rows with an activation that bends it (leakyrelu, gelu, silu) it is kept as the sum of two values of the rows' type, high
 //     and low (16 significant bits or more), and both products take both: rounded to one such value it would be an error of the gradients' own rounding's size in each
-//     of them (measured 1.45 times that rounding together, 1.06 so), and a slope up to 1.13 can take it past float16's largest number.  Twice the matrix instructions: 8192 x 1024
-//     -> 4096 in bfloat16, forward and backward, 453 us; with d_z rounded once it was 332.
+//     of them (measured 1.45 times that rounding together; so 1.05 in float16 and 1.00 in bfloat16, which is z's part), and a slope up to 1.13 can take it past float16's largest number.  Twice the matrix instructions: 8192 x 1024
+//     -> 4096 in bfloat16, forward and backward, 450 us; with d_z rounded once it was 332.
 //     d_b sums it in float32.
 #pragma once
 #include "linear.h"
@@ -319,16 +321,21 @@ __device__ __forceinline__ float kept_finite(float z) {
     const float most = largest<T>();
     return z == z ? __builtin_amdgcn_fmed3f(z, -most, most) : z;
 }
+template <typename Z, int E, bool LOOSE>
+__device__ __forceinline__ void put_z(const float (&v)[E], void* z, int64_t at) {
+    papr_pack<Z, E> t;
+#pragma unroll
+    for (int i = 0; i < E; ++i) t.v[i] = (Z)kept_finite<Z>(v[i]);
+    put<Z, E, LOOSE>(reinterpret_cast<Z*>(z) + at, t);
+}
 template <typename T, int OUT, int E, bool LOOSE>
 __device__ __forceinline__ void finish(float (&v)[E], int64_t m, int64_t n, int64_t N, const float (&bias)[E], const papr_pack<T, E>& res, const Epilogue& ep) {
     if (OUT == OUT_FORWARD) {
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] += bias[i];
         if (ep.z) {
-            papr_pack<T, E> t;
-#pragma unroll
-            for (int i = 0; i < E; ++i) t.v[i] = (T)kept_finite<T>(v[i]);
-            put<T, E, LOOSE>(reinterpret_cast<T*>(ep.z) + m * N + n, t);
+            if (__is_same(T, bf16) && z_in_f16(ep.act)) put_z<f16, E, LOOSE>(v, ep.z, m * N + n);
+            else put_z<T, E, LOOSE>(v, ep.z, m * N + n);
         }
         act_values<sizeof(T) == 4>(v, ep.act);
         if (ep.res)
@@ -901,8 +908,8 @@ int join_slabs(const float* slab, int64_t n, int parts, T* out, hipStream_t s) {
 // (float32; relu: d_y or zero), else SPLIT in two values of it: high = d_z rounded and kept finite, low = what is left, rounded (so an infinity stays one in their sum).  Bound by
 // HBM: 512,000 x 256 float32 320 us (4.9 TB/s), 8192 x 4096 bfloat16 in two values 55 (4.9).
 // A thread holds whole vectors of columns; the threads of a workgroup beyond one row's take further rows.
-template <typename T, bool SPLIT, bool VEC>
-__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, int64_t ld, const T* __restrict__ z, int64_t M, int N, int act, int lanes, T* __restrict__ d_z,
+template <typename T, typename Z, bool SPLIT, bool VEC>
+__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, int64_t ld, const Z* __restrict__ z, int64_t M, int N, int act, int lanes, T* __restrict__ d_z,
                                                     T* __restrict__ low, int64_t ldz, float* __restrict__ part, int64_t rows_per_block) {
     constexpr int V = VEC ? 16 / sizeof(T) : 1;
     __shared__ float fold[256 * V];
@@ -923,7 +930,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ d_y, i
         for (int64_t m = beg + rl; m < end; m += per) {
             const auto g = *reinterpret_cast<const papr_pack<T, V>*>(d_y + m * ld + c);
             if (d_z) {
-                const auto t = *reinterpret_cast<const papr_pack<T, V>*>(z + m * N + c);
+                const auto t = *reinterpret_cast<const papr_pack<Z, V>*>(z + m * N + c);
                 float v[V], zv[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) { v[i] = (float)g.v[i]; zv[i] = (float)t.v[i]; }
@@ -1048,13 +1055,16 @@ template <typename T>
 int slopes(bool vec, const SlopeGrid& g, const void* d_y, int64_t ld, const void* z, int64_t M, int N, int act, void* d_z, int64_t low, int64_t ldz, float* part, hipStream_t s) {
     const dim3 grid((unsigned)g.blocks, g.cols);
     T *high = (T*)d_z, *rest = low ? (T*)((char*)d_z + low) : nullptr;
-    if (low) {
-        if (vec) slope_kernel<T, sizeof(T) == 2, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
-        else slope_kernel<T, sizeof(T) == 2, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
-    } else {
-        if (vec) slope_kernel<T, false, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
-        else slope_kernel<T, false, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const T*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
-    }
+    auto launch = [&](auto of, auto split) {
+        typedef decltype(of) Z;
+        constexpr bool SPLIT = decltype(split)::value;
+        if (vec) slope_kernel<T, Z, SPLIT, true><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const Z*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
+        else slope_kernel<T, Z, SPLIT, false><<<grid, 256, 0, s>>>((const T*)d_y, ld, (const Z*)z, M, N, act, g.lanes, high, rest, ldz, part, g.rows_per_block);
+    };
+    if constexpr (sizeof(T) == 4) launch(T(), std::false_type());
+    else if (!low) launch(T(), std::false_type());
+    else if (__is_same(T, bf16) && z_in_f16(act)) launch(f16(), std::true_type());
+    else launch(T(), std::true_type());
     PAPR_CHECK_LAUNCH("papr_linear_bwd");
     return 0;
 }
